@@ -28,6 +28,9 @@ extern "C" {
 
 #define MAD_BF16 0
 #define MAD_F32 1
+/* 8-bit types (see "8-bit operands and checkpoints") */
+#define MAD_E4M3 2
+#define MAD_E5M2 3
 
 int mad_version(void);
 const char* mad_last_error(void);
@@ -432,6 +435,53 @@ int mad_mse_loss_grad(const float* pred, const float* target, float* grad, float
 int mad_adamw_step(float* param, const float* grad, float* m, float* v, float* ema, size_t n, float lr,
                    float beta1, float beta2, float eps, float weight_decay, int step, float grad_scale,
                    float ema_decay, void* stream);
+
+/* ------------------------------------------------------------------ 8-bit operands and checkpoints ---- */
+/* The reference has no 8-bit arithmetic: these entry points extend the training step (activations kept in 8 bits between
+ * forward and backward) and the layers that are matrix products (1x1 convolutions model.py:357-375, Linear.forward
+ * model.py:60-64).
+ *
+ * Format of a tensor of `rows` rows and C columns (all leading dimensions are rows): a row is cut into blocks of 128
+ * columns, the last one possibly shorter.  A block's scale is 2^e with the smallest integer e >= -126 for which the largest
+ * finite magnitude of the block is at most MAX * 2^e (MAX = 448 for MAD_E4M3, 57344 for MAD_E5M2; e = 0 for a block of
+ * zeros); an element is x * 2^-e rounded to nearest even.  NaN stays NaN; an infinity becomes NaN (MAD_E4M3) or stays one
+ * (MAD_E5M2).  A value whose rounding passes the largest fp32 is restored as an infinity.
+ *   q      bytes (rows, P), P = C rounded up to 16, zeros behind column C
+ *   scale  bytes (rows, S), S = ceil(C/128) rounded up to 4, each e + 127; 127 behind the last block
+ * A weight (N, K) has one scale per 128 x 128 block: q (N, ceil16(K)), scale (ceil(N/128), ceil4(ceil(K/128))).
+ * q must be 16-byte aligned, scale 4-byte aligned; C, N, K at most MAD_FP8_MAX_WIDTH; rows may be 0 (nothing is done). */
+#define MAD_FP8_MAX_WIDTH (1 << 20)
+
+/* x (rows, C) in `dtype` -> q, scale in the 8-bit type `fmt`; and back. */
+int mad_pack_fp8(const void* x, int dtype, int fmt, long rows, int C, void* q, void* scale, void* stream);
+int mad_unpack_fp8(const void* q, const void* scale, int fmt, long rows, int C, void* x, int dtype, void* stream);
+
+/* mad_gn_apply / mad_gn_apply_dropout of one source without pooling, y = drop(act(x*a + d)) over x (B, HW, C), that also
+ * packs x (MAD_E4M3) in the same pass: the checkpoint the backward restores x and y from.  Same y, bit for bit.
+ * Restore: x = what q and scale stand for, in `dtype`, and y computed from that x. */
+int mad_gn_apply_save_fp8(const void* x, const float* coef, void* y, void* q, void* scale, int dtype, int B, int HW,
+                          int C, int act, unsigned long long seed, float p, void* stream);
+int mad_gn_apply_restore_fp8(const void* q, const void* scale, const float* coef, void* x, void* y, int dtype, int B,
+                             int HW, int C, int act, unsigned long long seed, float p, void* stream);
+
+/* A weight w (N, K) in `dtype` -> q, scale (MAD_E4M3) and, unless qt and scale_t are NULL, the same bytes transposed:
+ * qt (K, ceil16(N)), scale_t (ceil(K/128), ceil4(ceil(N/128))), the operand of the data gradient. */
+int mad_pack_weight_fp8(const void* w, int dtype, int N, int K, void* q, void* scale, void* qt, void* scale_t,
+                        void* stream);
+
+/* y (rows, N) in `dtype` = x . w^T + bias (+ residual), products summed in fp32, rounded once.  w, w_scale: a packed
+ * weight.  x_type MAD_E4M3 / MAD_E5M2: x and x_scale are packed (rows, K); x_type = dtype: x is (rows, K) in `dtype` and is
+ * rounded to MAD_E4M3 by the same rule on its way in (x_scale ignored).  bias fp32 (N), residual (rows, N), or NULL. */
+int mad_linear_fp8(const void* x, int x_type, const void* x_scale, const void* w, const void* w_scale,
+                   const float* bias, const void* residual, void* y, int dtype, long rows, int K, int N, void* stream);
+
+/* dw (N, K) (+)= dy^T . x and db (N) (+)= column sums of dy (db may be NULL), fp32; x packed (rows, K), dy (rows, N) in
+ * `dtype`, unrounded.  Partial sums are added in a fixed order (deterministic).  The data gradient is mad_linear_fp8 of the
+ * packed dy and the transposed weight. */
+size_t mad_linear_fp8_wgrad_workspace(long rows, int N, int K);
+int mad_linear_fp8_wgrad(const void* dy, int dtype, const void* x, int x_type, const void* x_scale, float* dw, float* db,
+                         void* workspace, size_t workspace_bytes, long rows, int N, int K, int accumulate,
+                         int bias_accumulate, void* stream);
 
 #ifdef __cplusplus
 }

@@ -14,7 +14,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # swapped out from under a later run
 LIB_PATH = os.environ.get("MAD_LIB_PATH") or os.path.join(_HERE, "libmad_hip.so")
 
-MAD_BF16, MAD_F32 = 0, 1
+MAD_BF16, MAD_F32, MAD_E4M3, MAD_E5M2 = 0, 1, 2, 3
+FP8_MAX_WIDTH = 1 << 20                  # MAD_FP8_MAX_WIDTH: columns of a packed tensor
 ALGO_DDPM, ALGO_DDIM = 0, 1
 PRED_EPSILON, PRED_SAMPLE, PRED_V = 0, 1, 2
 OP_STEP, OP_COMPUTE_EPS, OP_INVERSE = 0, 1, 2
@@ -107,6 +108,15 @@ SIGNATURES = {
     "mad_attention": (c_int, [c_void_p, c_void_p] + [c_int] * 4 + [c_void_p]),
     "mad_attention_lse": (c_int, [c_void_p, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p]),
     "mad_attention_bwd": (c_int, [c_void_p] * 6 + [c_int] * 4 + [c_void_p]),
+    "mad_pack_fp8": (c_int, [c_void_p, c_int, c_int, ctypes.c_long, c_int, c_void_p, c_void_p, c_void_p]),
+    "mad_unpack_fp8": (c_int, [c_void_p, c_void_p, c_int, ctypes.c_long, c_int, c_void_p, c_int, c_void_p]),
+    "mad_gn_apply_save_fp8": (c_int, [c_void_p] * 5 + [c_int] * 5 + [ctypes.c_ulonglong, c_float, c_void_p]),
+    "mad_gn_apply_restore_fp8": (c_int, [c_void_p] * 5 + [c_int] * 5 + [ctypes.c_ulonglong, c_float, c_void_p]),
+    "mad_pack_weight_fp8": (c_int, [c_void_p, c_int, c_int, c_int] + [c_void_p] * 5),
+    "mad_linear_fp8": (c_int, [c_void_p, c_int] + [c_void_p] * 6 + [c_int, ctypes.c_long, c_int, c_int, c_void_p]),
+    "mad_linear_fp8_wgrad_workspace": (ctypes.c_size_t, [ctypes.c_long, c_int, c_int]),
+    "mad_linear_fp8_wgrad": (c_int, [c_void_p, c_int, c_void_p, c_int] + [c_void_p] * 4 +
+                             [ctypes.c_size_t, ctypes.c_long] + [c_int] * 4 + [c_void_p]),
 }
 
 

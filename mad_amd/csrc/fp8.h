@@ -1,0 +1,131 @@
+// The 8-bit block format shared by the fp8 kernels.
+//
+// A row of C elements is cut into blocks of 128 (the last one may be shorter).  A block is stored as one byte per
+// element (OCP e4m3 or e5m2) and one scale byte s = e + 127 standing for 2^e, where e is the smallest integer >= -126
+// with amax <= MAX * 2^e and amax is the largest FINITE magnitude of the block (a block without one has e = 0).
+// An element is round_to_nearest_even(x * 2^-e): the product is exact up to underflow far below the smallest 8-bit
+// step, so x is rounded once.  NaN stays NaN; an infinity becomes NaN in e4m3, which has none, and stays one in e5m2.
+// The scale is a power of two because the matrix instruction applies such scales itself (E8M0 operands of
+// v_mfma_scale_f32_16x16x128_f8f6f4, whose reduction length is exactly one block): no multiplication is left for the
+// vector unit, and bf16 holds every restored value exactly (4 significant bits at most).
+// Rows of bytes are padded with zeros to whole 16-byte pieces, rows of scales with 127 to whole groups of four.
+#pragma once
+#include "mma.h"
+
+namespace mad {
+
+constexpr int F8_BLOCK = 128;
+constexpr int F8_E4M3 = 0, F8_E5M2 = 1;      // also the matrix instruction's operand type codes
+
+__host__ __device__ __forceinline__ int f8_pitch(int C) { return (C + 15) & ~15; }
+__host__ __device__ __forceinline__ int f8_blocks(int C) { return (C + F8_BLOCK - 1) / F8_BLOCK; }
+__host__ __device__ __forceinline__ int f8_scale_pitch(int C) { return (f8_blocks(C) + 3) & ~3; }
+
+// packed parts lie where their wide accesses need them
+inline bool f8_aligned(const void* q, const void* scale) { return !((uintptr_t)q & 15) && !((uintptr_t)scale & 3); }
+
+// bits of |x|, 0 for a value that is not finite: their unsigned maximum is the block's amax
+__device__ __forceinline__ unsigned f8_mag(float x) {
+    const unsigned u = __float_as_uint(x) & 0x7fffffffu;
+    return u < 0x7f800000u ? u : 0u;
+}
+
+// scale byte of a block from the bits of its amax: MAX = 1.75 * 2^8 (e4m3), 1.75 * 2^15 (e5m2)
+template <int FMT> __device__ __forceinline__ unsigned f8_scale_byte(unsigned amax) {
+    int s = (int)(amax >> 23) - (FMT == F8_E4M3 ? 8 : 15) + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
+    s = s < 1 ? 1 : s;
+    return amax ? (unsigned)s : 127u;
+}
+__device__ __forceinline__ float f8_scale(unsigned byte) { return __uint_as_float(byte << 23); }            // 2^e
+__device__ __forceinline__ float f8_inv_scale(unsigned byte) { return __uint_as_float((254u - byte) << 23); }  // 2^-e
+
+template <int FMT> __device__ __forceinline__ unsigned f8_cvt4(float a, float b, float c, float d) {
+    int r;
+    if (FMT == F8_E4M3) {
+        r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+        r = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+    } else {
+        r = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, 0, false);
+        r = __builtin_amdgcn_cvt_pk_bf8_f32(c, d, r, true);
+    }
+    return (unsigned)r;
+}
+
+// the four values of one dword, times 2^e
+template <int FMT> __device__ __forceinline__ void f8_values4(unsigned q, float scale, float* f) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    f32x2 lo, hi;
+    if (FMT == F8_E4M3) {
+        lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, false);
+        hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, true);
+    } else {
+        lo = __builtin_amdgcn_cvt_pk_f32_bf8((int)q, false);
+        hi = __builtin_amdgcn_cvt_pk_f32_bf8((int)q, true);
+    }
+    f[0] = lo[0] * scale; f[1] = lo[1] * scale; f[2] = hi[0] * scale; f[3] = hi[1] * scale;
+}
+
+// eight bytes as bf16, unscaled: exact (4 significant bits, exponents far inside bf16's)
+template <int FMT> __device__ __forceinline__ bf16x8 f8_bf16x8(unsigned lo, unsigned hi) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    bf16x2 a, b, c, d;
+    if (FMT == F8_E4M3) {
+        a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false); b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+        c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false); d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+    } else {
+        a = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(lo, 1.0f, false); b = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(lo, 1.0f, true);
+        c = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(hi, 1.0f, false); d = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(hi, 1.0f, true);
+    }
+    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// unsigned maximum over the 16 lanes of a row of lanes (every lane receives it)
+__device__ __forceinline__ unsigned row16_umax(unsigned v) {
+    auto step = [](unsigned a, unsigned b) { return a > b ? a : b; };
+    v = step(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));     // lane ^ 1
+    v = step(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));     // lane ^ 2
+    v = step(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));    // mirror of 8
+    v = step(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));    // mirror of 16
+    return v;
+}
+
+// Eight consecutive elements at any element-aligned address (rows of odd length start anywhere).
+template <typename T> __device__ __forceinline__ void load8(const T* p, float* f);
+template <> __device__ __forceinline__ void load8<bf16_t>(const bf16_t* p, float* f) {
+    typedef unsigned u32x4u __attribute__((ext_vector_type(4), aligned(2)));
+    const u32x4u v = *reinterpret_cast<const u32x4u*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(v[i] << 16); f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u); }
+}
+template <> __device__ __forceinline__ void load8<float>(const float* p, float* f) {
+    typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+    const f32x4u a = reinterpret_cast<const f32x4u*>(p)[0], b = reinterpret_cast<const f32x4u*>(p)[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[i] = a[i]; f[4 + i] = b[i]; }
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, const float* f);
+template <> __device__ __forceinline__ void store8<bf16_t>(bf16_t* p, const float* f) {
+    typedef unsigned u32x4u __attribute__((ext_vector_type(4), aligned(2)));
+    u32x4u v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (unsigned)f32_to_bf16(f[2 * i]) | ((unsigned)f32_to_bf16(f[2 * i + 1]) << 16);
+    *reinterpret_cast<u32x4u*>(p) = v;
+}
+template <> __device__ __forceinline__ void store8<float>(float* p, const float* f) {
+    typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+    reinterpret_cast<f32x4u*>(p)[0] = f32x4u{f[0], f[1], f[2], f[3]};
+    reinterpret_cast<f32x4u*>(p)[1] = f32x4u{f[4], f[5], f[6], f[7]};
+}
+// the same for a piece that may reach past column C (columns behind it read as zero, are not written)
+template <typename T> __device__ __forceinline__ void load8_tail(const T* p, int c, int C, float* f) {
+    if (c + 8 <= C) { load8<T>(p, f); return; }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = c + i < C ? Elem<T>::load(p[i]) : 0.0f;
+}
+template <typename T> __device__ __forceinline__ void store8_tail(T* p, int c, int C, const float* f) {
+    if (c + 8 <= C) { store8<T>(p, f); return; }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) if (c + i < C) p[i] = Elem<T>::store(f[i]);
+}
+
+}  // namespace mad

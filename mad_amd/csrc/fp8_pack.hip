@@ -1,0 +1,328 @@
+// Packing to and from the 8-bit block format (fp8.h): activations, the GroupNorm application that stores or restores
+// its input as an 8-bit checkpoint on the way, and weights.
+//
+// All of it is bound by HBM: pack reads 2 (bf16) or 4 bytes per element and writes one, and so on.  A block of 128
+// channels is the work of 16 lanes with eight elements each, so a block's maximum is a reduction over one row of lanes
+// (four DPP steps), a wave covers four blocks and every access is a whole 16 (bytes: 8) per lane.
+#include "fp8.h"
+
+namespace mad {
+
+// The scale byte of block k of a row; the last block's lanes also write the padding behind it.
+__device__ __forceinline__ void write_scale(unsigned char* row, unsigned s, int k, int kb, int sp, int l) {
+    if (l < (k == kb - 1 ? sp - k : 1)) row[k + l] = (unsigned char)(l ? 127u : s);
+}
+
+// x (rows, C) -> q, scale.  One block per row of 16 lanes; a workgroup strides over the blocks.
+template <typename T, int FMT>
+__global__ __launch_bounds__(256) void pack_fp8_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
+                                                       unsigned char* __restrict__ scale, long rows, int C) {
+    const int kb = f8_blocks(C), pitch = f8_pitch(C), sp = f8_scale_pitch(C);
+    const int l = threadIdx.x & 15;
+    const long stride = (long)gridDim.x * 16;
+    long b = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const long total = rows * kb;
+    const long srow = stride / kb;
+    const int scol = (int)(stride - srow * kb);
+    long row = b / kb;
+    int k = (int)(b - row * kb);
+    for (; b < total; b += stride) {
+        const int c = k * F8_BLOCK + 8 * l;
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = 0.0f;
+        if (c < C) load8_tail<T>(x + row * C + c, c, C, f);
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { const unsigned u = f8_mag(f[i]); m = u > m ? u : m; }
+        const unsigned s = f8_scale_byte<FMT>(row16_umax(m));
+        const float inv = f8_inv_scale(s);
+        if (c < pitch) {
+            uint2 o;
+            o.x = f8_cvt4<FMT>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+            o.y = f8_cvt4<FMT>(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
+            *reinterpret_cast<uint2*>(q + row * pitch + c) = o;
+        }
+        write_scale(scale + row * sp, s, k, kb, sp, l);
+        row += srow; k += scol;
+        if (k >= kb) { k -= kb; ++row; }
+    }
+}
+
+template <typename T, int FMT>
+__global__ __launch_bounds__(256) void unpack_fp8_kernel(const unsigned char* __restrict__ q,
+                                                         const unsigned char* __restrict__ scale, T* __restrict__ x,
+                                                         long rows, int C) {
+    const int kb = f8_blocks(C), pitch = f8_pitch(C), sp = f8_scale_pitch(C);
+    const int l = threadIdx.x & 15;
+    const long stride = (long)gridDim.x * 16;
+    const long total = rows * kb;
+    const long srow = stride / kb;
+    const int scol = (int)(stride - srow * kb);
+    long b = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    long row = b / kb;
+    int k = (int)(b - row * kb);
+    for (; b < total; b += stride) {
+        const int c = k * F8_BLOCK + 8 * l;
+        if (c < C) {
+            const uint2 v = *reinterpret_cast<const uint2*>(q + row * pitch + c);
+            const float s = f8_scale(scale[row * sp + k]);
+            float f[8];
+            f8_values4<FMT>(v.x, s, f);
+            f8_values4<FMT>(v.y, s, f + 4);
+            store8_tail<T>(x + row * C + c, c, C, f);
+        }
+        row += srow; k += scol;
+        if (k >= kb) { k -= kb; ++row; }
+    }
+}
+
+// y = drop(act(x*a + d)) as gn_apply_kernel computes it, and x as an 8-bit checkpoint (SAVE) or restored from one
+// (!SAVE: x is written).  grid (pixel shares, B); a row of 16 lanes keeps its 128 channels, and their (a, d) in
+// registers, over the pixels it walks.
+template <typename T, bool SAVE>
+__global__ __launch_bounds__(256) void gn_fp8_kernel(T* __restrict__ x, const float* __restrict__ coef, T* __restrict__ y,
+                                                     unsigned char* __restrict__ q, unsigned char* __restrict__ scale,
+                                                     int HW, int C, int act, DropMask dm) {
+    const int kb = f8_blocks(C), pitch = f8_pitch(C), sp = f8_scale_pitch(C);
+    const int l = threadIdx.x & 15, grp = threadIdx.x >> 4;
+    const int b = blockIdx.y;
+    const int per = (HW + gridDim.x - 1) / gridDim.x;
+    const int p0 = blockIdx.x * per, p1 = p0 + per < HW ? p0 + per : HW;
+    const int step = kb >= 16 ? 1 : 16 / kb;                  // pixels a workgroup covers per sweep
+    for (int kbase = 0; kbase < kb; kbase += 16) {
+        const int k = kbase + (kb >= 16 ? grp : grp % kb);
+        const int row0 = kb >= 16 ? 0 : grp / kb;
+        if (k >= kb || row0 >= step) continue;
+        const int c = k * F8_BLOCK + 8 * l;
+        float a[8], d[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] = d[i] = 0.0f;
+        if (c < C) {
+            const float* cf = coef + ((size_t)b * C + c) * 2;
+            const int n = C - c < 8 ? C - c : 8;               // 4 (fp32) or 8
+#pragma unroll
+            for (int i = 0; i < 8; i += 2)
+                if (i < n) {
+                    const float4 v = *reinterpret_cast<const float4*>(cf + 2 * i);
+                    a[i] = v.x; d[i] = v.y; a[i + 1] = v.z; d[i + 1] = v.w;
+                }
+        }
+        for (int p = p0 + row0; p < p1; p += step) {
+            const size_t row = (size_t)b * HW + p;
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = 0.0f;
+            if (SAVE) {
+                if (c < C) load8_tail<T>(x + row * C + c, c, C, f);
+                unsigned m = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { const unsigned u = f8_mag(f[i]); m = u > m ? u : m; }
+                const unsigned s = f8_scale_byte<F8_E4M3>(row16_umax(m));
+                const float inv = f8_inv_scale(s);
+                if (c < pitch) {
+                    uint2 o;
+                    o.x = f8_cvt4<F8_E4M3>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+                    o.y = f8_cvt4<F8_E4M3>(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
+                    *reinterpret_cast<uint2*>(q + row * pitch + c) = o;
+                }
+                write_scale(scale + row * sp, s, k, kb, sp, l);
+            } else if (c < C) {
+                const uint2 v = *reinterpret_cast<const uint2*>(q + row * pitch + c);
+                const float s = f8_scale(scale[row * sp + k]);
+                f8_values4<F8_E4M3>(v.x, s, f);
+                f8_values4<F8_E4M3>(v.y, s, f + 4);
+                store8_tail<T>(x + row * C + c, c, C, f);
+                // the activation is that of the restored tensor as it is stored
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[i] = Elem<T>::load(Elem<T>::store(f[i]));
+            }
+            if (c >= C) continue;
+            float r[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float t = fmaf(f[i], a[i], d[i]);
+                r[i] = act ? silu_f(t) : t;
+            }
+            if (dm.thr) {                                     // the linear index of the element in y, as in gn_apply_kernel
+                const unsigned long long e0 = (unsigned long long)row * C + c;
+                float keep[4];
+#pragma unroll
+                for (int h = 0; h < 8; h += 4) {
+                    drop_factors<4>(dm, e0 + h, keep);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) r[h + i] *= keep[i];
+                }
+            }
+            store8_tail<T>(y + row * C + c, c, C, r);
+        }
+    }
+}
+
+// One 128 x 128 block of a weight (N, K) per workgroup: amax, the bytes as they lie, and transposed through LDS.
+template <typename T>
+__global__ __launch_bounds__(256) void pack_weight_fp8_kernel(const T* __restrict__ w, int N, int K,
+                                                              unsigned char* __restrict__ q, unsigned char* __restrict__ scale,
+                                                              unsigned char* __restrict__ qt, unsigned char* __restrict__ scale_t) {
+    __shared__ unsigned red[4];
+    __shared__ __attribute__((aligned(16))) unsigned char tile[128][144];      // [k][n], rows 16 bytes apart in banks
+    const int kbs = f8_scale_pitch(K), nbs = f8_scale_pitch(N);
+    const int nb = blockIdx.x / kbs, kb = blockIdx.x - nb * kbs;
+    const int nblocks = f8_blocks(N), kblocks = f8_blocks(K);
+    const int tid = threadIdx.x, l = tid & 15, r0 = tid >> 4;
+    if (nb >= nblocks || kb >= kblocks) {                     // padding of the scale rows
+        if (tid == 0) {
+            if (nb < nblocks) scale[(size_t)nb * kbs + kb] = 127;
+            if (kb < kblocks && scale_t) scale_t[(size_t)kb * nbs + nb] = 127;
+        }
+        return;
+    }
+    const int c = kb * F8_BLOCK + 8 * l;
+    float f[8][8];
+    unsigned m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int n = nb * F8_BLOCK + r0 + 16 * j;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[j][i] = 0.0f;
+        if (n < N && c < K) load8_tail<T>(w + (size_t)n * K + c, c, K, f[j]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { const unsigned u = f8_mag(f[j][i]); m = u > m ? u : m; }
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) { const unsigned u = __shfl_xor(m, o); m = u > m ? u : m; }
+    if ((tid & 63) == 0) red[tid >> 6] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = red[i] > m ? red[i] : m;
+    const unsigned s = f8_scale_byte<F8_E4M3>(m);
+    const float inv = f8_inv_scale(s);
+    const int kpitch = f8_pitch(K), npitch = f8_pitch(N);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int n = nb * F8_BLOCK + r0 + 16 * j;
+        uint2 o;
+        o.x = f8_cvt4<F8_E4M3>(f[j][0] * inv, f[j][1] * inv, f[j][2] * inv, f[j][3] * inv);
+        o.y = f8_cvt4<F8_E4M3>(f[j][4] * inv, f[j][5] * inv, f[j][6] * inv, f[j][7] * inv);
+        if (n < N && c < kpitch) *reinterpret_cast<uint2*>(q + (size_t)n * kpitch + c) = o;
+        if (qt) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                tile[8 * l + i][r0 + 16 * j] = (unsigned char)(o.x >> (8 * i));
+                tile[8 * l + 4 + i][r0 + 16 * j] = (unsigned char)(o.y >> (8 * i));
+            }
+        }
+    }
+    if (tid == 0) {
+        scale[(size_t)nb * kbs + kb] = (unsigned char)s;
+        if (qt) scale_t[(size_t)kb * nbs + nb] = (unsigned char)s;
+    }
+    if (!qt) return;
+    __syncthreads();
+    const int n = nb * F8_BLOCK + 8 * l;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int k = kb * F8_BLOCK + r0 + 16 * j;
+        if (k < K && n < npitch)
+            *reinterpret_cast<uint2*>(qt + (size_t)k * npitch + n) = *reinterpret_cast<const uint2*>(&tile[r0 + 16 * j][8 * l]);
+    }
+}
+
+// workgroups of 16 blocks each: enough to fill the chip several times, few enough that a workgroup walks many blocks
+static int pack_grid(long blocks) {
+    const long g = (blocks + 15) / 16;
+    return (int)(g < 4096 ? (g > 0 ? g : 1) : 4096);
+}
+
+}  // namespace mad
+
+using namespace mad;
+
+static bool dtype_ok(int d) { return d == MAD_BF16 || d == MAD_F32; }
+
+extern "C" int mad_pack_fp8(const void* x, int dtype, int fmt, long rows, int C, void* q, void* scale, void* stream) {
+    MAD_REQUIRE(dtype_ok(dtype), "mad_pack_fp8: bad dtype %d", dtype);
+    MAD_REQUIRE(fmt == MAD_E4M3 || fmt == MAD_E5M2, "mad_pack_fp8: bad 8-bit type %d", fmt);
+    MAD_REQUIRE(rows >= 0 && C > 0 && C <= MAD_FP8_MAX_WIDTH, "mad_pack_fp8: bad shape %ld x %d", rows, C);
+    if (rows == 0) return 0;
+    MAD_REQUIRE(x && q && scale, "mad_pack_fp8: null pointer");
+    MAD_REQUIRE(f8_aligned(q, scale), "mad_pack_fp8: q must be 16-byte, scale 4-byte aligned");
+    const int grid = pack_grid(rows * f8_blocks(C));
+#define LAUNCH(T, F)                                                                                                 \
+    hipLaunchKernelGGL((pack_fp8_kernel<T, F>), dim3(grid), dim3(256), 0, (hipStream_t)stream, (const T*)x,            \
+                       (unsigned char*)q, (unsigned char*)scale, rows, C)
+    if (dtype == MAD_BF16) { if (fmt == MAD_E4M3) LAUNCH(bf16_t, F8_E4M3); else LAUNCH(bf16_t, F8_E5M2); }
+    else { if (fmt == MAD_E4M3) LAUNCH(float, F8_E4M3); else LAUNCH(float, F8_E5M2); }
+#undef LAUNCH
+    return check_launch("mad_pack_fp8");
+}
+
+extern "C" int mad_unpack_fp8(const void* q, const void* scale, int fmt, long rows, int C, void* x, int dtype, void* stream) {
+    MAD_REQUIRE(dtype_ok(dtype), "mad_unpack_fp8: bad dtype %d", dtype);
+    MAD_REQUIRE(fmt == MAD_E4M3 || fmt == MAD_E5M2, "mad_unpack_fp8: bad 8-bit type %d", fmt);
+    MAD_REQUIRE(rows >= 0 && C > 0 && C <= MAD_FP8_MAX_WIDTH, "mad_unpack_fp8: bad shape %ld x %d", rows, C);
+    if (rows == 0) return 0;
+    MAD_REQUIRE(x && q && scale, "mad_unpack_fp8: null pointer");
+    MAD_REQUIRE(f8_aligned(q, scale), "mad_unpack_fp8: q must be 16-byte, scale 4-byte aligned");
+    const int grid = pack_grid(rows * f8_blocks(C));
+#define LAUNCH(T, F)                                                                                                 \
+    hipLaunchKernelGGL((unpack_fp8_kernel<T, F>), dim3(grid), dim3(256), 0, (hipStream_t)stream,                       \
+                       (const unsigned char*)q, (const unsigned char*)scale, (T*)x, rows, C)
+    if (dtype == MAD_BF16) { if (fmt == MAD_E4M3) LAUNCH(bf16_t, F8_E4M3); else LAUNCH(bf16_t, F8_E5M2); }
+    else { if (fmt == MAD_E4M3) LAUNCH(float, F8_E4M3); else LAUNCH(float, F8_E5M2); }
+#undef LAUNCH
+    return check_launch("mad_unpack_fp8");
+}
+
+template <bool SAVE>
+static int gn_fp8(const char* what, void* x, const float* coef, void* y, void* q, void* scale, int dtype, int B, int HW, int C,
+                  int act, unsigned long long seed, float p, void* stream) {
+    MAD_REQUIRE(dtype_ok(dtype), "%s: bad dtype %d", what, dtype);
+    const int VEC = dtype == MAD_BF16 ? 8 : 4;
+    MAD_REQUIRE(C > 0 && C % VEC == 0 && C <= MAD_FP8_MAX_WIDTH, "%s: channels must be a multiple of %d (C=%d)", what, VEC, C);
+    MAD_REQUIRE(B >= 0 && B <= 65535 && HW >= 0, "%s: bad shape B=%d HW=%d", what, B, HW);
+    MAD_REQUIRE(p >= 0.0f && p < 1.0f, "%s: p=%f out of [0,1)", what, (double)p);
+    if (B == 0 || HW == 0) return 0;
+    MAD_REQUIRE(x && coef && y && q && scale, "%s: null pointer", what);
+    MAD_REQUIRE(f8_aligned(q, scale), "%s: q must be 16-byte, scale 4-byte aligned", what);
+    // pixel shares: about 2048 workgroups in all, at least one sweep of pixels each
+    const int kb = f8_blocks(C), step = kb >= 16 ? 1 : 16 / kb;
+    int shares = (2048 + B - 1) / B;
+    if (shares > (HW + step - 1) / step) shares = (HW + step - 1) / step;
+    const DropMask dm = make_drop_mask(seed, p);
+    if (dtype == MAD_BF16)
+        hipLaunchKernelGGL((gn_fp8_kernel<bf16_t, SAVE>), dim3(shares, B), dim3(256), 0, (hipStream_t)stream, (bf16_t*)x, coef,
+                           (bf16_t*)y, (unsigned char*)q, (unsigned char*)scale, HW, C, act, dm);
+    else
+        hipLaunchKernelGGL((gn_fp8_kernel<float, SAVE>), dim3(shares, B), dim3(256), 0, (hipStream_t)stream, (float*)x, coef,
+                           (float*)y, (unsigned char*)q, (unsigned char*)scale, HW, C, act, dm);
+    return check_launch(what);
+}
+
+extern "C" int mad_gn_apply_save_fp8(const void* x, const float* coef, void* y, void* q, void* scale, int dtype, int B, int HW,
+                                     int C, int act, unsigned long long seed, float p, void* stream) {
+    return gn_fp8<true>("mad_gn_apply_save_fp8", const_cast<void*>(x), coef, y, q, scale, dtype, B, HW, C, act, seed, p, stream);
+}
+
+extern "C" int mad_gn_apply_restore_fp8(const void* q, const void* scale, const float* coef, void* x, void* y, int dtype, int B,
+                                        int HW, int C, int act, unsigned long long seed, float p, void* stream) {
+    return gn_fp8<false>("mad_gn_apply_restore_fp8", x, coef, y, const_cast<void*>(q), const_cast<void*>(scale), dtype, B, HW, C,
+                         act, seed, p, stream);
+}
+
+extern "C" int mad_pack_weight_fp8(const void* w, int dtype, int N, int K, void* q, void* scale, void* qt, void* scale_t,
+                                   void* stream) {
+    MAD_REQUIRE(dtype_ok(dtype), "mad_pack_weight_fp8: bad dtype %d", dtype);
+    MAD_REQUIRE(N > 0 && K > 0 && N <= MAD_FP8_MAX_WIDTH && K <= MAD_FP8_MAX_WIDTH, "mad_pack_weight_fp8: bad shape %d x %d", N, K);
+    MAD_REQUIRE(w && q && scale && (!qt == !scale_t), "mad_pack_weight_fp8: null pointer");
+    MAD_REQUIRE(f8_aligned(q, scale) && f8_aligned(qt, scale_t), "mad_pack_weight_fp8: bytes must be 16-byte, scales 4-byte aligned");
+    // whole groups of four blocks in both directions: their padding is written too
+    const dim3 grid((unsigned)f8_scale_pitch(N) * (unsigned)f8_scale_pitch(K));
+    if (dtype == MAD_BF16)
+        hipLaunchKernelGGL(pack_weight_fp8_kernel<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, (const bf16_t*)w, N, K,
+                           (unsigned char*)q, (unsigned char*)scale, (unsigned char*)qt, (unsigned char*)scale_t);
+    else
+        hipLaunchKernelGGL(pack_weight_fp8_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, (const float*)w, N, K,
+                           (unsigned char*)q, (unsigned char*)scale, (unsigned char*)qt, (unsigned char*)scale_t);
+    return check_launch("mad_pack_weight_fp8");
+}

@@ -6,7 +6,7 @@ stream and returns the output tensor.  Activations are NHWC: shape (B, H, W, C).
 """
 from __future__ import annotations
 
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -772,3 +772,255 @@ def attention_backward(qkv: Tensor, out: Tensor, dout: Tensor, lse: Tensor, head
     if end is not None:
         end.record()
     return dqkv
+
+
+# ------------------------------------------------------------------------------ 8-bit operands and checkpoints
+FP8_BLOCK = 128                          # columns (weights: rows and columns) that share a scale
+_FP8_TYPES = {"e4m3": (torch.float8_e4m3fn, _lib.MAD_E4M3), "e5m2": (torch.float8_e5m2, _lib.MAD_E5M2)}
+_FP8_CODES = {t: c for t, c in _FP8_TYPES.values()}
+
+
+class Fp8Tensor(NamedTuple):
+    """A tensor in 8 bits: every row (last axis) in blocks of 128 columns with a power-of-two scale each.  ``q`` holds the
+    rows as float8_e4m3fn / float8_e5m2, padded with zeros to whole 16 bytes; ``scale`` holds e + 127 of each block's 2^e
+    as uint8, padded with 127 to whole groups of four.  The tensor had ``shape`` and ``dtype``."""
+    q: Tensor
+    scale: Tensor
+    shape: Tuple[int, ...]
+    dtype: torch.dtype
+
+    @property
+    def nbytes(self) -> int:
+        return self.q.numel() + self.scale.numel()
+
+
+class Fp8Weight(NamedTuple):
+    """A weight (N, K) = ``shape`` in float8_e4m3fn with one scale per 128 x 128 block, rows padded as in ``Fp8Tensor``:
+    ``q`` (N, ceil16(K)), ``scale`` (ceil(N/128), ceil4(ceil(K/128))); ``qt`` / ``scale_t`` are the same values transposed,
+    which the data gradient reads."""
+    q: Tensor
+    scale: Tensor
+    shape: Tuple[int, int]
+    qt: Optional[Tensor] = None
+    scale_t: Optional[Tensor] = None
+
+
+def _pitch(c: int) -> int:
+    return (c + 15) & -16
+
+
+def _scale_pitch(c: int) -> int:
+    return (-(-c // FP8_BLOCK) + 3) & -4
+
+
+def _fp8_call(name: str, t: Tensor, *args) -> None:
+    """One entry point on the device of ``t``, on the stream that is current there."""
+    if t.device.index == torch.cuda.current_device():
+        check(getattr(lib, name)(*args, torch.cuda.current_stream().cuda_stream), name)
+        return
+    with torch.cuda.device(t.device):
+        check(getattr(lib, name)(*args, torch.cuda.current_stream().cuda_stream), name)
+
+
+def _fp8_rows(shape: Sequence[int], what: str) -> Tuple[int, int]:
+    if len(shape) < 1 or shape[-1] < 1 or shape[-1] > _lib.FP8_MAX_WIDTH:
+        raise ValueError(f"{what}: needs 1 to {_lib.FP8_MAX_WIDTH} columns, got shape {tuple(shape)}")
+    rows = 1
+    for n in shape[:-1]:
+        rows *= n
+    return rows, shape[-1]
+
+
+def _fp8_empty(rows: int, c: int, fmt: str, device) -> Tuple[Tensor, Tensor]:
+    if fmt not in _FP8_TYPES:
+        raise ValueError(f"unknown 8-bit type {fmt!r}: 'e4m3' or 'e5m2'")
+    return (torch.empty((rows, _pitch(c)), dtype=_FP8_TYPES[fmt][0], device=device),
+            torch.empty((rows, _scale_pitch(c)), dtype=torch.uint8, device=device))
+
+
+def _fp8_check(p: Fp8Tensor, what: str) -> Tuple[int, int, int]:
+    """(rows, columns, type code) of a packed tensor whose parts fit its shape."""
+    rows, c = _fp8_rows(p.shape, what)
+    _dev(p.q, p.scale)
+    if p.q.dtype not in _FP8_CODES or p.scale.dtype != torch.uint8:
+        raise TypeError(f"{what}: a packed tensor is float8_e4m3fn or float8_e5m2 with uint8 scales, got {p.q.dtype} / {p.scale.dtype}")
+    if tuple(p.q.shape) != (rows, _pitch(c)) or tuple(p.scale.shape) != (rows, _scale_pitch(c)):
+        raise ValueError(f"{what}: packed parts {tuple(p.q.shape)} / {tuple(p.scale.shape)} do not belong to shape {tuple(p.shape)}")
+    return rows, c, _FP8_CODES[p.q.dtype]
+
+
+def _fp8_weight_check(q: Optional[Tensor], scale: Optional[Tensor], n: int, k: int, what: str) -> None:
+    if q is None or scale is None:
+        raise ValueError(f"{what}: the weight was packed without its transposed copy")
+    if q.dtype != torch.float8_e4m3fn or scale.dtype != torch.uint8:
+        raise TypeError(f"{what}: a packed weight is float8_e4m3fn with uint8 scales, got {q.dtype} / {scale.dtype}")
+    if tuple(q.shape) != (n, _pitch(k)) or tuple(scale.shape) != (-(-n // FP8_BLOCK), _scale_pitch(k)):
+        raise ValueError(f"{what}: packed parts {tuple(q.shape)} / {tuple(scale.shape)} do not belong to a weight ({n}, {k})")
+
+
+def pack_fp8(x: Tensor, fmt: str = "e4m3") -> Fp8Tensor:
+    """``x`` (..., C) bf16 / fp32 in 8 bits, one power-of-two scale per row and 128 columns (the format: ``Fp8Tensor``).
+    NaN stays NaN and does not count towards its block's scale; an infinity becomes NaN (e4m3) or stays one (e5m2)."""
+    _dev(x)
+    code = _dtype_code(x)
+    rows, c = _fp8_rows(x.shape, "pack_fp8")
+    q, scale = _fp8_empty(rows, c, fmt, x.device)
+    _fp8_call("mad_pack_fp8", x, _ptr(x), code, _FP8_TYPES[fmt][1], rows, c, _ptr(q), _ptr(scale))
+    return Fp8Tensor(q, scale, tuple(x.shape), x.dtype)
+
+
+def unpack_fp8(p: Fp8Tensor) -> Tensor:
+    """The values ``p`` stands for, in the type and shape of the tensor that was packed."""
+    rows, c, fmt = _fp8_check(p, "unpack_fp8")
+    x = torch.empty(p.shape, dtype=p.dtype, device=p.q.device)
+    _fp8_call("mad_unpack_fp8", x, _ptr(p.q), _ptr(p.scale), fmt, rows, c, _ptr(x), _dtype_code(x))
+    return x
+
+
+def _coef_check(coef: Tensor, shape: Sequence[int], what: str) -> None:
+    if len(shape) != 4:
+        raise ValueError(f"{what}: needs an NHWC tensor, got shape {tuple(shape)}")
+    if coef.dtype != torch.float32 or tuple(coef.shape) != (shape[0], shape[3], 2):
+        raise ValueError(f"{what}: coef must be fp32 ({shape[0]}, {shape[3]}, 2), got {coef.dtype} {tuple(coef.shape)}")
+
+
+def gn_apply_save(x: Tensor, coef: Tensor, act: bool, drop_seed: int = 0, drop_p: float = 0.0) -> Tuple[Tensor, Fp8Tensor]:
+    """``gn_apply(x, coef, act, drop_seed=, drop_p=)`` and, from the same pass, ``x`` packed in e4m3: what
+    ``gn_apply_restore`` gives the backward ``x`` and the activation back from."""
+    _dev(x, coef)
+    code = _dtype_code(x)
+    _coef_check(coef, x.shape, "gn_apply_save")
+    B, H, W_, C = x.shape
+    rows, _ = _fp8_rows(x.shape, "gn_apply_save")
+    y = torch.empty_like(x)
+    q, scale = _fp8_empty(rows, C, "e4m3", x.device)
+    _fp8_call("mad_gn_apply_save_fp8", x, _ptr(x), _ptr(coef), _ptr(y), _ptr(q), _ptr(scale), code, B, H * W_, C, int(act),
+              drop_seed, float(drop_p))
+    return y, Fp8Tensor(q, scale, tuple(x.shape), x.dtype)
+
+
+def gn_apply_restore(p: Fp8Tensor, coef: Tensor, act: bool, drop_seed: int = 0, drop_p: float = 0.0) -> Tuple[Tensor, Tensor]:
+    """(x, y): the tensor a checkpoint stands for and ``gn_apply`` of it, in one pass over the 8 bits.  The same ``drop_seed``
+    and ``drop_p`` give the forward's dropout mask."""
+    _, C, fmt = _fp8_check(p, "gn_apply_restore")
+    if fmt != _lib.MAD_E4M3:
+        raise TypeError("gn_apply_restore: checkpoints are e4m3")
+    _coef_check(coef, p.shape, "gn_apply_restore")
+    _dev(p.q, coef)
+    B, H, W_, _ = p.shape
+    x = torch.empty(p.shape, dtype=p.dtype, device=p.q.device)
+    y = torch.empty_like(x)
+    _fp8_call("mad_gn_apply_restore_fp8", x, _ptr(p.q), _ptr(p.scale), _ptr(coef), _ptr(x), _ptr(y), _dtype_code(x), B, H * W_, C,
+              int(act), drop_seed, float(drop_p))
+    return x, y
+
+
+def pack_weight_fp8(w: Tensor, transposed: bool = False) -> Fp8Weight:
+    """A weight (N, K) bf16 / fp32 in e4m3 with one power-of-two scale per 128 x 128 block; ``transposed`` also writes the
+    copy ``linear_fp8_backward`` needs for the data gradient."""
+    _dev(w)
+    code = _dtype_code(w)
+    if w.dim() != 2:
+        raise ValueError(f"pack_weight_fp8: needs a matrix (N, K), got shape {tuple(w.shape)}")
+    N, K = w.shape
+    for n in (N, K):
+        _fp8_rows((1, n), "pack_weight_fp8")
+    new = lambda r, c: torch.empty((r, c), dtype=torch.float8_e4m3fn, device=w.device)
+    scales = lambda r, c: torch.empty((-(-r // FP8_BLOCK), _scale_pitch(c)), dtype=torch.uint8, device=w.device)
+    q, scale = new(N, _pitch(K)), scales(N, K)
+    qt, scale_t = (new(K, _pitch(N)), scales(K, N)) if transposed else (None, None)
+    _fp8_call("mad_pack_weight_fp8", w, _ptr(w), code, N, K, _ptr(q), _ptr(scale), _ptr(qt), _ptr(scale_t))
+    return Fp8Weight(q, scale, (N, K), qt, scale_t)
+
+
+# Rows up to which linear_fp8 rounds x inside the product's own launch: every workgroup rounds the rows it reads again, which
+# costs less than a launch while there are few.
+FP8_FUSED_ROWS = 64
+
+
+def _linear_fp8(x: Union[Tensor, Fp8Tensor], rows: int, k: int, dtype: torch.dtype, q: Tensor, scale: Tensor, n: int,
+                bias: Optional[Tensor], residual: Optional[Tensor], what: str) -> Tensor:
+    """y (rows, n) in ``dtype`` of an x whose parts are checked."""
+    packed = isinstance(x, Fp8Tensor)
+    xq, xs = (x.q, x.scale) if packed else (x, None)
+    _dev(xq, xs, q, scale, bias, residual)
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != n):
+        raise ValueError(f"{what}: bias must be fp32 with {n} elements")
+    y = torch.empty((rows, n), dtype=dtype, device=xq.device)
+    if residual is not None and (residual.dtype != dtype or residual.numel() != y.numel()):
+        raise ValueError(f"{what}: residual must be {dtype} with {y.numel()} elements")
+    code = _dtype_code(y)
+    end = TIMER.bracket("linear_fp8", 2.0 * rows * k * n)
+    _fp8_call("mad_linear_fp8", y, _ptr(xq), _FP8_CODES[xq.dtype] if packed else code, _ptr(xs), _ptr(q), _ptr(scale), _ptr(bias),
+              _ptr(residual), _ptr(y), code, rows, k, n)
+    if end is not None:
+        end.record()
+    return y
+
+
+def linear_fp8(x: Union[Tensor, Fp8Tensor], w: Fp8Weight, bias: Optional[Tensor] = None, residual: Optional[Tensor] = None,
+               save: bool = False):
+    """y (..., N) = x . w^T + bias (+ residual) with both operands in 8 bits and fp32 sums, in the type of ``x``.  ``x``
+    (..., K) is bf16 / fp32, rounded to e4m3 as ``pack_fp8`` does, or already packed.  ``save`` also returns the packed x, which
+    ``linear_fp8_backward`` takes."""
+    N, K = w.shape
+    _fp8_weight_check(w.q, w.scale, N, K, "linear_fp8")
+    if isinstance(x, Fp8Tensor):
+        rows, c, _ = _fp8_check(x, "linear_fp8")
+    else:
+        _dev(x)
+        _dtype_code(x)
+        rows, c = _fp8_rows(x.shape, "linear_fp8")
+    if c != K:
+        raise ValueError(f"linear_fp8: x has {c} columns, the weight {K}")
+    shape, dtype = tuple(x.shape[:-1]) + (N,), x.dtype
+    if residual is not None and tuple(residual.shape) != shape:
+        raise ValueError(f"linear_fp8: residual has shape {tuple(residual.shape)}, y {shape}")
+    if not isinstance(x, Fp8Tensor) and (save or rows > FP8_FUSED_ROWS):
+        x = pack_fp8(x)
+    y = _linear_fp8(x, rows, K, dtype, w.q, w.scale, N, bias, residual, "linear_fp8").view(shape)
+    if not save:
+        return y
+    return y, x
+
+
+def linear_fp8_backward(dy: Tensor, x: Fp8Tensor, w: Optional[Fp8Weight] = None, need_dx: bool = True, grad_fmt: str = "e4m3",
+                        dw: Optional[Tensor] = None, dbias: Optional[Tensor] = None, need_dbias: bool = True,
+                        accumulate: bool = False):
+    """Gradients of ``linear_fp8`` from dy (..., N) and the saved packed input: (dx, dw, dbias).
+
+    dx = Q(dy) . w with dy rounded to ``grad_fmt`` by rows as ``pack_fp8`` does (``w`` packed with its transposed copy);
+    dw = dy^T . x and dbias = column sums of dy in fp32 from the unrounded dy.  ``dw`` / ``dbias`` may be given (fp32, N*K and N
+    elements) and are then overwritten or, with ``accumulate``, added to."""
+    rows, K, fmt = _fp8_check(x, "linear_fp8_backward")
+    _dev(dy, x.q, dw, dbias)
+    code = _dtype_code(dy)
+    if dy.dtype != x.dtype or dy.dim() != len(x.shape) or tuple(dy.shape[:-1]) != tuple(x.shape[:-1]):
+        raise ValueError(f"linear_fp8_backward: dy {dy.dtype} {tuple(dy.shape)} does not belong to x {x.dtype} {tuple(x.shape)}")
+    _, N = _fp8_rows(dy.shape, "linear_fp8_backward")
+    if grad_fmt not in _FP8_TYPES:
+        raise ValueError(f"unknown 8-bit type {grad_fmt!r}: 'e4m3' or 'e5m2'")
+    if accumulate and (dw is None or (need_dbias and dbias is None)):
+        raise ValueError("linear_fp8_backward: accumulate needs dw and dbias to add to")
+    for t, n, what in ((dw, N * K, "dw"), (dbias, N, "dbias")):
+        if t is not None and (t.dtype != torch.float32 or t.numel() != n):
+            raise ValueError(f"linear_fp8_backward: {what} must be fp32 with {n} elements")
+    dx = None
+    if need_dx:
+        if w is None or tuple(w.shape) != (N, K):
+            raise ValueError(f"linear_fp8_backward: dx needs the packed weight ({N}, {K})")
+        _fp8_weight_check(w.qt, w.scale_t, K, N, "linear_fp8_backward")
+        g = pack_fp8(dy, grad_fmt)
+        dx = _linear_fp8(g, rows, N, dy.dtype, w.qt, w.scale_t, K, None, None, "linear_fp8_backward").view(x.shape)
+    if dw is None:
+        dw = torch.empty((N, K), dtype=torch.float32, device=dy.device)
+    if dbias is None and need_dbias:
+        dbias = torch.empty((N,), dtype=torch.float32, device=dy.device)
+    nbytes = lib.mad_linear_fp8_wgrad_workspace(rows, N, K)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dy.device) if nbytes else None
+    end = TIMER.bracket("linear_fp8_wgrad", 2.0 * rows * K * N)
+    _fp8_call("mad_linear_fp8_wgrad", dy, _ptr(dy), code, _ptr(x.q), fmt, _ptr(x.scale), _ptr(dw), _ptr(dbias), _ptr(ws), nbytes,
+              rows, N, K, int(accumulate), int(accumulate))
+    if end is not None:
+        end.record()
+    return dx, dw, dbias
