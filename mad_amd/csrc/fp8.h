@@ -128,4 +128,40 @@ template <typename T> __device__ __forceinline__ void store8_tail(T* p, int c, i
     for (int i = 0; i < 8; ++i) if (c + i < C) p[i] = Elem<T>::store(f[i]);
 }
 
+// four consecutive elements, likewise
+template <typename T> __device__ __forceinline__ void store4_tail(T* p, int c, int C, const f32x4& f) {
+    if (c + 4 <= C) {
+        if constexpr (sizeof(T) == 2) {
+            typedef unsigned u32x2u __attribute__((ext_vector_type(2), aligned(2)));
+            *reinterpret_cast<u32x2u*>(p) = u32x2u{(unsigned)f32_to_bf16(f[0]) | ((unsigned)f32_to_bf16(f[1]) << 16),
+                                                   (unsigned)f32_to_bf16(f[2]) | ((unsigned)f32_to_bf16(f[3]) << 16)};
+        } else {
+            typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+            *reinterpret_cast<f32x4u*>(p) = f;
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) if (c + i < C) p[i] = Elem<T>::store(f[i]);
+}
+template <typename T> __device__ __forceinline__ f32x4 load4_tail(const T* p, int c, int C) {
+    f32x4 f = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (c + 4 <= C) {
+        if constexpr (sizeof(T) == 2) {
+            typedef unsigned u32x2u __attribute__((ext_vector_type(2), aligned(2)));
+            const u32x2u v = *reinterpret_cast<const u32x2u*>(p);
+            f = f32x4{__uint_as_float(v[0] << 16), __uint_as_float(v[0] & 0xffff0000u), __uint_as_float(v[1] << 16),
+                      __uint_as_float(v[1] & 0xffff0000u)};
+        } else {
+            typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+            const f32x4u v = *reinterpret_cast<const f32x4u*>(p);
+            f = f32x4{v[0], v[1], v[2], v[3]};
+        }
+        return f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) if (c + i < C) f[i] = Elem<T>::load(p[i]);
+    return f;
+}
+
 }  // namespace mad

@@ -14,6 +14,8 @@
 //
 // The weights are the FIRST operand, so a lane's four results are four consecutive columns n of one row m.
 #include "fp8.h"
+#include <cstdlib>
+#include <type_traits>
 
 namespace mad {
 
@@ -24,8 +26,7 @@ struct F8LinArgs {
     const unsigned char* w; const unsigned char* ws;
     const float* bias; const void* residual; void* y;
     long M;
-    int K, N, ntiles;
-    int quads;                                     // rows of y are whole quads and every quad is aligned
+    int K, N, mtiles, ntiles;
 };
 
 // kinds of x
@@ -39,33 +40,9 @@ __device__ __forceinline__ i32x8 pair16(const uint4& a, const uint4& b) {
 template <typename TO>
 __device__ __forceinline__ void store_quad(const F8LinArgs& a, long m, int n, f32x4 v) {
     if (m >= a.M || n >= a.N) return;
-    TO* y = (TO*)a.y + m * a.N + n;
-    const TO* r = a.residual ? (const TO*)a.residual + m * a.N + n : nullptr;
-    if (a.quads) {
-        if (a.bias) v += *reinterpret_cast<const f32x4*>(a.bias + n);
-        if constexpr (sizeof(TO) == 4) {
-            if (r) v += *reinterpret_cast<const f32x4*>(r);
-            *reinterpret_cast<f32x4*>(y) = v;
-        } else {
-            if (r) {
-                const uint2 t = *reinterpret_cast<const uint2*>(r);
-                v += f32x4{__uint_as_float(t.x << 16), __uint_as_float(t.x & 0xffff0000u), __uint_as_float(t.y << 16),
-                           __uint_as_float(t.y & 0xffff0000u)};
-            }
-            uint2 o;
-            o.x = (unsigned)f32_to_bf16(v[0]) | ((unsigned)f32_to_bf16(v[1]) << 16);
-            o.y = (unsigned)f32_to_bf16(v[2]) | ((unsigned)f32_to_bf16(v[3]) << 16);
-            *reinterpret_cast<uint2*>(y) = o;
-        }
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (n + e < a.N) {
-            float s = v[e] + (a.bias ? a.bias[n + e] : 0.0f);
-            if (r) s += Elem<TO>::load(r[e]);
-            y[e] = Elem<TO>::store(s);
-        }
+    if (a.bias) v += load4_tail<float>(a.bias + n, n, a.N);
+    if (a.residual) v += load4_tail<TO>((const TO*)a.residual + m * a.N + n, n, a.N);
+    store4_tail<TO>((TO*)a.y + m * a.N + n, n, a.N, v);
 }
 
 // acc += one block of 128 columns, 32 of them in this lane: see "Accuracy" above.
@@ -176,7 +153,173 @@ __global__ __launch_bounds__(64 * NW) void linear_fp8_direct_kernel(F8LinArgs a)
     }
 }
 
-template <int XK, typename TO> static int launch_linear(F8LinArgs a, hipStream_t s) {
+// Tiled form, x packed: a workgroup of WM x WN waves owns BM rows x BN columns of y.
+//   K loop  = one block of 128 columns (128-byte rows of both operands) per step, through NST LDS stages filled by LDS-DMA
+//             NST - 1 steps ahead.  A copy instruction moves 8 rows of 128 bytes; its source is a scalar base (operand,
+//             step) plus one 32-bit offset per lane and row group, kept in registers.
+//   LDS     = 16-byte chunk c of row r lies at c ^ (r >> 1 & 7), and a lane takes chunks g and g + 4 of its row (g = lane / 16):
+//             measured at 5.5 cycles per 1 KiB read with four waves reading, as fast as consecutive addresses; c ^ (r & 7), or
+//             chunks 2g and 2g + 1, take 8.
+//   scales  = a lane's row scales of four steps are one dword, loaded four steps ahead and shifted down a byte per step.
+//   tails   = rows past the end repeat the last row (their results are not stored), chunks past the row come from zeros.
+//   store   = lane pairs exchange quads (v_permlane16_swap), so that a lane writes eight consecutive columns of its row.
+template <int XF, typename TO, int BM, int BN, int WM, int WN, int NST>
+__global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs a) {
+    constexpr int NW = WM * WN, MF = BM / WM / 16, NF = BN / WN / 16;
+    constexpr int XPW = BM / 8 / NW, WPW = BN / 8 / NW;                   // copy instructions per wave and step
+    constexpr int STAGE = (BM + BN) * F8_BLOCK;
+    static_assert(NW % 2 == 0 && BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && NF % 2 == 0 && BN / WN <= F8_BLOCK, "tile");
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    const int r = lane & 15, g = lane >> 4;
+
+    // Order of the tiles: an XCD (workgroups id mod 8) takes a run of consecutive tiles, and runs walk the tiles in
+    // groups of 8 row tiles, down a group before along it, so that the tiles in flight on an XCD share rows of both operands.
+    const int nwg = a.mtiles * a.ntiles, id = blockIdx.x;
+    const int q8 = nwg >> 3, r8 = nwg & 7, xcd = id & 7;
+    const int logical = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (id >> 3);
+    const int per = 8 * a.ntiles, grp = logical / per, in = logical - grp * per;
+    const int gm = a.mtiles - 8 * grp < 8 ? a.mtiles - 8 * grp : 8;
+    // (divisions run on the vector unit: hand the results back to scalar registers, which the copies' bases live in)
+    const int nt = __builtin_amdgcn_readfirstlane(in / gm), mt = __builtin_amdgcn_readfirstlane(8 * grp + in - nt * gm);
+    const long m0 = (long)mt * BM;
+    const int n0 = nt * BN;
+    const int kb = f8_blocks(a.K), pitch = f8_pitch(a.K), sp = f8_scale_pitch(a.K);
+    const int mrem = a.M - m0 < BM ? (int)(a.M - m0) : BM, nrem = a.N - n0 < BN ? a.N - n0 : BN;
+
+    const unsigned char* xbase = (const unsigned char*)a.x + (size_t)m0 * pitch;
+    const unsigned char* wbase = a.w + (size_t)n0 * pitch;
+    // lane of a copy: row lane/8 of its 8 rows, and the chunk that belongs at position lane%8 of that row
+    const int lr = lane >> 3, chunk = (lane & 7) ^ ((4 * wave + (lr >> 1)) & 7);
+    unsigned xoff[XPW], woff[WPW];
+#pragma unroll
+    for (int j = 0; j < XPW; ++j) {
+        const int row = 8 * (j * NW + wave) + lr;
+        xoff[j] = (unsigned)((row < mrem ? row : mrem - 1) * pitch + 16 * chunk);
+    }
+#pragma unroll
+    for (int j = 0; j < WPW; ++j) {
+        const int row = 8 * (j * NW + wave) + lr;
+        woff[j] = (unsigned)((row < nrem ? row : nrem - 1) * pitch + 16 * chunk);
+    }
+    const unsigned lds0 = lds_addr(smem);
+    auto stage = [&](int kt, int buf) {
+        const unsigned xs = lds0 + buf * STAGE + wave * 1024, ws = xs + BM * F8_BLOCK;
+        const int c0 = kt * F8_BLOCK;
+        if (c0 + F8_BLOCK <= pitch) {
+#pragma unroll
+            for (int j = 0; j < XPW; ++j) glds16s(xbase + c0, xoff[j], xs + j * NW * 1024);
+#pragma unroll
+            for (int j = 0; j < WPW; ++j) glds16s(wbase + c0, woff[j], ws + j * NW * 1024);
+        } else {
+            const bool live = c0 + 16 * chunk < pitch;
+#pragma unroll
+            for (int j = 0; j < XPW; ++j) glds16(live ? xbase + c0 + xoff[j] : g_zero_page + 16 * lane, xs + j * NW * 1024);
+#pragma unroll
+            for (int j = 0; j < WPW; ++j) glds16(live ? wbase + c0 + woff[j] : g_zero_page + 16 * lane, ws + j * NW * 1024);
+        }
+    };
+
+    // scales of this lane's rows, four steps to a dword
+    const unsigned char* xsp[MF];
+#pragma unroll
+    for (int i = 0; i < MF; ++i) {
+        const int row = wm * (BM / WM) + 16 * i + r;
+        xsp[i] = a.xs + (size_t)(m0 + (row < mrem ? row : mrem - 1)) * sp;
+    }
+    const int wrow = n0 + wn * (BN / WN) < a.N ? n0 + wn * (BN / WN) : a.N - 1;
+    const unsigned char* wsp = a.ws + (size_t)(wrow / F8_BLOCK) * sp;
+    unsigned xsc[MF], xnext[MF], wsc, wnext;
+    auto load_scales = [&](int kt) {
+#pragma unroll
+        for (int i = 0; i < MF; ++i) xnext[i] = *reinterpret_cast<const unsigned*>(xsp[i] + kt);
+        wnext = *reinterpret_cast<const unsigned*>(wsp + kt);
+    };
+
+    f32x4 acc[MF][NF];
+#pragma unroll
+    for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    // fragment addresses: row r of the wave's rows, chunks g and g + 4 (rows 16 apart share their swizzle)
+    const int c_lo = (g ^ (r >> 1)) << 4, c_hi = c_lo ^ 64;
+    const int xrow = (wm * (BM / WM) + r) * F8_BLOCK, wrow_l = (BM + wn * (BN / WN) + r) * F8_BLOCK;
+
+    load_scales(0);
+#pragma unroll
+    for (int p = 0; p < NST - 1; ++p)
+        if (p < kb) stage(p, p);
+    int buf = 0, fill = NST - 1;
+    for (int kt = 0; kt < kb; ++kt) {
+        if (NST > 2 && kt + NST - 2 < kb) dma_wait_upto<(NST - 2) * (XPW + WPW)>(); else dma_wait_all();
+        __syncthreads();                   // step kt is visible; every wave is done with the stage refilled below
+        if ((kt & 3) == 0) {
+#pragma unroll
+            for (int i = 0; i < MF; ++i) xsc[i] = xnext[i];
+            wsc = wnext;
+            if (kt + 4 < kb) load_scales(kt + 4);
+        }
+        if (kt + NST - 1 < kb) stage(kt + NST - 1, fill);
+        const unsigned char* st = smem + buf * STAGE;
+        i32x8 wf[NF];
+#pragma unroll
+        for (int j = 0; j < NF; ++j) {
+            const unsigned char* p = st + wrow_l + j * 16 * F8_BLOCK;
+            wf[j] = pair16(*reinterpret_cast<const uint4*>(p + c_lo), *reinterpret_cast<const uint4*>(p + c_hi));
+        }
+#pragma unroll
+        for (int i = 0; i < MF; ++i) {
+            const unsigned char* p = st + xrow + i * 16 * F8_BLOCK;
+            const i32x8 xf = pair16(*reinterpret_cast<const uint4*>(p + c_lo), *reinterpret_cast<const uint4*>(p + c_hi));
+#pragma unroll
+            for (int j = 0; j < NF; ++j)
+                block_product<XF, sizeof(TO) == 4>(acc[i][j], wf[j], xf, (int)(wsc & 255u), (int)(xsc[i] & 255u));
+        }
+#pragma unroll
+        for (int i = 0; i < MF; ++i) xsc[i] >>= 8;
+        wsc >>= 8;
+        buf = buf + 1 == NST ? 0 : buf + 1;
+        fill = fill + 1 == NST ? 0 : fill + 1;
+    }
+
+    const int nb = n0 + wn * (BN / WN) + (g & 1) * 16 + (g >> 1) * 8;     // this lane's first column, pair 0
+    float bias[NF / 2][8];
+#pragma unroll
+    for (int p = 0; p < NF / 2; ++p) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) bias[p][e] = 0.0f;
+        if (a.bias && nb + 32 * p < a.N) load8_tail<float>(a.bias + nb + 32 * p, nb + 32 * p, a.N, bias[p]);
+    }
+#pragma unroll
+    for (int i = 0; i < MF; ++i) {
+        const long m = m0 + wm * (BM / WM) + 16 * i + r;
+#pragma unroll
+        for (int p = 0; p < NF / 2; ++p) {
+            const int n = nb + 32 * p;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[i][2 * p][e]),
+                                                                 __float_as_uint(acc[i][2 * p + 1][e]), false, false);
+                v[e] = __uint_as_float(sw[0]) + bias[p][e];
+                v[4 + e] = __uint_as_float(sw[1]) + bias[p][4 + e];
+            }
+            if (m < a.M && n < a.N) {
+                if (a.residual) {
+                    float f[8];
+                    load8_tail<TO>((const TO*)a.residual + m * a.N + n, n, a.N, f);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] += f[e];
+                }
+                store8_tail<TO>((TO*)a.y + m * a.N + n, n, a.N, v);
+            }
+        }
+    }
+}
+
+template <int XK, typename TO> static int launch_direct(F8LinArgs a, hipStream_t s) {
     constexpr int MF = 4, NF = 4, NW = 4;
     const long mtiles = (a.M + 16 * MF - 1) / (16 * MF);
     a.ntiles = (a.N + 16 * NF - 1) / (16 * NF);
@@ -184,6 +327,36 @@ template <int XK, typename TO> static int launch_linear(F8LinArgs a, hipStream_t
                 a.M, a.N);
     hipLaunchKernelGGL((linear_fp8_direct_kernel<XK, TO, MF, NF, NW>), dim3((unsigned)(mtiles * a.ntiles)), dim3(64 * NW), 0, s, a);
     return check_launch("mad_linear_fp8");
+}
+
+template <int XF, typename TO, int BM, int BN, int WM, int WN, int NST> static int launch_tile(F8LinArgs a, hipStream_t s) {
+    constexpr int lds = NST * (BM + BN) * F8_BLOCK;
+    static int lds_dev = -1;
+    auto kernel = &linear_fp8_tile_kernel<XF, TO, BM, BN, WM, WN, NST>;
+    MAD_REQUIRE(raise_lds_limit(reinterpret_cast<const void*>(kernel), lds, &lds_dev),
+                "mad_linear_fp8: cannot raise the dynamic LDS limit to %d", lds);
+    const long mtiles = (a.M + BM - 1) / BM;
+    a.ntiles = (a.N + BN - 1) / BN;
+    MAD_REQUIRE(mtiles * a.ntiles <= 0x7fffffffL, "mad_linear_fp8: %ld rows x %d columns need more workgroups than a launch holds",
+                a.M, a.N);
+    a.mtiles = (int)mtiles;
+    hipLaunchKernelGGL((linear_fp8_tile_kernel<XF, TO, BM, BN, WM, WN, NST>), dim3((unsigned)(mtiles * a.ntiles)), dim3(64 * WM * WN),
+                       lds, s, a);
+    return check_launch("mad_linear_fp8");
+}
+
+template <int XK, typename TO> static int launch_linear(F8LinArgs a, hipStream_t s) {
+    if constexpr (XK < X_BF16) {
+        const char* f = getenv("MAD_F8_TILE");
+        const int w = f ? atoi(f) : 1;
+        if (w == 1) return launch_tile<XK, TO, 256, 256, 2, 4, 2>(a, s);
+        if (w == 2) return launch_tile<XK, TO, 256, 256, 2, 2, 2>(a, s);
+        if (w == 3) return launch_tile<XK, TO, 128, 128, 2, 2, 2>(a, s);
+        if (w == 4) return launch_tile<XK, TO, 256, 128, 4, 2, 3>(a, s);
+        if (w == 5) return launch_tile<XK, TO, 128, 128, 2, 2, 4>(a, s);
+        if (w == 6) return launch_tile<XK, TO, 128, 256, 2, 4, 2>(a, s);
+    }
+    return launch_direct<XK, TO>(a, s);
 }
 
 }  // namespace mad
@@ -205,9 +378,7 @@ extern "C" int mad_linear_fp8(const void* x, int x_type, const void* x_scale, co
                 "mad_linear_fp8: packed bytes must be 16-byte, scales 4-byte aligned");
     F8LinArgs a;
     a.x = x; a.xs = (const unsigned char*)x_scale; a.w = (const unsigned char*)w; a.ws = (const unsigned char*)w_scale;
-    a.bias = bias; a.residual = residual; a.y = y; a.M = rows; a.K = K; a.N = N; a.ntiles = 0;
-    const uintptr_t es = dtype == MAD_BF16 ? 2 : 4;
-    a.quads = N % 4 == 0 && !((uintptr_t)bias & 15) && !(((uintptr_t)residual | (uintptr_t)y) & (4 * es - 1));
+    a.bias = bias; a.residual = residual; a.y = y; a.M = rows; a.K = K; a.N = N; a.mtiles = a.ntiles = 0;
     hipStream_t s = (hipStream_t)stream;
     if (dtype == MAD_BF16) {
         if (x_type == MAD_E4M3) return launch_linear<X_E4M3, bf16_t>(a, s);
