@@ -14,7 +14,6 @@
 //
 // The weights are the FIRST operand, so a lane's four results are four consecutive columns n of one row m.
 #include "fp8.h"
-#include <cstdlib>
 #include <type_traits>
 
 namespace mad {
@@ -153,152 +152,177 @@ __global__ __launch_bounds__(64 * NW) void linear_fp8_direct_kernel(F8LinArgs a)
     }
 }
 
-// Tiled form, x packed: a workgroup of WM x WN waves owns BM rows x BN columns of y.
-//   K loop  = one block of 128 columns (128-byte rows of both operands) per step, through NST LDS stages filled by LDS-DMA
-//             NST - 1 steps ahead.  A copy instruction moves 8 rows of 128 bytes; its source is a scalar base (operand,
-//             step) plus one 32-bit offset per lane and row group, kept in registers.
+// Tiled form, x packed: a workgroup of WM x WN waves owns BM rows x BN columns of y at a time.
+//   K loop  = one block of 128 columns (128-byte rows of both operands) per step, two LDS stages filled by LDS-DMA one step
+//             ahead.  A copy instruction moves 8 rows of 128 bytes.
+//   tiles   = a workgroup walks its share of the tiles as one sequence of steps: the first step of the next tile is copied while
+//             the last step of this one is multiplied, and the results are stored while it lands.
 //   LDS     = 16-byte chunk c of row r lies at c ^ (r >> 1 & 7), and a lane takes chunks g and g + 4 of its row (g = lane / 16):
 //             measured at 5.5 cycles per 1 KiB read with four waves reading, as fast as consecutive addresses; c ^ (r & 7), or
 //             chunks 2g and 2g + 1, take 8.
-//   scales  = a lane's row scales of four steps are one dword, loaded four steps ahead and shifted down a byte per step.
-//   tails   = rows past the end repeat the last row (their results are not stored), chunks past the row come from zeros.
+//   scales  = the bytes of four steps are one dword per row, copied to LDS ahead of them as the operands are (loaded into
+//             registers instead, the wait for them cost 15 % at K = 4096).
 //   store   = lane pairs exchange quads (v_permlane16_swap), so that a lane writes eight consecutive columns of its row.
-template <int XF, typename TO, int BM, int BN, int WM, int WN, int NST>
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// Buffer descriptor of `bytes` bytes from p (both wave-uniform).  A lane whose offset lies outside reads zeros: that takes care of
+// rows past the end, of the tail of a row and of steps that do not exist, without a branch around any copy.
+__device__ __forceinline__ u32x4 f8_buffer(const unsigned char* p, unsigned bytes) {
+    const uintptr_t b = (uintptr_t)p;
+    return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)b),
+                 (unsigned)__builtin_amdgcn_readfirstlane((int)((b >> 32) & 0xffffu)),
+                 (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+}
+constexpr unsigned F8_OUTSIDE = 0xc0000000u;      // a tile's buffer is at most 256 rows of 2^20 bytes; offsets added to this stay outside
+
+// LDS-DMA through a buffer descriptor: 16 (4) bytes per lane to lds_wave_base + 16 (4) * lane; see glds16 for M0
+__device__ __forceinline__ void buf_lds16(const u32x4& buf, unsigned voff, unsigned soff, unsigned lds_wave_base) {
+    asm volatile(
+        "s_mov_b32 m0, %3\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %0, %1, %2 offen lds"
+        :
+        : "v"(voff), "s"(buf), "s"(soff), "s"(lds_wave_base)
+        : "memory", "m0");
+}
+__device__ __forceinline__ void buf_lds4(const u32x4& buf, unsigned voff, unsigned soff, unsigned lds_wave_base) {
+    asm volatile(
+        "s_mov_b32 m0, %3\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dword %0, %1, %2 offen lds"
+        :
+        : "v"(voff), "s"(buf), "s"(soff), "s"(lds_wave_base)
+        : "memory", "m0");
+}
+
+template <int BM, int BN> struct F8Tile {
+    static constexpr int STAGE = (BM + BN) * F8_BLOCK;          // one step of both operands
+    static constexpr int PANEL = BM * 4 + 256;                  // scales of four steps: BM rows, then the weight's row blocks
+    static constexpr int LDS = 2 * STAGE + 2 * PANEL;
+};
+
+template <int XF, typename TO, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs a) {
+    using L = F8Tile<BM, BN>;
     constexpr int NW = WM * WN, MF = BM / WM / 16, NF = BN / WN / 16;
+    constexpr int STORES = MF * NF / 2 * (sizeof(TO) == 2 ? 1 : 2);       // of a wave and a whole tile
     constexpr int XPW = BM / 8 / NW, WPW = BN / 8 / NW;                   // copy instructions per wave and step
-    constexpr int STAGE = (BM + BN) * F8_BLOCK;
-    static_assert(NW % 2 == 0 && BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && NF % 2 == 0 && BN / WN <= F8_BLOCK, "tile");
+    static_assert(NW % 2 == 0 && BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && NF % 2 == 0 && BN / WN <= F8_BLOCK && BM % 64 == 0 &&
+                  BM <= 64 * NW, "tile");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
     const int r = lane & 15, g = lane >> 4;
-
-    // Order of the tiles: an XCD (workgroups id mod 8) takes a run of consecutive tiles, and runs walk the tiles in
-    // groups of 8 row tiles, down a group before along it, so that the tiles in flight on an XCD share rows of both operands.
-    const int nwg = a.mtiles * a.ntiles, id = blockIdx.x;
-    const int q8 = nwg >> 3, r8 = nwg & 7, xcd = id & 7;
-    const int logical = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (id >> 3);
-    const int per = 8 * a.ntiles, grp = logical / per, in = logical - grp * per;
-    const int gm = a.mtiles - 8 * grp < 8 ? a.mtiles - 8 * grp : 8;
-    // (divisions run on the vector unit: hand the results back to scalar registers, which the copies' bases live in)
-    const int nt = __builtin_amdgcn_readfirstlane(in / gm), mt = __builtin_amdgcn_readfirstlane(8 * grp + in - nt * gm);
-    const long m0 = (long)mt * BM;
-    const int n0 = nt * BN;
     const int kb = f8_blocks(a.K), pitch = f8_pitch(a.K), sp = f8_scale_pitch(a.K);
-    const int mrem = a.M - m0 < BM ? (int)(a.M - m0) : BM, nrem = a.N - n0 < BN ? a.N - n0 : BN;
 
-    const unsigned char* xbase = (const unsigned char*)a.x + (size_t)m0 * pitch;
-    const unsigned char* wbase = a.w + (size_t)n0 * pitch;
+    // Order of the tiles: an XCD (workgroups id mod 8) takes a run of consecutive tiles, its workgroups in turn; the run goes
+    // down 8 row tiles before along the columns, so that the tiles in flight on an XCD share rows of both operands.
+    const int ntile = a.mtiles * a.ntiles, xcd = blockIdx.x & 7, nx = (gridDim.x + 7 - xcd) >> 3;
+    const int q8 = ntile >> 3, r8 = ntile & 7;
+    const int first = xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8;
+    const int last = first + q8 + (xcd < r8 ? 1 : 0);
+
     // lane of a copy: row lane/8 of its 8 rows, and the chunk that belongs at position lane%8 of that row
     const int lr = lane >> 3, chunk = (lane & 7) ^ ((4 * wave + (lr >> 1)) & 7);
-    unsigned xoff[XPW], woff[WPW];
-#pragma unroll
-    for (int j = 0; j < XPW; ++j) {
-        const int row = 8 * (j * NW + wave) + lr;
-        xoff[j] = (unsigned)((row < mrem ? row : mrem - 1) * pitch + 16 * chunk);
-    }
-#pragma unroll
-    for (int j = 0; j < WPW; ++j) {
-        const int row = 8 * (j * NW + wave) + lr;
-        woff[j] = (unsigned)((row < nrem ? row : nrem - 1) * pitch + 16 * chunk);
-    }
+    const unsigned off0 = (unsigned)((8 * wave + lr) * pitch + 16 * chunk), rowstep = (unsigned)(8 * NW * pitch);
+    const int tail = pitch - 16 * chunk;             // step offsets below it have this lane's chunk inside the row
     const unsigned lds0 = lds_addr(smem);
-    auto stage = [&](int kt, int buf) {
-        const unsigned xs = lds0 + buf * STAGE + wave * 1024, ws = xs + BM * F8_BLOCK;
-        const int c0 = kt * F8_BLOCK;
-        if (c0 + F8_BLOCK <= pitch) {
+
+    struct Tile { long m0; int n0; u32x4 x, w, xs, ws; };
+    auto open = [&](int t) {
+        const int per = 8 * a.ntiles, grp = t / per, in = t - grp * per;
+        const int gm = a.mtiles - 8 * grp < 8 ? a.mtiles - 8 * grp : 8, col = in / gm;
+        Tile o;
+        // (divisions run on the vector unit: hand the results back to scalar registers)
+        const int nt = __builtin_amdgcn_readfirstlane(col), mt = __builtin_amdgcn_readfirstlane(8 * grp + in - col * gm);
+        o.m0 = (long)mt * BM; o.n0 = nt * BN;
+        const int mrem = a.M - o.m0 < BM ? (int)(a.M - o.m0) : BM, nrem = a.N - o.n0 < BN ? a.N - o.n0 : BN;
+        o.x = f8_buffer((const unsigned char*)a.x + (size_t)o.m0 * pitch, (unsigned)(mrem * pitch));
+        o.w = f8_buffer(a.w + (size_t)o.n0 * pitch, (unsigned)(nrem * pitch));
+        o.xs = f8_buffer(a.xs + (size_t)o.m0 * sp, (unsigned)(mrem * sp));
+        o.ws = f8_buffer(a.ws + (size_t)(o.n0 / F8_BLOCK) * sp, (unsigned)(f8_blocks(nrem) * sp));
+        return o;
+    };
+    // step kt of a tile into a stage, panel p of its scales into a slot
+    auto stage = [&](const Tile& t, int kt, int buf) {
+        const unsigned off = kt * F8_BLOCK < tail ? off0 : F8_OUTSIDE, dst = lds0 + buf * L::STAGE + wave * 1024;
 #pragma unroll
-            for (int j = 0; j < XPW; ++j) glds16s(xbase + c0, xoff[j], xs + j * NW * 1024);
+        for (int j = 0; j < XPW; ++j) buf_lds16(t.x, off + j * rowstep, kt * F8_BLOCK, dst + j * NW * 1024);
 #pragma unroll
-            for (int j = 0; j < WPW; ++j) glds16s(wbase + c0, woff[j], ws + j * NW * 1024);
-        } else {
-            const bool live = c0 + 16 * chunk < pitch;
-#pragma unroll
-            for (int j = 0; j < XPW; ++j) glds16(live ? xbase + c0 + xoff[j] : g_zero_page + 16 * lane, xs + j * NW * 1024);
-#pragma unroll
-            for (int j = 0; j < WPW; ++j) glds16(live ? wbase + c0 + woff[j] : g_zero_page + 16 * lane, ws + j * NW * 1024);
-        }
+        for (int j = 0; j < WPW; ++j) buf_lds16(t.w, off + j * rowstep, kt * F8_BLOCK, dst + BM * F8_BLOCK + j * NW * 1024);
+    };
+    auto panel = [&](const Tile& t, int p, int slot) {
+        const unsigned dst = lds0 + 2 * L::STAGE + slot * L::PANEL;
+        if (64 * wave < BM) buf_lds4(t.xs, (unsigned)((64 * wave + lane) * sp), 4 * p, dst + wave * 256);
+        if (wave == NW - 1) buf_lds4(t.ws, (unsigned)(lane * sp), 4 * p, dst + BM * 4);
     };
 
-    // scales of this lane's rows, four steps to a dword
-    const unsigned char* xsp[MF];
-#pragma unroll
-    for (int i = 0; i < MF; ++i) {
-        const int row = wm * (BM / WM) + 16 * i + r;
-        xsp[i] = a.xs + (size_t)(m0 + (row < mrem ? row : mrem - 1)) * sp;
-    }
-    const int wrow = n0 + wn * (BN / WN) < a.N ? n0 + wn * (BN / WN) : a.N - 1;
-    const unsigned char* wsp = a.ws + (size_t)(wrow / F8_BLOCK) * sp;
-    unsigned xsc[MF], xnext[MF], wsc, wnext;
-    auto load_scales = [&](int kt) {
-#pragma unroll
-        for (int i = 0; i < MF; ++i) xnext[i] = *reinterpret_cast<const unsigned*>(xsp[i] + kt);
-        wnext = *reinterpret_cast<const unsigned*>(wsp + kt);
-    };
+    int t = first + (blockIdx.x >> 3);
+    if (t >= last) return;
+    Tile cur = open(t);
+    int buf = 0, slot = 1;
+    bool counted = false;
+    panel(cur, 0, 0);
+    stage(cur, 0, 0);
 
-    f32x4 acc[MF][NF];
-#pragma unroll
-    for (int i = 0; i < MF; ++i)
-#pragma unroll
-        for (int j = 0; j < NF; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-    // fragment addresses: row r of the wave's rows, chunks g and g + 4 (rows 16 apart share their swizzle)
+    // fragment addresses: row r of the wave's rows (rows 16 apart share their swizzle)
     const int c_lo = (g ^ (r >> 1)) << 4, c_hi = c_lo ^ 64;
-    const int xrow = (wm * (BM / WM) + r) * F8_BLOCK, wrow_l = (BM + wn * (BN / WN) + r) * F8_BLOCK;
+    const int xrow = (wm * (BM / WM) + r) * F8_BLOCK, wrow = (BM + wn * (BN / WN) + r) * F8_BLOCK;
+    const int wblock = wn * (BN / WN) / F8_BLOCK;
 
-    load_scales(0);
+    for (;;) {
+        f32x4 acc[MF][NF];
 #pragma unroll
-    for (int p = 0; p < NST - 1; ++p)
-        if (p < kb) stage(p, p);
-    int buf = 0, fill = NST - 1;
-    for (int kt = 0; kt < kb; ++kt) {
-        if (NST > 2 && kt + NST - 2 < kb) dma_wait_upto<(NST - 2) * (XPW + WPW)>(); else dma_wait_all();
-        __syncthreads();                   // step kt is visible; every wave is done with the stage refilled below
-        if ((kt & 3) == 0) {
+        for (int i = 0; i < MF; ++i)
 #pragma unroll
-            for (int i = 0; i < MF; ++i) xsc[i] = xnext[i];
-            wsc = wnext;
-            if (kt + 4 < kb) load_scales(kt + 4);
+            for (int j = 0; j < NF; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        const int tn = t + nx;
+        const bool more = tn < last;
+        Tile nxt = cur;
+        if (more) nxt = open(tn);
+        for (int kt = 0; kt < kb; ++kt) {
+            // the copies of this step are older than the stores of the tile before
+            if (kt == 0 && counted) dma_wait_upto<STORES>(); else dma_wait_all();
+            __syncthreads();               // this step is visible; every wave is done with the stage and slot refilled below
+            const bool fin = kt + 1 == kb;
+            if ((kt & 3) == 0) {
+                slot ^= 1;
+                if (kt + 4 < kb) panel(cur, (kt >> 2) + 1, slot ^ 1);
+                else if (more) panel(nxt, 0, slot ^ 1);
+            }
+            if (!fin) stage(cur, kt + 1, buf ^ 1);
+            else if (more) stage(nxt, 0, buf ^ 1);
+            const unsigned char* st = smem + buf * L::STAGE;
+            const unsigned char* scp = smem + 2 * L::STAGE + slot * L::PANEL + (kt & 3);
+            const unsigned wsc = scp[BM * 4 + wblock * 4];
+            unsigned xsc[MF];
+#pragma unroll
+            for (int i = 0; i < MF; ++i) xsc[i] = scp[(wm * (BM / WM) + 16 * i + r) * 4];
+            i32x8 wf[NF];
+#pragma unroll
+            for (int j = 0; j < NF; ++j) {
+                const unsigned char* p = st + wrow + j * 16 * F8_BLOCK;
+                wf[j] = pair16(*reinterpret_cast<const uint4*>(p + c_lo), *reinterpret_cast<const uint4*>(p + c_hi));
+            }
+#pragma unroll
+            for (int i = 0; i < MF; ++i) {
+                const unsigned char* p = st + xrow + i * 16 * F8_BLOCK;
+                const i32x8 xf = pair16(*reinterpret_cast<const uint4*>(p + c_lo), *reinterpret_cast<const uint4*>(p + c_hi));
+#pragma unroll
+                for (int j = 0; j < NF; ++j) block_product<XF, sizeof(TO) == 4>(acc[i][j], wf[j], xf, (int)wsc, (int)xsc[i]);
+            }
+            buf ^= 1;
         }
-        if (kt + NST - 1 < kb) stage(kt + NST - 1, fill);
-        const unsigned char* st = smem + buf * STAGE;
-        i32x8 wf[NF];
-#pragma unroll
-        for (int j = 0; j < NF; ++j) {
-            const unsigned char* p = st + wrow_l + j * 16 * F8_BLOCK;
-            wf[j] = pair16(*reinterpret_cast<const uint4*>(p + c_lo), *reinterpret_cast<const uint4*>(p + c_hi));
-        }
-#pragma unroll
-        for (int i = 0; i < MF; ++i) {
-            const unsigned char* p = st + xrow + i * 16 * F8_BLOCK;
-            const i32x8 xf = pair16(*reinterpret_cast<const uint4*>(p + c_lo), *reinterpret_cast<const uint4*>(p + c_hi));
-#pragma unroll
-            for (int j = 0; j < NF; ++j)
-                block_product<XF, sizeof(TO) == 4>(acc[i][j], wf[j], xf, (int)(wsc & 255u), (int)(xsc[i] & 255u));
-        }
-#pragma unroll
-        for (int i = 0; i < MF; ++i) xsc[i] >>= 8;
-        wsc >>= 8;
-        buf = buf + 1 == NST ? 0 : buf + 1;
-        fill = fill + 1 == NST ? 0 : fill + 1;
-    }
 
-    const int nb = n0 + wn * (BN / WN) + (g & 1) * 16 + (g >> 1) * 8;     // this lane's first column, pair 0
-    float bias[NF / 2][8];
-#pragma unroll
-    for (int p = 0; p < NF / 2; ++p) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) bias[p][e] = 0.0f;
-        if (a.bias && nb + 32 * p < a.N) load8_tail<float>(a.bias + nb + 32 * p, nb + 32 * p, a.N, bias[p]);
-    }
-#pragma unroll
-    for (int i = 0; i < MF; ++i) {
-        const long m = m0 + wm * (BM / WM) + 16 * i + r;
+        const int nb = cur.n0 + wn * (BN / WN) + (g & 1) * 16 + (g >> 1) * 8;     // this lane's first column, pair 0
+        float bias[NF / 2][8];
 #pragma unroll
         for (int p = 0; p < NF / 2; ++p) {
-            const int n = nb + 32 * p;
-            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) bias[p][e] = 0.0f;
+            if (a.bias && nb + 32 * p < a.N) load8_tail<float>(a.bias + nb + 32 * p, nb + 32 * p, a.N, bias[p]);
+        }
+        auto piece = [&](int i, int p, float* v) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[i][2 * p][e]),
@@ -306,17 +330,57 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
                 v[e] = __uint_as_float(sw[0]) + bias[p][e];
                 v[4 + e] = __uint_as_float(sw[1]) + bias[p][4 + e];
             }
-            if (m < a.M && n < a.N) {
-                if (a.residual) {
-                    float f[8];
-                    load8_tail<TO>((const TO*)a.residual + m * a.N + n, n, a.N, f);
+        };
+        const long mb = cur.m0 + wm * (BM / WM) + r;
+        // a whole tile without a residual is stored by straight code whose number of stores the next step's wait relies on
+        counted = cur.m0 + BM <= a.M && cur.n0 + BN <= a.N && !a.residual;
+        if (counted) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] += f[e];
+            for (int i = 0; i < MF; ++i)
+#pragma unroll
+                for (int p = 0; p < NF / 2; ++p) {
+                    float v[8];
+                    piece(i, p, v);
+                    TO* y = (TO*)a.y + (mb + 16 * i) * a.N + nb + 32 * p;
+                    store8<TO>(y, v);
                 }
-                store8_tail<TO>((TO*)a.y + m * a.N + n, n, a.N, v);
-            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < MF; ++i)
+#pragma unroll
+                for (int p = 0; p < NF / 2; ++p) {
+                    float v[8];
+                    piece(i, p, v);
+                    const long m = mb + 16 * i;
+                    const int n = nb + 32 * p;
+                    if (m < a.M && n < a.N) {
+                        if (a.residual) {
+                            float f[8];
+                            load8_tail<TO>((const TO*)a.residual + m * a.N + n, n, a.N, f);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) v[e] += f[e];
+                        }
+                        store8_tail<TO>((TO*)a.y + m * a.N + n, n, a.N, v);
+                    }
+                }
         }
+        if (!more) break;
+        t = tn;
+        cur = nxt;
     }
+}
+
+// Compute units of the current device (looked up once per device).
+static int f8_cus() {
+    static int known[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+    if (!known[dev]) {
+        int n = 0;
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1) n = 256;
+        known[dev] = n;
+    }
+    return known[dev];
 }
 
 template <int XK, typename TO> static int launch_direct(F8LinArgs a, hipStream_t s) {
@@ -329,32 +393,31 @@ template <int XK, typename TO> static int launch_direct(F8LinArgs a, hipStream_t
     return check_launch("mad_linear_fp8");
 }
 
-template <int XF, typename TO, int BM, int BN, int WM, int WN, int NST> static int launch_tile(F8LinArgs a, hipStream_t s) {
-    constexpr int lds = NST * (BM + BN) * F8_BLOCK;
+template <int XF, typename TO, int BM, int BN, int WM, int WN> static int launch_tile(F8LinArgs a, hipStream_t s) {
+    constexpr int lds = F8Tile<BM, BN>::LDS, resident = 163840 / lds;
     static int lds_dev = -1;
-    auto kernel = &linear_fp8_tile_kernel<XF, TO, BM, BN, WM, WN, NST>;
+    auto kernel = &linear_fp8_tile_kernel<XF, TO, BM, BN, WM, WN>;
     MAD_REQUIRE(raise_lds_limit(reinterpret_cast<const void*>(kernel), lds, &lds_dev),
                 "mad_linear_fp8: cannot raise the dynamic LDS limit to %d", lds);
     const long mtiles = (a.M + BM - 1) / BM;
     a.ntiles = (a.N + BN - 1) / BN;
-    MAD_REQUIRE(mtiles * a.ntiles <= 0x7fffffffL, "mad_linear_fp8: %ld rows x %d columns need more workgroups than a launch holds",
+    MAD_REQUIRE(mtiles * a.ntiles <= 0x7fffffffL / 8, "mad_linear_fp8: %ld rows x %d columns have more tiles than the kernel counts",
                 a.M, a.N);
     a.mtiles = (int)mtiles;
-    hipLaunchKernelGGL((linear_fp8_tile_kernel<XF, TO, BM, BN, WM, WN, NST>), dim3((unsigned)(mtiles * a.ntiles)), dim3(64 * WM * WN),
-                       lds, s, a);
+    const int tiles = a.mtiles * a.ntiles, grid = f8_cus() * resident;
+    hipLaunchKernelGGL((linear_fp8_tile_kernel<XF, TO, BM, BN, WM, WN>), dim3(tiles < grid ? tiles : grid), dim3(64 * WM * WN), lds, s, a);
     return check_launch("mad_linear_fp8");
 }
 
+// Which form.  Tiles of 256 x 256 need one for every compute unit; with fewer, tiles of 128 x 128 (two workgroups to a unit)
+// keep more of them busy (us, 256 / 128: 4096 x 4096 -> 4096 59 / 64, 4096 x 4096 -> 1024 52 / 26, 16384 x 1024 -> 4096
+// 74 / 84, 16384 x 1024 -> 256 19 / 11).  With fewer than one tile of 128 for each unit the direct form is as fast or
+// faster (1024 x 4096 -> 1024 22 / 24, 64 x 256 -> 4096 4.8 / 5.7; fp32 777 x 1000 -> 328 7 / 15).
 template <int XK, typename TO> static int launch_linear(F8LinArgs a, hipStream_t s) {
     if constexpr (XK < X_BF16) {
-        const char* f = getenv("MAD_F8_TILE");
-        const int w = f ? atoi(f) : 1;
-        if (w == 1) return launch_tile<XK, TO, 256, 256, 2, 4, 2>(a, s);
-        if (w == 2) return launch_tile<XK, TO, 256, 256, 2, 2, 2>(a, s);
-        if (w == 3) return launch_tile<XK, TO, 128, 128, 2, 2, 2>(a, s);
-        if (w == 4) return launch_tile<XK, TO, 256, 128, 4, 2, 3>(a, s);
-        if (w == 5) return launch_tile<XK, TO, 128, 128, 2, 2, 4>(a, s);
-        if (w == 6) return launch_tile<XK, TO, 128, 256, 2, 4, 2>(a, s);
+        const int cus = f8_cus();
+        if (((a.M + 255) / 256) * ((a.N + 255) / 256) >= cus) return launch_tile<XK, TO, 256, 256, 2, 4>(a, s);
+        if (((a.M + 127) / 128) * ((a.N + 127) / 128) >= cus) return launch_tile<XK, TO, 128, 128, 2, 2>(a, s);
     }
     return launch_direct<XK, TO>(a, s);
 }

@@ -227,6 +227,56 @@ def test_linear_of_the_wide_range_type(dev, rows, k, n):
         _close(y, xv @ wv.t() + bias.double(), xv.abs() @ wv.abs().t() + bias.double().abs(), k, dt, _eights(xv, wv))
 
 
+# Sizes that fill the chip with tiles (128 x 128 and 256 x 256), ragged in every direction: rows, K, N.  The operands' values are the
+# packed ones restored on the GPU (compared with the oracle above); product and bounds in fp64 on the GPU, in slices.
+LARGE = [(4100, 272, 1000), (8200, 200, 2050), (33000, 640, 264), (2100, 130, 4100), (16400, 384, 1152), (65, 16, 33000), (70000, 100, 130),
+         (8192, 1152, 2048), (5000, 17, 2303)]
+
+
+def _large_check(got, x, w, extra, extra_size, terms, dtype):
+    for lo in range(0, got.shape[0], 1024):
+        a = x[lo:lo + 1024].double()
+        want, size = a @ w.t(), a.abs() @ w.abs().t()
+        g8 = torch.zeros_like(want)
+        if dtype == torch.bfloat16:
+            for k in range(0, w.shape[1], 8):
+                top = torch.zeros_like(want)
+                for j in range(k, min(k + 8, w.shape[1])):
+                    top = torch.maximum(top, a[:, j, None].abs() * w[None, :, j].abs())
+                g8 += top
+        if extra is not None:
+            want, size = want + extra[lo:lo + 1024], size + extra_size[lo:lo + 1024]
+        tol = (terms + 4) * 2.0 ** -23 * size
+        if dtype == torch.bfloat16:
+            tol = (tol + 7 * 2.0 ** -13 * g8) * (1 + 2.0 ** -8) + 2.0 ** -8 * want.abs() + 2.0 ** -133
+        assert bool(((got[lo:lo + 1024].double() - want).abs() <= tol).all()), f"rows from {lo}"
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,k,n", LARGE)
+def test_linear_over_many_tiles(dev, rows, k, n, dt):
+    from mad_amd import ops
+    g = torch.Generator(device=dev).manual_seed(rows + k + n)
+    rand = lambda *s: torch.randn(s, generator=g, device=dev)
+    x8 = ops.pack_fp8((rand(rows, k) * torch.exp(0.5 * rand(k))).to(dt), "e5m2" if n % 2 else "e4m3")
+    w = rand(n, k) / math.sqrt(k)
+    pw = ops.pack_weight_fp8(w, transposed=True)
+    xv = ops.unpack_fp8(x8)
+    eye = ops.pack_fp8(torch.eye(k, device=dev))
+    wv = ops.linear_fp8(eye, pw).t().double()               # the weight's values: products with 1 and 0 alone are exact
+    _large_check(ops.linear_fp8(x8, pw), xv, wv, None, None, k, dt)
+    bias, res = rand(n), rand(rows, n).to(dt)
+    got = ops.linear_fp8(x8, pw, bias=bias, residual=res)
+    _large_check(got, xv, wv, bias.double() + res.double(), bias.double().abs() + res.double().abs(), k, dt)
+    # nothing behind the last row is written
+    buf = torch.full((rows + 2, n), 7.0, dtype=dt, device=dev)
+    from mad_amd import _lib
+    ops.check(_lib.lib.mad_linear_fp8(x8.q.data_ptr(), ops._FP8_CODES[x8.q.dtype], x8.scale.data_ptr(), pw.q.data_ptr(), pw.scale.data_ptr(),
+                                      bias.data_ptr(), res.data_ptr(), buf.data_ptr(), ops._dtype_code(buf), rows, k, n,
+                                      torch.cuda.current_stream().cuda_stream), "mad_linear_fp8")
+    assert torch.equal(buf[:rows], got) and bool((buf[rows:] == 7.0).all())
+
+
 @pytest.mark.parametrize("rows", [3, 300])
 def test_rows_do_not_touch_each_other(dev, rows):
     """NaN and infinities in one row reach that row of y alone, and zero rows give the bias."""
