@@ -65,16 +65,16 @@ template <int FMT> __device__ __forceinline__ void f8_values4(unsigned q, float 
     f[0] = lo[0] * scale; f[1] = lo[1] * scale; f[2] = hi[0] * scale; f[3] = hi[1] * scale;
 }
 
-// eight bytes as bf16, unscaled: exact (4 significant bits, exponents far inside bf16's)
-template <int FMT> __device__ __forceinline__ bf16x8 f8_bf16x8(unsigned lo, unsigned hi) {
+// eight bytes times a power of two as bf16: exact (4 significant bits)
+template <int FMT> __device__ __forceinline__ bf16x8 f8_bf16x8(unsigned lo, unsigned hi, float scale = 1.0f) {
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
     bf16x2 a, b, c, d;
     if (FMT == F8_E4M3) {
-        a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false); b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
-        c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false); d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+        a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false); b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+        c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false); d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
     } else {
-        a = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(lo, 1.0f, false); b = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(lo, 1.0f, true);
-        c = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(hi, 1.0f, false); d = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(hi, 1.0f, true);
+        a = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(lo, scale, false); b = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(lo, scale, true);
+        c = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(hi, scale, false); d = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(hi, scale, true);
     }
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
@@ -162,6 +162,51 @@ template <typename T> __device__ __forceinline__ f32x4 load4_tail(const T* p, in
 #pragma unroll
     for (int i = 0; i < 4; ++i) if (c + i < C) f[i] = Elem<T>::load(p[i]);
     return f;
+}
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// Buffer descriptor of `bytes` bytes from p (both wave-uniform).  A lane whose offset lies outside reads zeros: that takes care of
+// rows past the end, of the tail of a row and of steps that do not exist, without a branch around any copy.
+__device__ __forceinline__ u32x4 f8_buffer(const unsigned char* p, unsigned bytes) {
+    const uintptr_t b = (uintptr_t)p;
+    return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)b),
+                 (unsigned)__builtin_amdgcn_readfirstlane((int)((b >> 32) & 0xffffu)),
+                 (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+}
+constexpr unsigned F8_OUTSIDE = 0xc0000000u;      // buffers are smaller than 2^31 bytes; what is added to this stays outside
+
+// LDS-DMA through a buffer descriptor: 16 (4) bytes per lane to lds_wave_base + 16 (4) * lane; see glds16 for M0
+__device__ __forceinline__ void buf_lds16(const u32x4& buf, unsigned voff, unsigned soff, unsigned lds_wave_base) {
+    asm volatile(
+        "s_mov_b32 m0, %3\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %0, %1, %2 offen lds"
+        :
+        : "v"(voff), "s"(buf), "s"(soff), "s"(lds_wave_base)
+        : "memory", "m0");
+}
+__device__ __forceinline__ void buf_lds4(const u32x4& buf, unsigned voff, unsigned soff, unsigned lds_wave_base) {
+    asm volatile(
+        "s_mov_b32 m0, %3\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dword %0, %1, %2 offen lds"
+        :
+        : "v"(voff), "s"(buf), "s"(soff), "s"(lds_wave_base)
+        : "memory", "m0");
+}
+
+// Compute units of the current device (looked up once per device).
+inline int f8_cus() {
+    static int known[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+    if (!known[dev]) {
+        int n = 0;
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1) n = 256;
+        known[dev] = n;
+    }
+    return known[dev];
 }
 
 }  // namespace mad

@@ -163,38 +163,6 @@ __global__ __launch_bounds__(64 * NW) void linear_fp8_direct_kernel(F8LinArgs a)
 //   scales  = the bytes of four steps are one dword per row, copied to LDS ahead of them as the operands are (loaded into
 //             registers instead, the wait for them cost 15 % at K = 4096).
 //   store   = lane pairs exchange quads (v_permlane16_swap), so that a lane writes eight consecutive columns of its row.
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-
-// Buffer descriptor of `bytes` bytes from p (both wave-uniform).  A lane whose offset lies outside reads zeros: that takes care of
-// rows past the end, of the tail of a row and of steps that do not exist, without a branch around any copy.
-__device__ __forceinline__ u32x4 f8_buffer(const unsigned char* p, unsigned bytes) {
-    const uintptr_t b = (uintptr_t)p;
-    return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)b),
-                 (unsigned)__builtin_amdgcn_readfirstlane((int)((b >> 32) & 0xffffu)),
-                 (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
-}
-constexpr unsigned F8_OUTSIDE = 0xc0000000u;      // a tile's buffer is at most 256 rows of 2^20 bytes; offsets added to this stay outside
-
-// LDS-DMA through a buffer descriptor: 16 (4) bytes per lane to lds_wave_base + 16 (4) * lane; see glds16 for M0
-__device__ __forceinline__ void buf_lds16(const u32x4& buf, unsigned voff, unsigned soff, unsigned lds_wave_base) {
-    asm volatile(
-        "s_mov_b32 m0, %3\n\t"
-        "s_nop 0\n\t"
-        "buffer_load_dwordx4 %0, %1, %2 offen lds"
-        :
-        : "v"(voff), "s"(buf), "s"(soff), "s"(lds_wave_base)
-        : "memory", "m0");
-}
-__device__ __forceinline__ void buf_lds4(const u32x4& buf, unsigned voff, unsigned soff, unsigned lds_wave_base) {
-    asm volatile(
-        "s_mov_b32 m0, %3\n\t"
-        "s_nop 0\n\t"
-        "buffer_load_dword %0, %1, %2 offen lds"
-        :
-        : "v"(voff), "s"(buf), "s"(soff), "s"(lds_wave_base)
-        : "memory", "m0");
-}
-
 template <int BM, int BN> struct F8Tile {
     static constexpr int STAGE = (BM + BN) * F8_BLOCK;          // one step of both operands
     static constexpr int PANEL = BM * 4 + 256;                  // scales of four steps: BM rows, then the weight's row blocks
@@ -368,19 +336,6 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
         t = tn;
         cur = nxt;
     }
-}
-
-// Compute units of the current device (looked up once per device).
-static int f8_cus() {
-    static int known[64];
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-    if (!known[dev]) {
-        int n = 0;
-        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1) n = 256;
-        known[dev] = n;
-    }
-    return known[dev];
 }
 
 template <int XK, typename TO> static int launch_direct(F8LinArgs a, hipStream_t s) {

@@ -8,6 +8,9 @@
 // products give fp32 accuracy).  Both operands are stored with the reduction index slow and read with the transposing LDS
 // read (ds_read_b64_tr_b16: a row of 16 lanes fetches 4 rows m x 16 columns, lane i receives column i).
 // Shares of the rows write partial sums that a second kernel adds in share order: the result does not depend on timing.
+//
+// db is the gradient of an input column of ones: one more product per fragment of dy.  A workgroup makes it for every
+// ktiles-th step only (kt = step mod ktiles), so that no tile of dw has more work than another; the parts are joined.
 #include "fp8.h"
 
 namespace mad {
@@ -61,7 +64,8 @@ __global__ __launch_bounds__(256) void wgrad_fp8_kernel(F8WgradArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    const bool with_bias = a.db && kt == 0 && wk == 0;        // column sums: the gradient of an input column of ones
+    const bool with_bias = a.db && wk == 0;
+    int turn = 0;                                             // step mod ktiles
     const __bf16 one = (__bf16)1.0f;
     const bf16x8 ones = {one, one, one, one, one, one, one, one};
 
@@ -108,6 +112,8 @@ __global__ __launch_bounds__(256) void wgrad_fp8_kernel(F8WgradArgs a) {
             *reinterpret_cast<uint4*>(dst + NP * TILE) = pack8_bf16(f);
         }
         __syncthreads();
+        const bool mine = with_bias && turn == kt;
+        turn = turn + 1 == a.ktiles ? 0 : turn + 1;
         bf16x8 xf[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) xf[i] = frag(smem + NP * TILE, wk * 64 + 16 * i);
@@ -116,7 +122,7 @@ __global__ __launch_bounds__(256) void wgrad_fp8_kernel(F8WgradArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const bf16x8 d = frag(smem + p * TILE, wn * 64 + 16 * j);
-                if (with_bias) accb[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, d, accb[j], 0, 0, 0);
+                if (mine) accb[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, d, accb[j], 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[i], d, acc[i][j], 0, 0, 0);
             }
@@ -139,29 +145,185 @@ __global__ __launch_bounds__(256) void wgrad_fp8_kernel(F8WgradArgs a) {
                 if (k + e < a.K) p[e] = (direct && a.acc_w ? p[e] : 0.0f) + acc[i][j][e];
         }
         if (with_bias && g == 0) {
-            float* p = a.db + (direct ? 0 : (size_t)split * a.N) + n;
-            *p = (direct && a.acc_b ? *p : 0.0f) + accb[j][0];
+            float* p = a.db + ((size_t)split * a.ktiles + kt) * a.N + n;
+            *p = (a.acc_b ? *p : 0.0f) + accb[j][0];
         }
     }
 }
 
-// dst[i] (+)= sum of the shares' partial sums, in share order
+// Tiled form: dy in bf16 with rows of whole 16-byte pieces.  BN (n) x BK (k) of dw per workgroup of WN x WK waves, 64 rows m per
+// step, two LDS stages.  dy comes by LDS-DMA; x is loaded into registers one step ahead and widened into LDS after the step's
+// products, so that one barrier per step remains.  Columns past the end read what lies there, which only reaches results that
+// are not stored; rows past the share are zeros (buffer loads outside their buffer).
+template <int BN, int BK> struct F8Wg {
+    static constexpr int ROWS = 64, DY = ROWS * BN * 2, STAGE = DY + ROWS * BK * 2, LDS = 2 * STAGE;
+};
+
+template <int FMT, int BN, int BK, int WN, int WK>
+__global__ __launch_bounds__(64 * WN * WK) void wgrad_fp8_tile_kernel(F8WgradArgs a) {
+    using L = F8Wg<BN, BK>;
+    constexpr int NW = WN * WK, FN = BN / WN / 16, FK = BK / WK / 16;
+    constexpr int DPW = BN / 8 / NW;                                      // dy copies per wave and step (4 rows x 128 columns each)
+    constexpr int XPT = 64 * BK / 16 / (64 * NW);                         // 16-byte pieces of x per thread and step
+    static_assert(BN % 128 == 0 && BK % 128 == 0 && BN % (8 * NW) == 0 && XPT * 16 * NW == BK, "tile");
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wn = wave / WK, wk = wave % WK;
+    const int g = lane >> 4, q = (lane >> 2) & 3, pp = lane & 3;
+
+    // an XCD takes a run of consecutive (share, tile): the tiles of a share read the same rows
+    const int tiles = a.ntiles * a.ktiles, nwg = gridDim.x, id = blockIdx.x;
+    const int q8 = nwg >> 3, r8 = nwg & 7, xcd = id & 7;
+    const int logical = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (id >> 3);
+    const int split = __builtin_amdgcn_readfirstlane(logical / tiles), t = logical - split * tiles;
+    const int per = 8 * a.ktiles, grp = t / per, in = t - grp * per;
+    const int gn = a.ntiles - 8 * grp < 8 ? a.ntiles - 8 * grp : 8, col = in / gn;
+    const int kt = __builtin_amdgcn_readfirstlane(col), nt = __builtin_amdgcn_readfirstlane(8 * grp + in - col * gn);
+    const int n0 = nt * BN, k0 = kt * BK;
+    const long m_begin = (long)split * a.per, m_end = m_begin + a.per < a.M ? m_begin + a.per : a.M;
+    const int steps = (int)((m_end - m_begin + L::ROWS - 1) / L::ROWS);
+    const int xp = f8_pitch(a.K), sp = f8_scale_pitch(a.K), kb = f8_blocks(a.K);
+
+    // where this lane's copies read: offsets inside the 64 rows of a step
+    const int lr = lane >> 4;
+    unsigned doff[DPW];
+#pragma unroll
+    for (int j = 0; j < DPW; ++j) {
+        const int c = j * NW + wave;                                      // half c / 16, rows 4 (c % 16) ..
+        doff[j] = (unsigned)((4 * (c & 15) + lr) * a.N * 2 + (n0 + (c >> 4) * 128) * 2 + (((lane & 15) ^ (lr << 2)) << 4));
+    }
+    unsigned xoff[XPT], soff[XPT];
+    int xdst[XPT];
+#pragma unroll
+    for (int u = 0; u < XPT; ++u) {
+        const int i = u * 64 * NW + tid, row = i / (BK / 16), piece = i % (BK / 16), half = piece >> 3;
+        xoff[u] = (unsigned)(row * xp + k0 + 16 * piece);
+        const int block = k0 / F8_BLOCK + half;
+        soff[u] = (unsigned)(row * sp + (block < kb ? block : kb - 1));
+        xdst[u] = L::DY + (half * L::ROWS + row) * 256 + (((2 * (piece & 7)) ^ ((row & 3) << 2)) << 4);
+    }
+    const unsigned lds0 = lds_addr(smem);
+    uint4 xr[XPT];
+    unsigned sr[XPT];
+    auto fetch = [&](int s, int buf) {                                    // step s: dy into its stage, x into registers
+        const long m = m_begin + (long)s * L::ROWS;
+        const int rows = m_end - m < L::ROWS ? (int)(m_end - m) : L::ROWS;
+        const u32x4 db = f8_buffer((const unsigned char*)a.dy + (size_t)m * a.N * 2, (unsigned)(rows * a.N * 2));
+#pragma unroll
+        for (int j = 0; j < DPW; ++j) buf_lds16(db, doff[j], 0, lds0 + buf * L::STAGE + (j * NW + wave) * 1024);
+        const auto xrs = __builtin_amdgcn_make_buffer_rsrc((void*)(a.x + (size_t)m * xp), 0, rows * xp, 0x00020000);
+        const auto srs = __builtin_amdgcn_make_buffer_rsrc((void*)(a.xs + (size_t)m * sp), 0, rows * sp, 0x00020000);
+#pragma unroll
+        for (int u = 0; u < XPT; ++u) {
+            xr[u] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(xrs, (int)xoff[u], 0, 0));
+            sr[u] = (unsigned char)__builtin_amdgcn_raw_buffer_load_b8(srs, (int)soff[u], 0, 0);
+        }
+    };
+    auto widen = [&](int buf) {                                           // the fetched x into the stage
+#pragma unroll
+        for (int u = 0; u < XPT; ++u) {
+            const float s = f8_scale(sr[u]);
+            unsigned char* d = smem + buf * L::STAGE;
+            *reinterpret_cast<bf16x8*>(d + xdst[u]) = f8_bf16x8<FMT>(xr[u].x, xr[u].y, s);
+            *reinterpret_cast<bf16x8*>(d + (xdst[u] ^ 16)) = f8_bf16x8<FMT>(xr[u].z, xr[u].w, s);
+        }
+    };
+
+    f32x4 acc[FK][FN], accb[FN];                              // [k fragment][n fragment]
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        accb[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < FK; ++i) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const __bf16 one = (__bf16)1.0f;
+    const bf16x8 ones = {one, one, one, one, one, one, one, one};
+    const bool with_bias = a.db && wk == 0;
+    int turn = 0;
+
+    // fragment of 16 columns: rows 4g + q and 16 rows on, 8 bytes at columns 4 pp
+    const int frow = (4 * g + q) * 256 + (pp & 1) * 8;
+    auto frag = [&](const unsigned char* tile, int c, int h) {
+        const int chunk = ((c & 127) >> 3) + (pp >> 1);
+        const unsigned char* p = tile + (c >> 7) * L::ROWS * 256 + h * 32 * 256 + frow + ((chunk ^ (q << 2)) << 4);
+        return tr_pair(p, p + 16 * 256);
+    };
+
+    if (steps > 0) { fetch(0, 0); widen(0); }
+    for (int s = 0; s < steps; ++s) {
+        const int buf = s & 1;
+        dma_wait_all();
+        __syncthreads();                   // step s is visible; every wave is done with the stage refilled below
+        if (s + 1 < steps) fetch(s + 1, buf ^ 1);
+        const bool mine = with_bias && turn == kt;
+        turn = turn + 1 == a.ktiles ? 0 : turn + 1;
+        const unsigned char* st = smem + buf * L::STAGE;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            bf16x8 xf[FK];
+#pragma unroll
+            for (int i = 0; i < FK; ++i) xf[i] = frag(st + L::DY, wk * (BK / WK) + 16 * i, h);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                const bf16x8 d = frag(st, wn * (BN / WN) + 16 * j, h);
+                if (mine) accb[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, d, accb[j], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < FK; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[i], d, acc[i][j], 0, 0, 0);
+            }
+        }
+        if (s + 1 < steps) widen(buf ^ 1);
+    }
+
+    // a lane holds four consecutive k of one n
+    const bool direct = a.splits == 1;
+    float* dw = a.dw + (direct ? 0 : (size_t)split * a.N * a.K);
+    const int r = lane & 15;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const int n = n0 + wn * (BN / WN) + 16 * j + r;
+        if (n >= a.N) continue;
+#pragma unroll
+        for (int i = 0; i < FK; ++i) {
+            const int k = k0 + wk * (BK / WK) + 16 * i + 4 * g;
+            if (k >= a.K) continue;
+            float* p = dw + (size_t)n * a.K + k;
+            f32x4 v = acc[i][j];
+            if (direct && a.acc_w) v += load4_tail<float>(p, k, a.K);
+            store4_tail<float>(p, k, a.K, v);
+        }
+        if (with_bias && g == 0) {
+            float* p = a.db + ((size_t)split * a.ktiles + kt) * a.N + n;
+            *p = (a.acc_b ? *p : 0.0f) + accb[j][0];
+        }
+    }
+}
+
+// dst[i] (+)= sum of the parts' partial sums, in order
 __global__ __launch_bounds__(256) void wgrad_fp8_join_kernel(const float* __restrict__ part, float* __restrict__ dst, size_t n,
-                                                             int splits, int accumulate) {
+                                                             int parts, int accumulate) {
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
         float s = 0.0f;
-        for (int z = 0; z < splits; ++z) s += part[(size_t)z * n + i];
+        for (int z = 0; z < parts; ++z) s += part[(size_t)z * n + i];
         dst[i] = accumulate ? dst[i] + s : s;
     }
 }
 
-// Shares of the rows: enough workgroups to fill the chip, at least 256 rows each.
-static int wgrad_splits(long rows, int N, int K) {
-    const long tiles = (long)((N + 127) / 128) * ((K + 127) / 128);
-    long s = (512 + tiles - 1) / tiles;
+// How a gradient is cut: the form, its tiles and the shares of the rows.
+struct F8WgradPlan { int tile, ntiles, ktiles, splits; long per; };
+
+static F8WgradPlan wgrad_plan(long rows, int N, int K, bool tiled) {
+    F8WgradPlan p;
+    auto tiles = [&](int t) { return (long)((N + t - 1) / t) * ((K + t - 1) / t); };
+    const int cus = f8_cus();
+    p.tile = tiled && tiles(256) >= cus ? 256 : 128;
+    p.ntiles = (N + p.tile - 1) / p.tile; p.ktiles = (K + p.tile - 1) / p.tile;
+    long s = (2 * cus + tiles(p.tile) - 1) / tiles(p.tile);
+    if (p.tile == 256) s = 1;
     const long most = (rows + 255) / 256;
     if (s > most) s = most;
-    return (int)(s < 1 ? 1 : s);
+    p.splits = (int)(s < 1 ? 1 : s);
+    p.per = ((rows + p.splits - 1) / p.splits + 63) / 64 * 64;
+    return p;
 }
 
 }  // namespace mad
@@ -172,10 +334,31 @@ static bool wgrad_shape_ok(long rows, int N, int K) {
     return rows >= 0 && N > 0 && N <= MAD_FP8_MAX_WIDTH && K > 0 && K <= MAD_FP8_MAX_WIDTH;
 }
 
+static size_t wgrad_workspace(const F8WgradPlan& p, int N, int K) {
+    const size_t w = p.splits > 1 ? (size_t)p.splits * N * K : 0;
+    const size_t b = (size_t)p.splits * p.ktiles > 1 ? (size_t)p.splits * p.ktiles * N : 0;
+    return (w + b) * sizeof(float);
+}
+
+// the form with LDS-DMA of dy needs whole 16-byte pieces, and 64 rows within a buffer's 32-bit offsets
+static bool wgrad_tiled(const void* dy, int dtype, int N) {
+    return dtype == MAD_BF16 && N % 8 == 0 && !((uintptr_t)dy & 15);
+}
+
 extern "C" size_t mad_linear_fp8_wgrad_workspace(long rows, int N, int K) {
     if (!wgrad_shape_ok(rows, N, K)) return 0;
-    const int s = wgrad_splits(rows, N, K);
-    return s > 1 ? (size_t)s * ((size_t)N * K + N) * sizeof(float) : 0;
+    const size_t a = wgrad_workspace(wgrad_plan(rows, N, K, true), N, K), b = wgrad_workspace(wgrad_plan(rows, N, K, false), N, K);
+    return a > b ? a : b;                       // whichever form the operands' alignment allows
+}
+
+template <int FMT, int T, int WN, int WK> static int launch_wgrad_tile(const F8WgradArgs& a, unsigned wgs, hipStream_t s) {
+    constexpr int lds = F8Wg<T, T>::LDS;
+    static int lds_dev = -1;
+    auto kernel = &wgrad_fp8_tile_kernel<FMT, T, T, WN, WK>;
+    MAD_REQUIRE(raise_lds_limit(reinterpret_cast<const void*>(kernel), lds, &lds_dev),
+                "mad_linear_fp8_wgrad: cannot raise the dynamic LDS limit to %d", lds);
+    hipLaunchKernelGGL((wgrad_fp8_tile_kernel<FMT, T, T, WN, WK>), dim3(wgs), dim3(64 * WN * WK), lds, s, a);
+    return check_launch("mad_linear_fp8_wgrad");
 }
 
 extern "C" int mad_linear_fp8_wgrad(const void* dy, int dtype, const void* x, int x_type, const void* x_scale, float* dw, float* db,
@@ -186,36 +369,45 @@ extern "C" int mad_linear_fp8_wgrad(const void* dy, int dtype, const void* x, in
     MAD_REQUIRE(wgrad_shape_ok(rows, N, K), "mad_linear_fp8_wgrad: bad shape rows=%ld N=%d K=%d", rows, N, K);
     MAD_REQUIRE(dw && (rows == 0 || (dy && x && x_scale)), "mad_linear_fp8_wgrad: null pointer");
     MAD_REQUIRE(f8_aligned(x, x_scale), "mad_linear_fp8_wgrad: x must be 16-byte, its scales 4-byte aligned");
-    F8WgradArgs a;
-    a.dy = dy; a.x = (const unsigned char*)x; a.xs = (const unsigned char*)x_scale;
-    a.M = rows; a.N = N; a.K = K;
-    a.splits = wgrad_splits(rows, N, K);
     const size_t need = mad_linear_fp8_wgrad_workspace(rows, N, K);
     MAD_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "mad_linear_fp8_wgrad: workspace of %zu bytes, %zu needed",
                 workspace_bytes, need);
-    a.per = ((rows + a.splits - 1) / a.splits + 31) / 32 * 32;
-    a.ntiles = (N + 127) / 128; a.ktiles = (K + 127) / 128;
-    a.acc_w = accumulate; a.acc_b = bias_accumulate;
-    const size_t nk = (size_t)N * K;
-    float* part_b = a.splits > 1 ? (float*)workspace + (size_t)a.splits * nk : nullptr;
-    a.dw = a.splits > 1 ? (float*)workspace : dw;
-    a.db = db ? (a.splits > 1 ? part_b : db) : nullptr;
-    const long wgs = (long)a.ntiles * a.ktiles * a.splits;
+    const bool tiled = wgrad_tiled(dy, dtype, N);
+    const F8WgradPlan p = wgrad_plan(rows, N, K, tiled);
+    const long wgs = (long)p.ntiles * p.ktiles * p.splits;
     MAD_REQUIRE(wgs <= 0x7fffffffL, "mad_linear_fp8_wgrad: N=%d K=%d need more workgroups than a launch holds", N, K);
+    const size_t nk = (size_t)N * K;
+    const bool join_w = p.splits > 1, join_b = db && (size_t)p.splits * p.ktiles > 1;
+    float* part_w = (float*)workspace;
+    float* part_b = part_w + (join_w ? (size_t)p.splits * nk : 0);
+    F8WgradArgs a;
+    a.dy = dy; a.x = (const unsigned char*)x; a.xs = (const unsigned char*)x_scale;
+    a.dw = join_w ? part_w : dw;
+    a.db = join_b ? part_b : db;
+    a.M = rows; a.per = p.per; a.N = N; a.K = K;
+    a.ntiles = p.ntiles; a.ktiles = p.ktiles; a.splits = p.splits;
+    a.acc_w = accumulate; a.acc_b = !join_b && bias_accumulate;
     hipStream_t s = (hipStream_t)stream;
+    int rc;
+    if (tiled && p.tile == 256)
+        rc = x_type == MAD_E4M3 ? launch_wgrad_tile<F8_E4M3, 256, 2, 4>(a, (unsigned)wgs, s) : launch_wgrad_tile<F8_E5M2, 256, 2, 4>(a, (unsigned)wgs, s);
+    else if (tiled)
+        rc = x_type == MAD_E4M3 ? launch_wgrad_tile<F8_E4M3, 128, 2, 2>(a, (unsigned)wgs, s) : launch_wgrad_tile<F8_E5M2, 128, 2, 2>(a, (unsigned)wgs, s);
+    else {
 #define LAUNCH(T, F) hipLaunchKernelGGL((wgrad_fp8_kernel<T, F>), dim3((unsigned)wgs), dim3(256), 0, s, a)
-    if (dtype == MAD_BF16) { if (x_type == MAD_E4M3) LAUNCH(bf16_t, F8_E4M3); else LAUNCH(bf16_t, F8_E5M2); }
-    else { if (x_type == MAD_E4M3) LAUNCH(float, F8_E4M3); else LAUNCH(float, F8_E5M2); }
+        if (dtype == MAD_BF16) { if (x_type == MAD_E4M3) LAUNCH(bf16_t, F8_E4M3); else LAUNCH(bf16_t, F8_E5M2); }
+        else { if (x_type == MAD_E4M3) LAUNCH(float, F8_E4M3); else LAUNCH(float, F8_E5M2); }
 #undef LAUNCH
-    if (int rc = check_launch("mad_linear_fp8_wgrad")) return rc;
-    if (a.splits > 1) {
+        rc = check_launch("mad_linear_fp8_wgrad");
+    }
+    if (rc) return rc;
+    if (join_w) {
         const size_t blocks = (nk + 255) / 256;
         hipLaunchKernelGGL(wgrad_fp8_join_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s,
-                           (const float*)workspace, dw, nk, a.splits, accumulate);
-        if (db)
-            hipLaunchKernelGGL(wgrad_fp8_join_kernel, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, s, (const float*)part_b, db,
-                               (size_t)N, a.splits, bias_accumulate);
-        return check_launch("mad_linear_fp8_wgrad");
+                           (const float*)part_w, dw, nk, p.splits, accumulate);
     }
-    return 0;
+    if (join_b)
+        hipLaunchKernelGGL(wgrad_fp8_join_kernel, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, s, (const float*)part_b, db,
+                           (size_t)N, p.splits * p.ktiles, bias_accumulate);
+    return join_w || join_b ? check_launch("mad_linear_fp8_wgrad") : 0;
 }

@@ -406,6 +406,35 @@ def test_linear_backward(dev, rows, k, n, fmt, dt):
     assert none is None and nodb is None and torch.equal(dw2, dw)
 
 
+# rows, K, N: many shares of the rows, tiles of 128 and of 256, ragged in every direction, rows of dy that are no whole 16 bytes
+WGRAD_LARGE = [(66000, 272, 136), (333, 4000, 4104), (20001, 384, 1152), (5000, 16, 8), (3000, 1040, 131), (64, 4096, 4096), (129, 130, 264)]
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,k,n", WGRAD_LARGE)
+def test_weight_gradient_over_many_tiles(dev, rows, k, n, dt):
+    from mad_amd import ops
+    g = torch.Generator(device=dev).manual_seed(rows + k + n)
+    rand = lambda *s: torch.randn(s, generator=g, device=dev)
+    dy = (1e-3 * rand(rows, n) * torch.exp(rand(rows, 1))).to(dt)
+    x8 = ops.pack_fp8((rand(rows, k) * torch.exp(2 * rand(rows, 1))).to(dt), "e5m2" if rows % 2 else "e4m3")
+    xv, gd = ops.unpack_fp8(x8).double(), dy.double()
+    _, dw, db = ops.linear_fp8_backward(dy, x8, need_dx=False)
+    within = lambda got, want, size: bool(((got.double() - want).abs() <= (rows + 4) * 2.0 ** -23 * size).all())
+    want, size = gd.t() @ xv, gd.abs().t() @ xv.abs()
+    assert within(dw, want, size) and within(db, gd.sum(0), gd.abs().sum(0))
+    again = ops.linear_fp8_backward(dy, x8, need_dx=False)
+    assert torch.equal(again[1], dw) and torch.equal(again[2], db)
+    base, bb = torch.full((n + 1, k), 0.5, device=dev), torch.full((n + 1,), 0.25, device=dev)
+    ops.linear_fp8_backward(dy, x8, need_dx=False, dw=base[:n], dbias=bb[:n], accumulate=True)
+    assert within(base[:n], want + 0.5, size + 0.5) and within(bb[:n], gd.sum(0) + 0.25, gd.abs().sum(0) + 0.25)
+    assert bool((base[n] == 0.5).all()) and float(bb[n]) == 0.25
+    # dy anywhere in memory: the form that does not need whole pieces
+    off = torch.cat([dy.flatten()[:1], dy.flatten()])[1:].view(rows, n)
+    _, dw, db = ops.linear_fp8_backward(off, x8, need_dx=False)
+    assert within(dw, want, size) and within(db, gd.sum(0), gd.abs().sum(0))
+
+
 @pytest.mark.parametrize("dt", DTYPES)
 def test_gradients_against_differences(dev, dt):
     """On small whole numbers every rounding of the operator is exact, so <g, y> is linear in x, w and the bias and differences of it
