@@ -174,8 +174,11 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
     using L = F8Tile<BM, BN>;
     constexpr int NW = WM * WN, MF = BM / WM / 16, NF = BN / WN / 16;
     constexpr int STORES = MF * NF / 2 * (sizeof(TO) == 2 ? 1 : 2);       // of a wave and a whole tile
-    constexpr int XPW = BM / 8 / NW, WPW = BN / 8 / NW;                   // copy instructions per wave and step
-    static_assert(NW % 2 == 0 && BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && NF % 2 == 0 && BN / WN <= F8_BLOCK && BM % 64 == 0 &&
+    // Copies are issued by one wave of each SIMD (CW of them): a wave sits in a copy's issue for longer than in a product's, and
+    // meanwhile the SIMD's other wave multiplies (16384 x 4096 -> 8192: 489 us with all eight waves copying, 463 with four)
+    constexpr int CW = NW == 8 ? 4 : NW;
+    constexpr int XPW = BM / 8 / CW, WPW = BN / 8 / CW;                   // copy instructions per copying wave and step
+    static_assert(CW % 2 == 0 && BM % (8 * CW) == 0 && BN % (8 * CW) == 0 && NF % 2 == 0 && BN / WN <= F8_BLOCK && BM % 64 == 0 &&
                   BM <= 64 * NW, "tile");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -192,7 +195,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
 
     // lane of a copy: row lane/8 of its 8 rows, and the chunk that belongs at position lane%8 of that row
     const int lr = lane >> 3, chunk = (lane & 7) ^ ((4 * wave + (lr >> 1)) & 7);
-    const unsigned off0 = (unsigned)((8 * wave + lr) * pitch + 16 * chunk), rowstep = (unsigned)(8 * NW * pitch);
+    const unsigned off0 = (unsigned)((8 * wave + lr) * pitch + 16 * chunk), rowstep = (unsigned)(8 * CW * pitch);
     const int tail = pitch - 16 * chunk;             // step offsets below it have this lane's chunk inside the row
     const unsigned lds0 = lds_addr(smem);
 
@@ -215,9 +218,9 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
     auto stage = [&](const Tile& t, int kt, int buf) {
         const unsigned off = kt * F8_BLOCK < tail ? off0 : F8_OUTSIDE, dst = lds0 + buf * L::STAGE + wave * 1024;
 #pragma unroll
-        for (int j = 0; j < XPW; ++j) buf_lds16(t.x, off + j * rowstep, kt * F8_BLOCK, dst + j * NW * 1024);
+        for (int j = 0; j < XPW; ++j) buf_lds16(t.x, off + j * rowstep, kt * F8_BLOCK, dst + j * CW * 1024);
 #pragma unroll
-        for (int j = 0; j < WPW; ++j) buf_lds16(t.w, off + j * rowstep, kt * F8_BLOCK, dst + BM * F8_BLOCK + j * NW * 1024);
+        for (int j = 0; j < WPW; ++j) buf_lds16(t.w, off + j * rowstep, kt * F8_BLOCK, dst + BM * F8_BLOCK + j * CW * 1024);
     };
     auto panel = [&](const Tile& t, int p, int slot) {
         const unsigned dst = lds0 + 2 * L::STAGE + slot * L::PANEL;
@@ -231,7 +234,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
     int buf = 0, slot = 1;
     bool counted = false;
     panel(cur, 0, 0);
-    stage(cur, 0, 0);
+    if (wave < CW) stage(cur, 0, 0);
 
     // fragment addresses: row r of the wave's rows (rows 16 apart share their swizzle)
     const int c_lo = (g ^ (r >> 1)) << 4, c_hi = c_lo ^ 64;
@@ -258,8 +261,10 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
                 if (kt + 4 < kb) panel(cur, (kt >> 2) + 1, slot ^ 1);
                 else if (more) panel(nxt, 0, slot ^ 1);
             }
-            if (!fin) stage(cur, kt + 1, buf ^ 1);
-            else if (more) stage(nxt, 0, buf ^ 1);
+            if (wave < CW) {
+                if (!fin) stage(cur, kt + 1, buf ^ 1);
+                else if (more) stage(nxt, 0, buf ^ 1);
+            }
             const unsigned char* st = smem + buf * L::STAGE;
             const unsigned char* scp = smem + 2 * L::STAGE + slot * L::PANEL + (kt & 3);
             const unsigned wsc = scp[BM * 4 + wblock * 4];
@@ -364,15 +369,18 @@ template <int XF, typename TO, int BM, int BN, int WM, int WN> static int launch
     return check_launch("mad_linear_fp8");
 }
 
-// Which form.  Tiles of 256 x 256 need one for every compute unit; with fewer, tiles of 128 x 128 (two workgroups to a unit)
-// keep more of them busy (us, 256 / 128: 4096 x 4096 -> 4096 59 / 64, 4096 x 4096 -> 1024 52 / 26, 16384 x 1024 -> 4096
-// 74 / 84, 16384 x 1024 -> 256 19 / 11).  With fewer than one tile of 128 for each unit the direct form is as fast or
-// faster (1024 x 4096 -> 1024 22 / 24, 64 x 256 -> 4096 4.8 / 5.7; fp32 777 x 1000 -> 328 7 / 15).
+// Which form.  The units work in rounds of one tile of 256 x 256, or two of 128 x 128, each: the form whose rounds cover less area
+// takes less time, where a round of small tiles counts 1.18 of its area from K = 1024 on (16384 x 4096 -> 4096 240 us with
+// large tiles, 274 with small; 4096 x 4096 -> 1024 52 / 26) and nothing extra below (65536 x 384 -> 1152 51 / 47,
+// 16384 x 256 -> 4096 37 / 37).  With fewer than one small tile for each unit the direct form is as fast or faster
+// (1024 x 4096 -> 1024 22 / 24, 64 x 256 -> 4096 4.8 / 5.7; fp32 777 x 1000 -> 328 7 / 15).
 template <int XK, typename TO> static int launch_linear(F8LinArgs a, hipStream_t s) {
     if constexpr (XK < X_BF16) {
-        const int cus = f8_cus();
-        if (((a.M + 255) / 256) * ((a.N + 255) / 256) >= cus) return launch_tile<XK, TO, 256, 256, 2, 4>(a, s);
-        if (((a.M + 127) / 128) * ((a.N + 127) / 128) >= cus) return launch_tile<XK, TO, 128, 128, 2, 2>(a, s);
+        const long cus = f8_cus(), small = ((a.M + 127) / 128) * ((a.N + 127) / 128), large = ((a.M + 255) / 256) * ((a.N + 255) / 256);
+        if (small >= cus) {
+            const long rl = (large + cus - 1) / cus * 4 * 100, rs = (small + 2 * cus - 1) / (2 * cus) * 2 * (a.K >= 1024 ? 118 : 100);
+            return rl < rs ? launch_tile<XK, TO, 256, 256, 2, 4>(a, s) : launch_tile<XK, TO, 128, 128, 2, 2>(a, s);
+        }
     }
     return launch_direct<XK, TO>(a, s);
 }

@@ -152,20 +152,28 @@ __global__ __launch_bounds__(256) void wgrad_fp8_kernel(F8WgradArgs a) {
 }
 
 // Tiled form: dy in bf16 with rows of whole 16-byte pieces.  BN (n) x BK (k) of dw per workgroup of WN x WK waves, 64 rows m per
-// step, two LDS stages.  dy comes by LDS-DMA; x is loaded into registers one step ahead and widened into LDS after the step's
-// products, so that one barrier per step remains.  Columns past the end read what lies there, which only reaches results that
-// are not stored; rows past the share are zeros (buffer loads outside their buffer).
+// step, two LDS stages.  dy comes by LDS-DMA one step ahead.  The bytes of x come by LDS-DMA two steps ahead into
+// slots that only the lane that copied them reads (registers filled by ordinary loads had the compiler wait for them early), and are
+// widened into the next stage between the products of this one, so that one barrier per step remains.  Columns past the end read
+// what lies there, which only reaches results that are not stored; rows past the share are zeros (reads outside their buffer).
 template <int BN, int BK> struct F8Wg {
-    static constexpr int ROWS = 64, DY = ROWS * BN * 2, STAGE = DY + ROWS * BK * 2, LDS = 2 * STAGE;
+    static constexpr int ROWS = 64, DY = ROWS * BN * 2, STAGE = DY + ROWS * BK * 2;
+    static constexpr int RAW = ROWS * BK, SCALES = 2 * ROWS * 4;          // x as it comes; scales of two steps, a dword per row
+    static constexpr int LDS = 2 * STAGE + RAW + SCALES;
 };
+
+// The 16-byte chunk c of row m lies at c ^ swizzle(m): the eight rows that two lane groups read at a time, 32 bytes each, are in
+// eight different parts of the 256 bytes that the banks span (with (m & 3) << 2 alone every read took twice as long).
+__device__ __forceinline__ int swizzle(int m) { return ((m & 3) << 2) | ((m >> 2 & 1) << 1); }
 
 template <int FMT, int BN, int BK, int WN, int WK>
 __global__ __launch_bounds__(64 * WN * WK) void wgrad_fp8_tile_kernel(F8WgradArgs a) {
     using L = F8Wg<BN, BK>;
     constexpr int NW = WN * WK, FN = BN / WN / 16, FK = BK / WK / 16;
+    constexpr int FB = FN / WK;                                           // column sums: the waves of a row share its fragments
     constexpr int DPW = BN / 8 / NW;                                      // dy copies per wave and step (4 rows x 128 columns each)
     constexpr int XPT = 64 * BK / 16 / (64 * NW);                         // 16-byte pieces of x per thread and step
-    static_assert(BN % 128 == 0 && BK % 128 == 0 && BN % (8 * NW) == 0 && XPT * 16 * NW == BK, "tile");
+    static_assert(BK <= 512 && NW % 2 == 0 && (64 * NW / (BK / 16)) % 8 == 0 && BN % 128 == 0 && BK % 128 == 0 && BN % (8 * NW) == 0 && XPT * 16 * NW == BK && FN % WK == 0, "tile");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wn = wave / WK, wk = wave % WK;
@@ -182,7 +190,7 @@ __global__ __launch_bounds__(64 * WN * WK) void wgrad_fp8_tile_kernel(F8WgradArg
     const int n0 = nt * BN, k0 = kt * BK;
     const long m_begin = (long)split * a.per, m_end = m_begin + a.per < a.M ? m_begin + a.per : a.M;
     const int steps = (int)((m_end - m_begin + L::ROWS - 1) / L::ROWS);
-    const int xp = f8_pitch(a.K), sp = f8_scale_pitch(a.K), kb = f8_blocks(a.K);
+    const int xp = f8_pitch(a.K), sp = f8_scale_pitch(a.K);
 
     // where this lane's copies read: offsets inside the 64 rows of a step
     const int lr = lane >> 4;
@@ -190,89 +198,120 @@ __global__ __launch_bounds__(64 * WN * WK) void wgrad_fp8_tile_kernel(F8WgradArg
 #pragma unroll
     for (int j = 0; j < DPW; ++j) {
         const int c = j * NW + wave;                                      // half c / 16, rows 4 (c % 16) ..
-        doff[j] = (unsigned)((4 * (c & 15) + lr) * a.N * 2 + (n0 + (c >> 4) * 128) * 2 + (((lane & 15) ^ (lr << 2)) << 4));
+        doff[j] = (unsigned)((4 * (c & 15) + lr) * a.N * 2 + (n0 + (c >> 4) * 128) * 2 + (((lane & 15) ^ swizzle(4 * wave + lr)) << 4));   // NW is even
     }
-    unsigned xoff[XPT], soff[XPT];
-    int xdst[XPT];
+    unsigned xoff[XPT];
+    int xdst[XPT], sbyte[XPT];
 #pragma unroll
     for (int u = 0; u < XPT; ++u) {
         const int i = u * 64 * NW + tid, row = i / (BK / 16), piece = i % (BK / 16), half = piece >> 3;
         xoff[u] = (unsigned)(row * xp + k0 + 16 * piece);
         const int block = k0 / F8_BLOCK + half;
-        soff[u] = (unsigned)(row * sp + (block < kb ? block : kb - 1));
-        xdst[u] = L::DY + (half * L::ROWS + row) * 256 + (((2 * (piece & 7)) ^ ((row & 3) << 2)) << 4);
+        sbyte[u] = row * 4 + (block & 3);
+        // odd rows write their second piece first: the pieces of a write then cover all banks
+        xdst[u] = L::DY + (half * L::ROWS + row) * 256 + (((2 * (piece & 7) + (row & 1)) ^ swizzle(row)) << 4);
     }
     const unsigned lds0 = lds_addr(smem);
-    uint4 xr[XPT];
-    unsigned sr[XPT];
-    auto fetch = [&](int s, int buf) {                                    // step s: dy into its stage, x into registers
+    // rows of step s that exist (none behind the last: the reads then deliver zeros)
+    auto step_rows = [&](int s) {
+        const long left = m_end - m_begin - (long)s * L::ROWS;
+        return left < 0 ? 0 : left < L::ROWS ? (int)left : L::ROWS;
+    };
+    auto fetch_dy = [&](int s, int buf) {                                 // dy of step s into its stage
         const long m = m_begin + (long)s * L::ROWS;
-        const int rows = m_end - m < L::ROWS ? (int)(m_end - m) : L::ROWS;
-        const u32x4 db = f8_buffer((const unsigned char*)a.dy + (size_t)m * a.N * 2, (unsigned)(rows * a.N * 2));
+        const u32x4 db = f8_buffer((const unsigned char*)a.dy + (size_t)m * a.N * 2, (unsigned)(step_rows(s) * a.N * 2));
 #pragma unroll
         for (int j = 0; j < DPW; ++j) buf_lds16(db, doff[j], 0, lds0 + buf * L::STAGE + (j * NW + wave) * 1024);
-        const auto xrs = __builtin_amdgcn_make_buffer_rsrc((void*)(a.x + (size_t)m * xp), 0, rows * xp, 0x00020000);
-        const auto srs = __builtin_amdgcn_make_buffer_rsrc((void*)(a.xs + (size_t)m * sp), 0, rows * sp, 0x00020000);
+    };
+    constexpr int RAW = 2 * L::STAGE, SCALES = RAW + L::RAW;
+    // scales of step s: the dword of each row that holds the tile's blocks (k0 is a multiple of BK, so they are in one)
+    auto fetch_scales = [&](int s) {
+        const long m = m_begin + (long)s * L::ROWS;
+        const u32x4 sb = f8_buffer(a.xs + (size_t)m * sp, (unsigned)(step_rows(s) * sp));
+        if (wave == NW - 1) buf_lds4(sb, (unsigned)(lane * sp + (k0 / F8_BLOCK & ~3)), 0, lds0 + SCALES + (s & 1) * 256);
+    };
+    auto fetch_x = [&](int s) {                                           // x of step s into this lane's slots
+        const long m = m_begin + (long)s * L::ROWS;
+        const u32x4 xb = f8_buffer(a.x + (size_t)m * xp, (unsigned)(step_rows(s) * xp));
 #pragma unroll
         for (int u = 0; u < XPT; ++u) {
-            xr[u] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(xrs, (int)xoff[u], 0, 0));
-            sr[u] = (unsigned char)__builtin_amdgcn_raw_buffer_load_b8(srs, (int)soff[u], 0, 0);
+            buf_lds16(xb, xoff[u], 0, lds0 + RAW + (u * NW + wave) * 1024);
         }
     };
-    auto widen = [&](int buf) {                                           // the fetched x into the stage
+    auto widen = [&](int s, int buf) {                                    // the fetched x of step s into the stage
+        const bool odd = tid / (BK / 16) & 1;                            // of the row: 64 NW / (BK / 16) rows apart is even
+        unsigned char* d = smem + buf * L::STAGE;
 #pragma unroll
         for (int u = 0; u < XPT; ++u) {
-            const float s = f8_scale(sr[u]);
-            unsigned char* d = smem + buf * L::STAGE;
-            *reinterpret_cast<bf16x8*>(d + xdst[u]) = f8_bf16x8<FMT>(xr[u].x, xr[u].y, s);
-            *reinterpret_cast<bf16x8*>(d + (xdst[u] ^ 16)) = f8_bf16x8<FMT>(xr[u].z, xr[u].w, s);
+            const uint4 v = *reinterpret_cast<const uint4*>(smem + RAW + (u * 64 * NW + tid) * 16);
+            const float sc = f8_scale(smem[SCALES + (s & 1) * 256 + sbyte[u]]);
+            const unsigned a0 = odd ? v.z : v.x, a1 = odd ? v.w : v.y, b0 = odd ? v.x : v.z, b1 = odd ? v.y : v.w;
+            *reinterpret_cast<bf16x8*>(d + xdst[u]) = f8_bf16x8<FMT>(a0, a1, sc);
+            *reinterpret_cast<bf16x8*>(d + (xdst[u] ^ 16)) = f8_bf16x8<FMT>(b0, b1, sc);
         }
     };
 
-    f32x4 acc[FK][FN], accb[FN];                              // [k fragment][n fragment]
+    f32x4 acc[FK][FN], accb[FB];                              // [k fragment][n fragment]
+#pragma unroll
+    for (int j = 0; j < FB; ++j) accb[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
-        accb[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < FK; ++i) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     const __bf16 one = (__bf16)1.0f;
     const bf16x8 ones = {one, one, one, one, one, one, one, one};
-    const bool with_bias = a.db && wk == 0;
-    int turn = 0;
+    int turn = a.db ? 0 : -1;                                 // step mod ktiles
 
     // fragment of 16 columns: rows 4g + q and 16 rows on, 8 bytes at columns 4 pp
-    const int frow = (4 * g + q) * 256 + (pp & 1) * 8;
+    const int frow = (4 * g + q) * 256 + (pp & 1) * 8, fswz = swizzle(4 * g + q);
     auto frag = [&](const unsigned char* tile, int c, int h) {
         const int chunk = ((c & 127) >> 3) + (pp >> 1);
-        const unsigned char* p = tile + (c >> 7) * L::ROWS * 256 + h * 32 * 256 + frow + ((chunk ^ (q << 2)) << 4);
+        const unsigned char* p = tile + (c >> 7) * L::ROWS * 256 + h * 32 * 256 + frow + ((chunk ^ fswz) << 4);
         return tr_pair(p, p + 16 * 256);
     };
 
-    if (steps > 0) { fetch(0, 0); widen(0); }
+    fetch_scales(0);
+    fetch_x(0);
+    fetch_scales(1);
+    dma_wait_all();
+    __syncthreads();
+    fetch_dy(0, 0);
+    widen(0, 0);
+    fetch_x(1);
     for (int s = 0; s < steps; ++s) {
         const int buf = s & 1;
         dma_wait_all();
         __syncthreads();                   // step s is visible; every wave is done with the stage refilled below
-        if (s + 1 < steps) fetch(s + 1, buf ^ 1);
-        const bool mine = with_bias && turn == kt;
-        turn = turn + 1 == a.ktiles ? 0 : turn + 1;
+        fetch_dy(s + 1, buf ^ 1);
+        fetch_scales(s + 2);
         const unsigned char* st = smem + buf * L::STAGE;
+        if (turn == kt) {                  // not among the products below: a branch around each would keep their reads from running ahead
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < FB; ++j)
+                    accb[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, frag(st, wn * (BN / WN) + 16 * (wk * FB + j), h), accb[j], 0, 0, 0);
+        }
+        if (a.db) turn = turn + 1 == a.ktiles ? 0 : turn + 1;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            bf16x8 xf[FK];
+            bf16x8 xf[FK], d[FN];
 #pragma unroll
             for (int i = 0; i < FK; ++i) xf[i] = frag(st + L::DY, wk * (BK / WK) + 16 * i, h);
 #pragma unroll
-            for (int j = 0; j < FN; ++j) {
-                const bf16x8 d = frag(st, wn * (BN / WN) + 16 * j, h);
-                if (mine) accb[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, d, accb[j], 0, 0, 0);
+            for (int j = 0; j < FN; ++j) d[j] = frag(st, wn * (BN / WN) + 16 * j, h);
 #pragma unroll
-                for (int i = 0; i < FK; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[i], d, acc[i][j], 0, 0, 0);
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int i = 0; i < FK; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[i], d[j], acc[i][j], 0, 0, 0);
+            if (h == 0) {                  // between the products of the other waves
+                widen(s + 1, buf ^ 1);
+                fetch_x(s + 2);
             }
         }
-        if (s + 1 < steps) widen(buf ^ 1);
     }
+    dma_wait_all();                        // the copies of the step behind the last
 
     // a lane holds four consecutive k of one n
     const bool direct = a.splits == 1;
@@ -291,20 +330,47 @@ __global__ __launch_bounds__(64 * WN * WK) void wgrad_fp8_tile_kernel(F8WgradArg
             if (direct && a.acc_w) v += load4_tail<float>(p, k, a.K);
             store4_tail<float>(p, k, a.K, v);
         }
-        if (with_bias && g == 0) {
+    }
+    if (a.db && g == 0) {
+#pragma unroll
+        for (int j = 0; j < FB; ++j) {
+            const int n = n0 + wn * (BN / WN) + 16 * (wk * FB + j) + r;
+            if (n >= a.N) continue;
             float* p = a.db + ((size_t)split * a.ktiles + kt) * a.N + n;
             *p = (a.acc_b ? *p : 0.0f) + accb[j][0];
         }
     }
 }
 
-// dst[i] (+)= sum of the parts' partial sums, in order
-__global__ __launch_bounds__(256) void wgrad_fp8_join_kernel(const float* __restrict__ part, float* __restrict__ dst, size_t n,
-                                                             int parts, int accumulate) {
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+// dw[i] (+)= sum of `parts` partial sums of n elements, in order; the last workgroups do the same for db (nb elements of
+// `parts_b`).  Four elements per thread and eight parts in flight: the loads, not the additions, take the time.
+struct F8JoinArgs { const float* part; float* dst; const float* part_b; float* dst_b; size_t n; int nb, parts, parts_b, acc, acc_b, blocks; };
+
+__global__ __launch_bounds__(256) void wgrad_fp8_join_kernel(F8JoinArgs a) {
+    if ((int)blockIdx.x >= a.blocks) {
+        const int i = (blockIdx.x - a.blocks) * 256 + threadIdx.x;
+        if (i >= a.nb) return;
         float s = 0.0f;
-        for (int z = 0; z < parts; ++z) s += part[(size_t)z * n + i];
-        dst[i] = accumulate ? dst[i] + s : s;
+#pragma unroll 8
+        for (int z = 0; z < a.parts_b; ++z) s += a.part_b[(size_t)z * a.nb + i];
+        a.dst_b[i] = a.acc_b ? a.dst_b[i] + s : s;
+        return;
+    }
+    for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4; i < a.n; i += (size_t)a.blocks * 1024) {
+        f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (i + 4 <= a.n) {
+            typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll 8
+            for (int z = 0; z < a.parts; ++z) s += *reinterpret_cast<const f32x4u*>(a.part + (size_t)z * a.n + i);
+            if (a.acc) s += load4_tail<float>(a.dst + i, 0, 4);
+            store4_tail<float>(a.dst + i, 0, 4, s);
+        } else {
+            for (size_t e = i; e < a.n; ++e) {
+                float v = 0.0f;
+                for (int z = 0; z < a.parts; ++z) v += a.part[(size_t)z * a.n + e];
+                a.dst[e] = a.acc ? a.dst[e] + v : v;
+            }
+        }
     }
 }
 
@@ -317,8 +383,8 @@ static F8WgradPlan wgrad_plan(long rows, int N, int K, bool tiled) {
     const int cus = f8_cus();
     p.tile = tiled && tiles(256) >= cus ? 256 : 128;
     p.ntiles = (N + p.tile - 1) / p.tile; p.ktiles = (K + p.tile - 1) / p.tile;
-    long s = (2 * cus + tiles(p.tile) - 1) / tiles(p.tile);
-    if (p.tile == 256) s = 1;
+    // two workgroups of the small tile fit a unit at a time: no more shares than fill them once
+    long s = p.tile == 256 ? 1 : 2 * cus / tiles(p.tile);
     const long most = (rows + 255) / 256;
     if (s > most) s = most;
     p.splits = (int)(s < 1 ? 1 : s);
@@ -401,13 +467,13 @@ extern "C" int mad_linear_fp8_wgrad(const void* dy, int dtype, const void* x, in
         rc = check_launch("mad_linear_fp8_wgrad");
     }
     if (rc) return rc;
-    if (join_w) {
-        const size_t blocks = (nk + 255) / 256;
-        hipLaunchKernelGGL(wgrad_fp8_join_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s,
-                           (const float*)part_w, dw, nk, p.splits, accumulate);
-    }
-    if (join_b)
-        hipLaunchKernelGGL(wgrad_fp8_join_kernel, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, s, (const float*)part_b, db,
-                           (size_t)N, p.splits * p.ktiles, bias_accumulate);
-    return join_w || join_b ? check_launch("mad_linear_fp8_wgrad") : 0;
+    if (!join_w && !join_b) return 0;
+    F8JoinArgs j;
+    j.part = part_w; j.dst = dw; j.part_b = part_b; j.dst_b = db;
+    j.n = join_w ? nk : 0; j.nb = join_b ? N : 0; j.parts = p.splits; j.parts_b = p.splits * p.ktiles;
+    j.acc = accumulate; j.acc_b = bias_accumulate;
+    const size_t blocks = (j.n + 1023) / 1024;
+    j.blocks = (int)(blocks < 4096 ? blocks : 4096);
+    hipLaunchKernelGGL(wgrad_fp8_join_kernel, dim3((unsigned)(j.blocks + (j.nb + 255) / 256)), dim3(256), 0, s, j);
+    return check_launch("mad_linear_fp8_wgrad");
 }
