@@ -51,6 +51,22 @@ template <int FMT> __device__ __forceinline__ unsigned f8_cvt4(float a, float b,
     return (unsigned)r;
 }
 
+// Four bf16 (two dwords) times 2^-e as four bytes, one instruction per pair.  The conversion divides by its scale operand, whose
+// exponent alone counts: scale is 2^e.
+template <int FMT> __device__ __forceinline__ unsigned f8_cvt4_bf16(unsigned lo, unsigned hi, float scale) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    s16x2 r = {0, 0};
+    if (FMT == F8_E4M3) {
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, lo), scale, false);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, hi), scale, true);
+    } else {
+        r = __builtin_amdgcn_cvt_scalef32_pk_bf8_bf16(r, __builtin_bit_cast(bf16x2, lo), scale, false);
+        r = __builtin_amdgcn_cvt_scalef32_pk_bf8_bf16(r, __builtin_bit_cast(bf16x2, hi), scale, true);
+    }
+    return __builtin_bit_cast(unsigned, r);
+}
+
 // the four values of one dword, times 2^e
 template <int FMT> __device__ __forceinline__ void f8_values4(unsigned q, float scale, float* f) {
     typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -116,6 +132,25 @@ template <> __device__ __forceinline__ void store8<float>(float* p, const float*
     reinterpret_cast<f32x4u*>(p)[0] = f32x4u{f[0], f[1], f[2], f[3]};
     reinterpret_cast<f32x4u*>(p)[1] = f32x4u{f[4], f[5], f[6], f[7]};
 }
+// eight elements as they were loaded (their conversion waits until they are added)
+template <typename T> struct Piece8;
+template <> struct Piece8<bf16_t> {
+    typedef unsigned u32x4u __attribute__((ext_vector_type(4), aligned(2)));
+    u32x4u v;
+    __device__ __forceinline__ void load(const bf16_t* p) { v = *reinterpret_cast<const u32x4u*>(p); }
+    __device__ __forceinline__ void add(float* f) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { f[2 * i] += __uint_as_float(v[i] << 16); f[2 * i + 1] += __uint_as_float(v[i] & 0xffff0000u); }
+    }
+};
+template <> struct Piece8<float> {
+    float v[8];
+    __device__ __forceinline__ void load(const float* p) { load8<float>(p, v); }
+    __device__ __forceinline__ void add(float* f) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] += v[i];
+    }
+};
 // the same for a piece that may reach past column C (columns behind it read as zero, are not written)
 template <typename T> __device__ __forceinline__ void load8_tail(const T* p, int c, int C, float* f) {
     if (c + 8 <= C) { load8<T>(p, f); return; }
@@ -175,6 +210,11 @@ __device__ __forceinline__ u32x4 f8_buffer(const unsigned char* p, unsigned byte
                  (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
 }
 constexpr unsigned F8_OUTSIDE = 0xc0000000u;      // buffers are smaller than 2^31 bytes; what is added to this stays outside
+
+// the same for the compiler's own buffer loads
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t f8_resource(const void* p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
+}
 
 // LDS-DMA through a buffer descriptor: 16 (4) bytes per lane to lds_wave_base + 16 (4) * lane; see glds16 for M0
 __device__ __forceinline__ void buf_lds16(const u32x4& buf, unsigned voff, unsigned soff, unsigned lds_wave_base) {

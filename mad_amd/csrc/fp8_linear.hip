@@ -62,10 +62,11 @@ __device__ __forceinline__ void block_product(f32x4& acc, const i32x8& w, const 
 }
 
 // Direct form: operands from global memory straight into registers, (16 MF) x (16 NF) outputs per workgroup, its NW
-// waves taking every NW-th block of the reduction; their sums are added in wave order through LDS.
+// waves taking every NW-th block of the reduction.  Few rows are bound by the latency of reading the weights once, so the reduction is
+// spread over many waves; their sums are joined through LDS pairwise, wave w and w + NW/2 first: a fixed order.
 template <int XK, typename TO, int MF, int NF, int NW>
 __global__ __launch_bounds__(64 * NW) void linear_fp8_direct_kernel(F8LinArgs a) {
-    __shared__ __attribute__((aligned(16))) f32x4 red[NW > 1 ? NW : 1][MF * NF][64];
+    __shared__ __attribute__((aligned(16))) f32x4 red[NW / 2][MF * NF][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4;
     const long mt = blockIdx.x / a.ntiles;
@@ -74,81 +75,132 @@ __global__ __launch_bounds__(64 * NW) void linear_fp8_direct_kernel(F8LinArgs a)
     const int n0 = nt * (16 * NF);
     const int kb = f8_blocks(a.K), wp = f8_pitch(a.K), sp = f8_scale_pitch(a.K);
 
+    // Buffer loads without a branch: lanes behind the last row, or behind the end of their row, read zeros.
+    const int mrem = a.M - m0 < 16 * MF ? (int)(a.M - m0) : 16 * MF, nrem = a.N - n0 < 16 * NF ? a.N - n0 : 16 * NF;
+    const auto wbuf = f8_resource(a.w + (size_t)n0 * wp, nrem * wp);
+    const auto wsbuf = f8_resource(a.ws + (size_t)(n0 / F8_BLOCK) * sp, f8_blocks(n0 % F8_BLOCK + nrem) * sp);
+    constexpr int XB = XK < X_BF16 ? 1 : XK == X_BF16 ? 2 : 4;
+    const int xpitch = XK < X_BF16 ? wp : a.K * XB;
+    const auto xbuf = f8_resource((const unsigned char*)a.x + (size_t)m0 * xpitch, mrem * xpitch);
+    const auto xsbuf = f8_resource(a.xs + (XK < X_BF16 ? (size_t)m0 * sp : 0), XK < X_BF16 ? mrem * sp : 0);
+    const bool whole = XK >= X_BF16 && (a.K * XB) % 16 == 0 && ((uintptr_t)a.x & 15) == 0;
+    auto load16 = [](const auto& rsrc, int off) { return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 0)); };
+
     f32x4 acc[NF][MF];
 #pragma unroll
     for (int j = 0; j < NF; ++j)
 #pragma unroll
         for (int i = 0; i < MF; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
+#pragma unroll 1
     for (int kt = wave; kt < kb; kt += NW) {
         const int c = kt * F8_BLOCK + 32 * g;
-        i32x8 wf[NF], xf[MF];
-        int wsc[NF], xsc[MF];
+        i32x8 wf[NF];
+        int wsc[NF];
 #pragma unroll
         for (int j = 0; j < NF; ++j) {
-            int n = n0 + 16 * j + r;
-            n = n < a.N ? n : a.N - 1;                 // rows past the end repeat the last one: their results are not stored
-            const unsigned char* p = a.w + (size_t)n * wp + c;
-            uint4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-            if (c < wp) lo = *reinterpret_cast<const uint4*>(p);
-            if (c + 16 < wp) hi = *reinterpret_cast<const uint4*>(p + 16);
-            wf[j] = pair16(lo, hi);
-            wsc[j] = a.ws[(size_t)(n / F8_BLOCK) * sp + kt];
+            const int off = (16 * j + r) * wp + c;
+            wf[j] = pair16(load16(wbuf, c < wp ? off : (int)F8_OUTSIDE), load16(wbuf, c + 16 < wp ? off + 16 : (int)F8_OUTSIDE));
+            wsc[j] = (unsigned char)__builtin_amdgcn_raw_buffer_load_b8(wsbuf, ((n0 % F8_BLOCK + 16 * j + r) / F8_BLOCK) * sp + kt, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < MF; ++i) {
-            long m = m0 + 16 * i + r;
-            m = m < a.M ? m : a.M - 1;
+            i32x8 xf;
+            int xsc;
             if constexpr (XK < X_BF16) {
-                const unsigned char* p = (const unsigned char*)a.x + (size_t)m * wp + c;
-                uint4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-                if (c < wp) lo = *reinterpret_cast<const uint4*>(p);
-                if (c + 16 < wp) hi = *reinterpret_cast<const uint4*>(p + 16);
-                xf[i] = pair16(lo, hi);
-                xsc[i] = a.xs[(size_t)m * sp + kt];
+                const int off = (16 * i + r) * wp + c;
+                xf = pair16(load16(xbuf, c < wp ? off : (int)F8_OUTSIDE), load16(xbuf, c + 16 < wp ? off + 16 : (int)F8_OUTSIDE));
+                xsc = (unsigned char)__builtin_amdgcn_raw_buffer_load_b8(xsbuf, (16 * i + r) * sp + kt, 0, 0);
             } else {
                 using T = typename std::conditional<XK == X_BF16, bf16_t, float>::type;
-                const T* p = (const T*)a.x + (size_t)m * a.K + c;
-                float f[32];
                 unsigned u = 0;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) load8_tail<T>(p + 8 * q, c + 8 * q, a.K, f + 8 * q);
-#pragma unroll
-                for (int e = 0; e < 32; ++e) { const unsigned t = f8_mag(f[e]); u = t > u ? t : u; }
                 // the row's block: this lane's quarter and those of the lanes 16, 32 and 48 on
-                unsigned t = __shfl_xor(u, 16); u = t > u ? t : u;
-                t = __shfl_xor(u, 32); u = t > u ? t : u;
-                const unsigned s = f8_scale_byte<F8_E4M3>(u);
-                const float inv = f8_inv_scale(s);
+                auto over_block = [](unsigned v) {
+                    unsigned t = __shfl_xor(v, 16); v = t > v ? t : v;
+                    t = __shfl_xor(v, 32); return t > v ? t : v;
+                };
+                if (XK == X_BF16 && whole) {
+                    // on pairs of bf16 as they are: their magnitudes' maximum as 16-bit integers, and one conversion for two
+                    uint4 v[4];
 #pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    xf[i][q] = (int)f8_cvt4<F8_E4M3>(f[4 * q] * inv, f[4 * q + 1] * inv, f[4 * q + 2] * inv, f[4 * q + 3] * inv);
-                xsc[i] = (int)s;
+                    for (int q = 0; q < 4; ++q) v[q] = load16(xbuf, c + 8 * q < a.K ? (16 * i + r) * xpitch + 2 * c + 16 * q : (int)F8_OUTSIDE);
+                    const unsigned* w = &v[0].x;
+                    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+                    u16x2 m = {0, 0};
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[e] & 0x7fff7fffu));
+                    u = m[0] > m[1] ? m[0] : m[1];
+                    if (__any(u >= 0x7f80u)) {                             // something is not finite: it does not count
+                        u = 0;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const unsigned lo = w[e] & 0x7fffu, hi = w[e] >> 16 & 0x7fffu;
+                            u = lo < 0x7f80u && lo > u ? lo : u;
+                            u = hi < 0x7f80u && hi > u ? hi : u;
+                        }
+                    }
+                    xsc = (int)f8_scale_byte<F8_E4M3>(over_block(u) << 16);
+                    const float scale = f8_scale((unsigned)xsc);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) xf[q] = (int)f8_cvt4_bf16<F8_E4M3>(w[2 * q], w[2 * q + 1], scale);
+                } else {
+                    float f[32];
+                    if (whole) {
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) {                      // 32 floats; the last block's lanes behind K read zeros
+                            const uint4 v = load16(xbuf, c + 4 * q < a.K ? (16 * i + r) * xpitch + 4 * c + 16 * q : (int)F8_OUTSIDE);
+                            f[4 * q] = __uint_as_float(v.x); f[4 * q + 1] = __uint_as_float(v.y);
+                            f[4 * q + 2] = __uint_as_float(v.z); f[4 * q + 3] = __uint_as_float(v.w);
+                        }
+                    } else {                                               // rows that start, or end, anywhere
+                        const long m = m0 + 16 * i + r < a.M ? m0 + 16 * i + r : a.M - 1;
+                        const T* p = (const T*)a.x + (size_t)m * a.K + c;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) load8_tail<T>(p + 8 * q, c + 8 * q, a.K, f + 8 * q);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) { const unsigned t = f8_mag(f[e]); u = t > u ? t : u; }
+                    xsc = (int)f8_scale_byte<F8_E4M3>(over_block(u));
+                    const float inv = f8_inv_scale((unsigned)xsc);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        xf[q] = (int)f8_cvt4<F8_E4M3>(f[4 * q] * inv, f[4 * q + 1] * inv, f[4 * q + 2] * inv, f[4 * q + 3] * inv);
+                }
             }
+#pragma unroll
+            for (int j = 0; j < NF; ++j) block_product<XK == X_E5M2 ? F8_E5M2 : F8_E4M3, sizeof(TO) == 4>(acc[j][i], wf[j], xf, wsc[j], xsc);
         }
-#pragma unroll
-        for (int j = 0; j < NF; ++j)
-#pragma unroll
-            for (int i = 0; i < MF; ++i)
-                block_product<XK == X_E5M2 ? F8_E5M2 : F8_E4M3, sizeof(TO) == 4>(acc[j][i], wf[j], xf[i], wsc[j], xsc[i]);
     }
-    if constexpr (NW > 1) {
 #pragma unroll
-        for (int j = 0; j < NF; ++j)
+    for (int half = NW / 2; half > 1; half /= 2) {
+        if (wave >= half && wave < 2 * half) {
 #pragma unroll
-            for (int i = 0; i < MF; ++i) red[wave][j * MF + i][lane] = acc[j][i];
-        __syncthreads();
-        for (int f = wave; f < MF * NF; f += NW) {
-            f32x4 v = red[0][f][lane];
+            for (int j = 0; j < NF; ++j)
 #pragma unroll
-            for (int w = 1; w < NW; ++w) v += red[w][f][lane];
-            store_quad<TO>(a, m0 + 16 * (f % MF) + r, n0 + 16 * (f / MF) + 4 * g, v);
+                for (int i = 0; i < MF; ++i) red[wave - half][j * MF + i][lane] = acc[j][i];
         }
-    } else {
+        __syncthreads();
+        if (wave < half) {
+#pragma unroll
+            for (int j = 0; j < NF; ++j)
+#pragma unroll
+                for (int i = 0; i < MF; ++i) acc[j][i] += red[wave][j * MF + i][lane];
+        }
+        __syncthreads();
+    }
+    // the last pair: wave 1 hands over, wave 0 stores
+    if (wave == 1) {
 #pragma unroll
         for (int j = 0; j < NF; ++j)
 #pragma unroll
-            for (int i = 0; i < MF; ++i) store_quad<TO>(a, m0 + 16 * i + r, n0 + 16 * j + 4 * g, acc[j][i]);
+            for (int i = 0; i < MF; ++i) red[0][j * MF + i][lane] = acc[j][i];
+    }
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+        for (int j = 0; j < NF; ++j)
+#pragma unroll
+            for (int i = 0; i < MF; ++i) store_quad<TO>(a, m0 + 16 * i + r, n0 + 16 * j + 4 * g, acc[j][i] + red[0][j * MF + i][lane]);
     }
 }
 
@@ -178,7 +230,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
     // meanwhile the SIMD's other wave multiplies (16384 x 4096 -> 8192: 489 us with all eight waves copying, 463 with four)
     constexpr int CW = NW == 8 ? 4 : NW;
     constexpr int XPW = BM / 8 / CW, WPW = BN / 8 / CW;                   // copy instructions per copying wave and step
-    static_assert(CW % 2 == 0 && BM % (8 * CW) == 0 && BN % (8 * CW) == 0 && NF % 2 == 0 && BN / WN <= F8_BLOCK && BM % 64 == 0 &&
+    static_assert(CW % 2 == 0 && BM % (8 * CW) == 0 && BN % (8 * CW) == 0 && NF % 2 == 0 && MF % 4 == 0 && BN / WN <= F8_BLOCK && BM % 64 == 0 &&
                   BM <= 64 * NW, "tile");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -305,18 +357,30 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
             }
         };
         const long mb = cur.m0 + wm * (BM / WM) + r;
-        // a whole tile without a residual is stored by straight code whose number of stores the next step's wait relies on
-        counted = cur.m0 + BM <= a.M && cur.n0 + BN <= a.N && !a.residual;
+        // A whole tile is stored by straight code whose number of stores the next step's wait relies on; its residual is loaded
+        // G row fragments at a time before their stores (a load behind a store waits for it: they complete in order).
+        counted = cur.m0 + BM <= a.M && cur.n0 + BN <= a.N;
         if (counted) {
+            constexpr int G = sizeof(TO) == 2 ? 4 : 2;                        // row fragments at a time: what registers hold
 #pragma unroll
-            for (int i = 0; i < MF; ++i)
+            for (int i0 = 0; i0 < MF; i0 += G) {
+                Piece8<TO> res[G][NF / 2];
+                if (a.residual) {
 #pragma unroll
-                for (int p = 0; p < NF / 2; ++p) {
-                    float v[8];
-                    piece(i, p, v);
-                    TO* y = (TO*)a.y + (mb + 16 * i) * a.N + nb + 32 * p;
-                    store8<TO>(y, v);
+                    for (int i = 0; i < G; ++i)
+#pragma unroll
+                        for (int p = 0; p < NF / 2; ++p) res[i][p].load((const TO*)a.residual + (mb + 16 * (i0 + i)) * a.N + nb + 32 * p);
                 }
+#pragma unroll
+                for (int i = 0; i < G; ++i)
+#pragma unroll
+                    for (int p = 0; p < NF / 2; ++p) {
+                        float v[8];
+                        piece(i0 + i, p, v);
+                        if (a.residual) res[i][p].add(v);
+                        store8<TO>((TO*)a.y + (mb + 16 * (i0 + i)) * a.N + nb + 32 * p, v);
+                    }
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < MF; ++i)
@@ -343,8 +407,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
     }
 }
 
-template <int XK, typename TO> static int launch_direct(F8LinArgs a, hipStream_t s) {
-    constexpr int MF = 4, NF = 4, NW = 4;
+template <int XK, typename TO, int MF, int NF, int NW> static int launch_direct(F8LinArgs a, hipStream_t s) {
     const long mtiles = (a.M + 16 * MF - 1) / (16 * MF);
     a.ntiles = (a.N + 16 * NF - 1) / (16 * NF);
     MAD_REQUIRE(mtiles * a.ntiles <= 0x7fffffffL, "mad_linear_fp8: %ld rows x %d columns need more workgroups than a launch holds",
@@ -355,14 +418,14 @@ template <int XK, typename TO> static int launch_direct(F8LinArgs a, hipStream_t
 
 template <int XF, typename TO, int BM, int BN, int WM, int WN> static int launch_tile(F8LinArgs a, hipStream_t s) {
     constexpr int lds = F8Tile<BM, BN>::LDS, resident = 163840 / lds;
+    const long mtiles = (a.M + BM - 1) / BM;
+    a.ntiles = (a.N + BN - 1) / BN;
+    MAD_REQUIRE(mtiles * a.ntiles <= 0x7fffffffL / 8, "mad_linear_fp8: %ld rows x %d columns need more tiles than the workgroups count",
+                a.M, a.N);
     static int lds_dev = -1;
     auto kernel = &linear_fp8_tile_kernel<XF, TO, BM, BN, WM, WN>;
     MAD_REQUIRE(raise_lds_limit(reinterpret_cast<const void*>(kernel), lds, &lds_dev),
                 "mad_linear_fp8: cannot raise the dynamic LDS limit to %d", lds);
-    const long mtiles = (a.M + BM - 1) / BM;
-    a.ntiles = (a.N + BN - 1) / BN;
-    MAD_REQUIRE(mtiles * a.ntiles <= 0x7fffffffL / 8, "mad_linear_fp8: %ld rows x %d columns have more tiles than the kernel counts",
-                a.M, a.N);
     a.mtiles = (int)mtiles;
     const int tiles = a.mtiles * a.ntiles, grid = f8_cus() * resident;
     hipLaunchKernelGGL((linear_fp8_tile_kernel<XF, TO, BM, BN, WM, WN>), dim3(tiles < grid ? tiles : grid), dim3(64 * WM * WN), lds, s, a);
@@ -373,7 +436,7 @@ template <int XF, typename TO, int BM, int BN, int WM, int WN> static int launch
 // takes less time, where a round of small tiles counts 1.18 of its area from K = 1024 on (16384 x 4096 -> 4096 240 us with
 // large tiles, 274 with small; 4096 x 4096 -> 1024 52 / 26) and nothing extra below (65536 x 384 -> 1152 51 / 47,
 // 16384 x 256 -> 4096 37 / 37).  With fewer than one small tile for each unit the direct form is as fast or faster
-// (1024 x 4096 -> 1024 22 / 24, 64 x 256 -> 4096 4.8 / 5.7; fp32 777 x 1000 -> 328 7 / 15).
+// (1024 x 4096 -> 1024 23 / 24, 64 x 256 -> 4096 3.5 / 5.7; fp32 777 x 1000 -> 328 7 / 15).
 template <int XK, typename TO> static int launch_linear(F8LinArgs a, hipStream_t s) {
     if constexpr (XK < X_BF16) {
         const long cus = f8_cus(), small = ((a.M + 127) / 128) * ((a.N + 127) / 128), large = ((a.M + 255) / 256) * ((a.N + 255) / 256);
@@ -382,7 +445,18 @@ template <int XK, typename TO> static int launch_linear(F8LinArgs a, hipStream_t
             return rl < rs ? launch_tile<XK, TO, 256, 256, 2, 4>(a, s) : launch_tile<XK, TO, 128, 128, 2, 2>(a, s);
         }
     }
-    return launch_direct<XK, TO>(a, s);
+    // Of the direct form, the smaller its workgroups the more of them share the latency, until re-reading costs more.  Sixteen by
+    // sixteen results each up to two workgroups for each unit, then 32 x 32, then 64 x 64 (packed x, us: 64 x 1024 -> 1024 3.6 / 4.9
+    // / 7.5, 64 x 4096 -> 4096 20.9 / 12.6 / 25, 1024 x 4096 -> 1024 73 / 39 / 23).  Where x is rounded on its way in, every
+    // workgroup rounds it again, so they get wider in n first (16 x 4096 -> 8192 19.7 / 14.9 for 16 / 32 columns).
+    const long f = ((a.M + 15) / 16) * ((a.N + 15) / 16), cus = f8_cus();
+    if constexpr (XK < X_BF16) {
+        if (f <= 2 * cus) return launch_direct<XK, TO, 1, 1, 8>(a, s);
+        return f <= 8 * cus ? launch_direct<XK, TO, 2, 2, 4>(a, s) : launch_direct<XK, TO, 4, 4, 4>(a, s);
+    } else {
+        if (f <= cus) return launch_direct<XK, TO, 1, 1, 8>(a, s);
+        return a.M <= 16 ? launch_direct<XK, TO, 1, 2, 16>(a, s) : launch_direct<XK, TO, 2, 2, 8>(a, s);
+    }
 }
 
 }  // namespace mad

@@ -385,7 +385,7 @@ static F8WgradPlan wgrad_plan(long rows, int N, int K, bool tiled) {
     p.ntiles = (N + p.tile - 1) / p.tile; p.ktiles = (K + p.tile - 1) / p.tile;
     // two workgroups of the small tile fit a unit at a time: no more shares than fill them once
     long s = p.tile == 256 ? 1 : 2 * cus / tiles(p.tile);
-    const long most = (rows + 255) / 256;
+    const long most = (rows + 63) / 64;
     if (s > most) s = most;
     p.splits = (int)(s < 1 ? 1 : s);
     p.per = ((rows + p.splits - 1) / p.splits + 63) / 64 * 64;

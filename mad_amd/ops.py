@@ -8,6 +8,8 @@ from __future__ import annotations
 
 from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
+import math
+
 import torch
 
 from . import _lib
@@ -813,22 +815,29 @@ def _scale_pitch(c: int) -> int:
     return (-(-c // FP8_BLOCK) + 3) & -4
 
 
+# the current stream's handle and the current device's index without the objects around them: the smallest of these calls are shorter
+# than torch.cuda.current_stream() takes
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
 def _fp8_call(name: str, t: Tensor, *args) -> None:
     """One entry point on the device of ``t``, on the stream that is current there."""
-    if t.device.index == torch.cuda.current_device():
-        check(getattr(lib, name)(*args, torch.cuda.current_stream().cuda_stream), name)
-        return
-    with torch.cuda.device(t.device):
-        check(getattr(lib, name)(*args, torch.cuda.current_stream().cuda_stream), name)
+    i = t.get_device()
+    if i == _current_device():
+        status = getattr(lib, name)(*args, _raw_stream(i))
+    else:
+        with torch.cuda.device(i):
+            status = getattr(lib, name)(*args, _raw_stream(i))
+    if status:
+        check(status, name)
 
 
 def _fp8_rows(shape: Sequence[int], what: str) -> Tuple[int, int]:
-    if len(shape) < 1 or shape[-1] < 1 or shape[-1] > _lib.FP8_MAX_WIDTH:
+    if not shape or not 1 <= shape[-1] <= _lib.FP8_MAX_WIDTH:
         raise ValueError(f"{what}: needs 1 to {_lib.FP8_MAX_WIDTH} columns, got shape {tuple(shape)}")
-    rows = 1
-    for n in shape[:-1]:
-        rows *= n
-    return rows, shape[-1]
+    return (shape[0] if len(shape) == 2 else math.prod(shape[:-1])), shape[-1]
 
 
 def _fp8_empty(rows: int, c: int, fmt: str, device) -> Tuple[Tensor, Tensor]:
@@ -844,7 +853,7 @@ def _fp8_check(p: Fp8Tensor, what: str) -> Tuple[int, int, int]:
     _dev(p.q, p.scale)
     if p.q.dtype not in _FP8_CODES or p.scale.dtype != torch.uint8:
         raise TypeError(f"{what}: a packed tensor is float8_e4m3fn or float8_e5m2 with uint8 scales, got {p.q.dtype} / {p.scale.dtype}")
-    if tuple(p.q.shape) != (rows, _pitch(c)) or tuple(p.scale.shape) != (rows, _scale_pitch(c)):
+    if p.q.shape != (rows, _pitch(c)) or p.scale.shape != (rows, _scale_pitch(c)):
         raise ValueError(f"{what}: packed parts {tuple(p.q.shape)} / {tuple(p.scale.shape)} do not belong to shape {tuple(p.shape)}")
     return rows, c, _FP8_CODES[p.q.dtype]
 
@@ -854,7 +863,7 @@ def _fp8_weight_check(q: Optional[Tensor], scale: Optional[Tensor], n: int, k: i
         raise ValueError(f"{what}: the weight was packed without its transposed copy")
     if q.dtype != torch.float8_e4m3fn or scale.dtype != torch.uint8:
         raise TypeError(f"{what}: a packed weight is float8_e4m3fn with uint8 scales, got {q.dtype} / {scale.dtype}")
-    if tuple(q.shape) != (n, _pitch(k)) or tuple(scale.shape) != (-(-n // FP8_BLOCK), _scale_pitch(k)):
+    if q.shape != (n, _pitch(k)) or scale.shape != (-(-n // FP8_BLOCK), _scale_pitch(k)):
         raise ValueError(f"{what}: packed parts {tuple(q.shape)} / {tuple(scale.shape)} do not belong to a weight ({n}, {k})")
 
 
@@ -866,7 +875,7 @@ def pack_fp8(x: Tensor, fmt: str = "e4m3") -> Fp8Tensor:
     rows, c = _fp8_rows(x.shape, "pack_fp8")
     q, scale = _fp8_empty(rows, c, fmt, x.device)
     _fp8_call("mad_pack_fp8", x, _ptr(x), code, _FP8_TYPES[fmt][1], rows, c, _ptr(q), _ptr(scale))
-    return Fp8Tensor(q, scale, tuple(x.shape), x.dtype)
+    return Fp8Tensor(q, scale, x.shape, x.dtype)
 
 
 def unpack_fp8(p: Fp8Tensor) -> Tensor:
@@ -896,7 +905,7 @@ def gn_apply_save(x: Tensor, coef: Tensor, act: bool, drop_seed: int = 0, drop_p
     q, scale = _fp8_empty(rows, C, "e4m3", x.device)
     _fp8_call("mad_gn_apply_save_fp8", x, _ptr(x), _ptr(coef), _ptr(y), _ptr(q), _ptr(scale), code, B, H * W_, C, int(act),
               drop_seed, float(drop_p))
-    return y, Fp8Tensor(q, scale, tuple(x.shape), x.dtype)
+    return y, Fp8Tensor(q, scale, x.shape, x.dtype)
 
 
 def gn_apply_restore(p: Fp8Tensor, coef: Tensor, act: bool, drop_seed: int = 0, drop_p: float = 0.0) -> Tuple[Tensor, Tensor]:
@@ -935,7 +944,7 @@ def pack_weight_fp8(w: Tensor, transposed: bool = False) -> Fp8Weight:
 
 # Rows up to which linear_fp8 rounds x inside the product's own launch: every workgroup rounds the rows it reads again, which
 # costs less than a launch while there are few.
-FP8_FUSED_ROWS = 64
+FP8_FUSED_ROWS = 32
 
 
 def _linear_fp8(x: Union[Tensor, Fp8Tensor], rows: int, k: int, dtype: torch.dtype, q: Tensor, scale: Tensor, n: int,
@@ -973,12 +982,14 @@ def linear_fp8(x: Union[Tensor, Fp8Tensor], w: Fp8Weight, bias: Optional[Tensor]
         rows, c = _fp8_rows(x.shape, "linear_fp8")
     if c != K:
         raise ValueError(f"linear_fp8: x has {c} columns, the weight {K}")
-    shape, dtype = tuple(x.shape[:-1]) + (N,), x.dtype
-    if residual is not None and tuple(residual.shape) != shape:
+    shape, dtype = (*x.shape[:-1], N), x.dtype
+    if residual is not None and residual.shape != shape:
         raise ValueError(f"linear_fp8: residual has shape {tuple(residual.shape)}, y {shape}")
     if not isinstance(x, Fp8Tensor) and (save or rows > FP8_FUSED_ROWS):
         x = pack_fp8(x)
-    y = _linear_fp8(x, rows, K, dtype, w.q, w.scale, N, bias, residual, "linear_fp8").view(shape)
+    y = _linear_fp8(x, rows, K, dtype, w.q, w.scale, N, bias, residual, "linear_fp8")
+    if len(shape) != 2:
+        y = y.view(shape)
     if not save:
         return y
     return y, x

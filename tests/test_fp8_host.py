@@ -151,7 +151,7 @@ def test_c_linear_refusals():
     _refused(call(w=None), "null")
     _refused(call(w=ODD), "aligned")
     _refused(call(x=ODD), "aligned")
-    _refused(call(rows=1 << 40, N=1 << 20), "workgroups")
+    _refused(call(rows=1 << 40, N=1 << 20), "need more")
     assert call(rows=0) == 0
 
 
