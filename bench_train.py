@@ -35,6 +35,8 @@ def parse_args():
                    help="fused: the accum*batch images of one optimizer step run as ONE batch (same mean gradient; "
                         "288 GB of HBM hold its activations); micro: accum separate micro-batches as the reference runs them")
     p.add_argument("--precision", default="bf16", choices=["bf16", "fp32"])
+    p.add_argument("--checkpoints", default=None, choices=["fp8"], help="keep activations for the backward in 8 bits")
+    p.add_argument("--products", default=None, choices=["fp8"], help="attention projections on 8-bit operands")
     p.add_argument("--no-cpu-baseline", action="store_true")
     return p.parse_args()
 
@@ -144,7 +146,8 @@ def main():
     model = model.to(dev).train()
     spec = model.spec
     R = spec.img_resolution
-    tr = UNetTrainer(model.unet, lr=float(cfg.TRAIN.LR), dropout=0.10, seed=rank)
+    tr = UNetTrainer(model.unet, lr=float(cfg.TRAIN.LR), dropout=0.10, seed=rank, checkpoints=args.checkpoints,
+                     products=args.products)
     betas = torch.linspace(float(cfg.TRAIN.NOISE_SCHEDULER.BETA_START), float(cfg.TRAIN.NOISE_SCHEDULER.BETA_END),
                            int(cfg.TRAIN.TIME_STEPS), dtype=torch.float32)
     alphas = torch.cumprod(1.0 - betas, 0).to(dev)
@@ -204,6 +207,7 @@ def main():
                                    + ", dropout 0.1, epsilon prediction, MSE, AdamW(0.95, 0.999) + EMA, random-init "
                                      "(seeded) weights",
                        "batch_per_gpu": B, "accumulation": accum, "passes_per_step": passes, "resolution": R,
+                       "checkpoints": args.checkpoints, "products": args.products,
                        "parallelism": f"dp{world}", "peak_hbm_gib": torch.cuda.max_memory_allocated(dev) / 2 ** 30,
                        "parameters": int(tr.flat.numel()), "gflop_per_image_forward": f_fwd / 1e9,
                        "final_loss": loss},

@@ -61,9 +61,11 @@ def _dgrad_weight(e: dict, key: str) -> Tensor:
 
 
 class _Saved:
-    """What one UNetBlock's backward needs from its forward."""
+    """What one UNetBlock's backward needs from its forward.  With 8-bit checkpoints x, skip, h and y are ``ops.Fp8Tensor``
+    and h0, h1, hn (the normalised inputs of the convolutions, which follow from them) are not kept; hn8 and att8 are the
+    packed inputs of 8-bit products."""
     __slots__ = ("x", "x_part", "skip", "skip_part", "c0", "h0", "h", "h_part", "c1", "h1", "seed", "y", "y_part",
-                 "c2", "hn", "qkv", "att", "lse")
+                 "c2", "hn", "qkv", "att", "lse", "hn8", "att8")
 
     def __init__(self):
         for k in self.__slots__:
@@ -71,12 +73,22 @@ class _Saved:
 
 
 class UNetTrainer:
-    """Owns flat fp32 parameter / gradient / AdamW / EMA buffers of a ``DhariwalUNet`` and runs training steps."""
+    """Owns flat fp32 parameter / gradient / AdamW / EMA buffers of a ``DhariwalUNet`` and runs training steps.
+
+    ``checkpoints="fp8"`` keeps the activations between forward and backward in 8 bits (one power-of-two scale per pixel and
+    128 channels) and restores them block by block: the forward's results do not change, the gradients are those of the
+    rounded activations.  The attention's q, k, v and output stay in the compute type: its scores are exponentiated, and its
+    tensors are few (32x32 pixels at most).  ``products="fp8"`` runs the qkv and output projections of the attention blocks, and
+    their data gradients, on 8-bit operands (``ops.linear_fp8``); master weights, weight gradients and sums stay fp32."""
 
     def __init__(self, unet: DhariwalUNet, lr: float = 1e-4, betas=(0.95, 0.999), eps: float = 1e-7,
                  weight_decay: float = 1e-2, dropout: float = 0.10, ema: bool = True, ema_max_decay: float = 0.9999,
                  ema_inv_gamma: float = 1.0, ema_power: float = 0.75, process_group=None, bucket_mb: float = 128,
-                 seed: int = 0):
+                 seed: int = 0, checkpoints: Optional[str] = None, products: Optional[str] = None):
+        for name, v in (("checkpoints", checkpoints), ("products", products)):
+            if v not in (None, "fp8"):
+                raise ValueError(f"UNetTrainer: {name} must be None or 'fp8', got {v!r}")
+        self.checkpoints, self.products = checkpoints, products
         self.unet = unet
         self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
         self.dropout = float(dropout)
@@ -194,6 +206,8 @@ class UNetTrainer:
                 e["qkv.w"].copy_(W[f"{n}.qkv.weight"].permute(0, 2, 3, 1)[e["qkv.idx"]])
                 e["qkv.b"].copy_(W[f"{n}.qkv.bias"][e["qkv.idx"]])
                 e.pop("qkv.w.T", None)
+                e.pop("qkv.w8", None)
+                e.pop("proj.w8", None)
         torch.cat([W[f"{b.name}.affine.weight"] for b in s.blocks()], 0, out=P["aff.w"])
         torch.cat([W[f"{b.name}.affine.bias"] for b in s.blocks()], 0, out=P["aff.b"])
         P["out.w"].copy_(W["out_conv.weight"].permute(0, 2, 3, 1))
@@ -284,9 +298,38 @@ class UNetTrainer:
     def _part(self, t: Tensor, part: Optional[Tensor]) -> Tensor:
         return part if part is not None else ops.gn_partial(t)
 
+    def _weight8(self, e: dict, key: str) -> "ops.Fp8Weight":
+        """The 8-bit copy of an attention projection, packed from the fp32 master when first used after an update; qkv's rows in
+        the working order (q, k, v of a head in one piece)."""
+        k8 = key + "8"
+        if k8 not in e:
+            w = self._param[f"{e['spec'].name}.{key[:-1]}weight"].reshape(-1, e["spec"].out_channels)
+            e[k8] = ops.pack_weight_fp8(w[self._qkv_order(e["spec"])] if key == "qkv.w" else w, transposed=True)
+        return e[k8]
+
+    def _qkv_order(self, b: BlockSpec) -> Tensor:
+        return torch.arange(3 * b.out_channels, device=self.flat.device).reshape(b.num_heads, 64, 3).permute(0, 2, 1).reshape(-1)
+
+    # ------------------------------------------------------------------ 8-bit checkpoints
+    def _keep(self, x: Tensor, coef: Tensor, act: bool, drop_seed: int = 0, drop_p: float = 0.0):
+        """(gn_apply of x, what the backward keeps of x, what it keeps of the result)."""
+        if self.checkpoints:
+            y, x8 = ops.gn_apply_save(x, coef, act, drop_seed=drop_seed, drop_p=drop_p)
+            return y, x8, None
+        y = ops.gn_apply(x, coef, act=act, drop_seed=drop_seed, drop_p=drop_p)
+        return y, x, y
+
+    @staticmethod
+    def _restore(x, y: Optional[Tensor], coef: Tensor, act: bool, drop_seed: int = 0, drop_p: float = 0.0):
+        """The pair (x, gn_apply of x) of ``_keep``."""
+        if isinstance(x, ops.Fp8Tensor):
+            return ops.gn_apply_restore(x, coef, act, drop_seed=drop_seed, drop_p=drop_p)
+        return x, y
+
     # ------------------------------------------------------------------ forward (train mode)
     def _block_fwd(self, e: dict, x: Tensor, x_part: Optional[Tensor], skip: Optional[Tensor],
-                   skip_part: Optional[Tensor], ada: Tensor, ada_total: int):
+                   skip_part: Optional[Tensor], ada: Tensor, ada_total: int, skip_kept=None):
+        """``skip_kept``: what an earlier block has kept of ``skip`` as its own input (8-bit checkpoints)."""
         b: BlockSpec = e["spec"]
         sv = _Saved()
         hw_in, hw_out = b.res_in ** 2, b.res_out ** 2
@@ -296,22 +339,30 @@ class UNetTrainer:
         sv.c0 = ops.gn_finalize(sv.x_part, hw_in, e["norm0.g"], e["norm0.b"], gn_groups(b.in_channels), GN_EPS,
                                 partial2=sv.skip_part)
         ada_v = ada[:, e["ada_off"]:]
-        sv.h0 = ops.gn_apply(x, sv.c0, act=True, x2=skip, pool=b.down)
-        sv.h, sv.h_part = self._conv3(sv.h0, e["conv0.w"], e["conv0.b"], upsample=b.up)
-        sv.h_part = self._part(sv.h, sv.h_part)
+        if skip is None and not b.down:
+            h0, sv.x, sv.h0 = self._keep(x, sv.c0, True)
+        else:
+            h0 = sv.h0 = ops.gn_apply(x, sv.c0, act=True, x2=skip, pool=b.down)
+            if self.checkpoints:
+                sv.x, sv.h0 = ops.pack_fp8(x), None
+                sv.skip = None if skip is None else (skip_kept if skip_kept is not None else ops.pack_fp8(skip))
+        h, sv.h_part = self._conv3(h0, e["conv0.w"], e["conv0.b"], upsample=b.up)
+        del h0
+        sv.h_part = self._part(h, sv.h_part)
         sv.c1 = ops.gn_finalize(sv.h_part, hw_out, e["norm1.g"], e["norm1.b"], gn_groups(b.out_channels), GN_EPS,
                                 ada=ada_v, ada_stride=ada_total)
         if self.dropout > 0.0:                   # dropout fused into the apply pass; the backward rebuilds the mask
             self._drop_calls += 1
             # one mask per (optimizer step, micro-batch, layer): accumulated micro-batches draw independently
             sv.seed = (self.seed << 32) ^ (self.step_count << 16) ^ (self._micro_index << 10) ^ self._drop_calls
-        sv.h1 = ops.gn_apply(sv.h, sv.c1, act=True, drop_seed=sv.seed or 0, drop_p=self.dropout if sv.seed is not None else 0.0)
+        h1, sv.h, sv.h1 = self._keep(h, sv.c1, True, drop_seed=sv.seed or 0, drop_p=self.dropout if sv.seed is not None else 0.0)
+        del h
         cm = 32 if x.dtype == torch.bfloat16 else 16
         if (b.skip_conv and self.FUSE_SKIP and ops.fused_conv_ok(b.res_out, b.res_out, b.out_channels)
                 and b.out_channels % cm == 0 and x.shape[3] % cm == 0 and (skip is None or skip.shape[3] % cm == 0)):
             # the 1x1 projection of the block input rides in conv1's launch (more reduction steps of the same
             # accumulators) instead of a pass of its own that writes a residual tensor conv1 then re-reads
-            sv.y, sv.y_part = ops.conv3x3_fused(sv.h1, e["conv1.w"], e["conv1+skip.b"], coef=None, want_stats=True,
+            y, sv.y_part = ops.conv3x3_fused(h1, e["conv1.w"], e["conv1+skip.b"], coef=None, want_stats=True,
                                                 skip=(x, skip, e["skip.w2d"]))
             res = mode = None
         elif b.skip_conv:
@@ -323,17 +374,29 @@ class UNetTrainer:
         else:
             res, mode = x, _lib.RES_SAME
         if mode is not None:
-            sv.y, sv.y_part = self._conv3(sv.h1, e["conv1.w"], e["conv1.b"], residual=res, res_mode=mode)
-        out, out_part = sv.y, sv.y_part
+            y, sv.y_part = self._conv3(h1, e["conv1.w"], e["conv1.b"], residual=res, res_mode=mode)
+        del h1
+        out, out_part = y, sv.y_part
         if b.attention:
-            sv.y_part = self._part(sv.y, sv.y_part)
+            sv.y_part = self._part(y, sv.y_part)
             sv.c2 = ops.gn_finalize(sv.y_part, hw_out, e["norm2.g"], e["norm2.b"], gn_groups(b.out_channels), GN_EPS)
-            sv.hn = ops.gn_apply(sv.y, sv.c2, act=False)
-            sv.qkv = ops.conv2d(sv.hn, e["qkv.w"], e["qkv.b"])
+            hn, sv.y, sv.hn = self._keep(y, sv.c2, False)
+            if self.products:
+                sv.qkv, sv.hn8 = ops.linear_fp8(hn, self._weight8(e, "qkv.w"), bias=e["qkv.b"], save=True)
+                sv.hn = None
+            else:
+                sv.qkv = ops.conv2d(hn, e["qkv.w"], e["qkv.b"])
+            del hn
             sv.att, sv.lse = ops.attention(sv.qkv, b.num_heads, want_lse=True)
-            stats = hw_out % 64 == 0
-            r = ops.conv2d(sv.att, e["proj.w"], e["proj.b"], residual=sv.y, res_mode=_lib.RES_SAME, want_stats=stats)
-            out, out_part = r if stats else (r, None)
+            if self.products:
+                out, sv.att8 = ops.linear_fp8(sv.att, self._weight8(e, "proj.w"), bias=e["proj.b"], residual=y, save=True)
+                out_part = None
+            else:
+                stats = hw_out % 64 == 0
+                r = ops.conv2d(sv.att, e["proj.w"], e["proj.b"], residual=y, res_mode=_lib.RES_SAME, want_stats=stats)
+                out, out_part = r if stats else (r, None)
+        elif not self.checkpoints:
+            sv.y = y
         return out, out_part, sv
 
     def forward(self, x: Tensor, t: Tensor, class_labels: Optional[Tensor]):
@@ -363,7 +426,7 @@ class UNetTrainer:
 
         h = ops.conv_in(x, P["in.w"], P["in.b"], dt)
         h_part = None
-        skips = [(h, None)]
+        skips = [(h, None)]                  # entry i is the input of block i
         saved: List[_Saved] = []
         n_enc = len(s.enc)
         for i, e in enumerate(P["blocks"]):
@@ -373,18 +436,21 @@ class UNetTrainer:
                 skips.append((h, h_part))
             else:
                 sk, sk_part = skips.pop() if b.cat_skip else (None, None)
-                h, h_part, sv = self._block_fwd(e, h, h_part, sk, sk_part, ada, total)
+                # that tensor was the input of block len(skips), which has packed it already (unless it is this block's own input)
+                kept = saved[len(skips)].x if self.checkpoints and sk is not None and len(skips) < i else None
+                h, h_part, sv = self._block_fwd(e, h, h_part, sk, sk_part, ada, total, skip_kept=kept)
+                del sk
             saved.append(sv)
         R = s.img_resolution
         h_part = self._part(h, h_part)
         c = ops.gn_finalize(h_part, R * R, P["out_norm.g"], P["out_norm.b"], gn_groups(s.final_channels), GN_EPS)
-        hact = ops.gn_apply(h, c, act=True)
+        hact, h_kept, hact_kept = self._keep(h, c, True)
         fused_out = R % 16 == 0 and s.out_channels <= 32 and s.final_channels % 32 == 0
         if fused_out:
             pred = ops.conv_out_fused(hact, P["out.w32"], P["out.b"], s.out_channels, coef=None)
         else:
             pred = ops.conv_out(hact, P["out.w"], P["out.b"])
-        tape.update(saved=saved, h_last=h, h_last_part=h_part, c_out=c, hact=hact)
+        tape.update(saved=saved, h_last=h_kept, h_last_part=h_part, c_out=c, hact=hact_kept)
         return pred, tape
 
     # ------------------------------------------------------------------ backward
@@ -399,14 +465,28 @@ class UNetTrainer:
         ada_v, dada_v = ada[:, e["ada_off"]:], dada[:, e["ada_off"]:]
         dy = dout
         if b.attention:
-            self._wgrad(f"{n}.proj.weight", sv.att, dout, 1, bias=f"{n}.proj.bias")
-            datt = ops.conv2d(dout, _dgrad_weight(e, "proj.w"), None)
+            if self.products:
+                y, hn = ops.unpack_fp8(sv.y) if self.checkpoints else sv.y, None
+            else:
+                y, hn = self._restore(sv.y, sv.hn, sv.c2, False)
+            if self.products:
+                datt, _, _ = ops.linear_fp8_backward(dout, sv.att8, self._weight8(e, "proj.w"), dw=self.grads[f"{n}.proj.weight"],
+                                                     dbias=self.grads[f"{n}.proj.bias"], accumulate=self._accumulating)
+                self._mark(f"{n}.proj.weight")
+                self._mark(f"{n}.proj.bias")
+            else:
+                self._wgrad(f"{n}.proj.weight", sv.att, dout, 1, bias=f"{n}.proj.bias")
+                datt = ops.conv2d(dout, _dgrad_weight(e, "proj.w"), None)
             dqkv = ops.attention_backward(sv.qkv, sv.att, datt, sv.lse, b.num_heads)
             # the packed qkv rows are a permutation of the reference's (model.py:359-363): undo it for the masters
-            co, heads = b.out_channels, b.num_heads
-            idx = torch.arange(3 * co, device=dout.device).reshape(heads, 64, 3).permute(0, 2, 1).reshape(-1)
-            gb = torch.empty((3 * co,), dtype=torch.float32, device=dout.device)
-            gw = ops.conv_wgrad(sv.hn, dqkv, 1, dbias=gb)
+            co = b.out_channels
+            idx = self._qkv_order(b)
+            if self.products:
+                dhn, gw, gb = ops.linear_fp8_backward(dqkv, sv.hn8, self._weight8(e, "qkv.w"))
+                gw = gw.view(3 * co, co, 1, 1)
+            else:
+                gb = torch.empty((3 * co,), dtype=torch.float32, device=dout.device)
+                gw = ops.conv_wgrad(hn, dqkv, 1, dbias=gb)
             if self._accumulating:
                 self.grads[f"{n}.qkv.weight"].index_add_(0, idx, gw)
                 self.grads[f"{n}.qkv.bias"].index_add_(0, idx, gb)
@@ -415,19 +495,21 @@ class UNetTrainer:
                 self.grads[f"{n}.qkv.bias"].index_copy_(0, idx, gb)
             self._mark(f"{n}.qkv.weight")
             self._mark(f"{n}.qkv.bias")
-            dhn = ops.conv2d(dqkv, _dgrad_weight(e, "qkv.w"), None)
-            dy, _, dg, db = ops.gn_backward(sv.y, dhn, sv.c2, sv.y_part, e["norm2.g"], e["norm2.b"],
+            if not self.products:
+                dhn = ops.conv2d(dqkv, _dgrad_weight(e, "qkv.w"), None)
+            dy, _, dg, db = ops.gn_backward(y, dhn, sv.c2, sv.y_part, e["norm2.g"], e["norm2.b"],
                                             gn_groups(b.out_channels), GN_EPS, act=False, add1=dout,
                                             dgamma=self.grads[f"{n}.norm2.weight"], dbeta=self.grads[f"{n}.norm2.bias"],
                                             accumulate=self._accumulating)
             self._mark(f"{n}.norm2.weight")
             self._mark(f"{n}.norm2.bias")
         # conv1 and the AdaGN in front of it
-        self._wgrad(f"{n}.conv1.weight", sv.h1, dy, 3, bias=f"{n}.conv1.bias",
-                    same_bias=f"{n}.skip.bias" if b.skip_conv else None)
         drop_p = self.dropout if sv.seed is not None else 0.0
-        dh1, gs1 = self._dgrad3_sums(dy, _dgrad_weight(e, "conv1.w"), sv.h, sv.c1, drop_seed=sv.seed or 0, drop_p=drop_p)
-        dh, _, dg, db = ops.gn_backward(sv.h, dh1, sv.c1, sv.h_part, e["norm1.g"], e["norm1.b"],
+        h, h1 = self._restore(sv.h, sv.h1, sv.c1, True, drop_seed=sv.seed or 0, drop_p=drop_p)
+        self._wgrad(f"{n}.conv1.weight", h1, dy, 3, bias=f"{n}.conv1.bias",
+                    same_bias=f"{n}.skip.bias" if b.skip_conv else None)
+        dh1, gs1 = self._dgrad3_sums(dy, _dgrad_weight(e, "conv1.w"), h, sv.c1, drop_seed=sv.seed or 0, drop_p=drop_p)
+        dh, _, dg, db = ops.gn_backward(h, dh1, sv.c1, sv.h_part, e["norm1.g"], e["norm1.b"],
                                         gn_groups(b.out_channels), GN_EPS, act=True, ada=ada_v, ada_stride=ada_total,
                                         dada=dada_v, drop_seed=sv.seed or 0, drop_p=drop_p,
                                         dgamma=self.grads[f"{n}.norm1.weight"], dbeta=self.grads[f"{n}.norm1.bias"],
@@ -435,19 +517,26 @@ class UNetTrainer:
         self._mark(f"{n}.norm1.weight")
         self._mark(f"{n}.norm1.bias")
         # conv0 (input possibly resampled after norm0 + SiLU)
-        self._wgrad(f"{n}.conv0.weight", sv.h0, dh, 3, upsample=b.up, bias=f"{n}.conv0.bias")
+        del h, h1, dh1
+        if isinstance(sv.x, ops.Fp8Tensor) and (sv.skip is not None or b.down):
+            x, skip = ops.unpack_fp8(sv.x), None if sv.skip is None else ops.unpack_fp8(sv.skip)
+            h0 = ops.gn_apply(x, sv.c0, act=True, x2=skip, pool=b.down)
+        else:
+            skip = sv.skip
+            x, h0 = self._restore(sv.x, sv.h0, sv.c0, True)
+        self._wgrad(f"{n}.conv0.weight", h0, dh, 3, upsample=b.up, bias=f"{n}.conv0.bias")
         mode0 = ops.GRAD_FROM_DOUBLE if b.up else (ops.GRAD_FROM_HALF if b.down else ops.GRAD_SAME)
         if mode0 == ops.GRAD_SAME:
-            dh0, gs0 = self._dgrad3_sums(dh, _dgrad_weight(e, "conv0.w"), sv.x, sv.c0, gx2=sv.skip)
+            dh0, gs0 = self._dgrad3_sums(dh, _dgrad_weight(e, "conv0.w"), x, sv.c0, gx2=skip)
         else:                                # norm0 runs at the other resolution: its sums need the resampled gradient
             dh0, gs0 = self._dgrad3(dh, _dgrad_weight(e, "conv0.w")), None
         # the residual branch's gradient w.r.t. the block input
         if b.skip_conv:
-            if sv.skip is None:
-                self._wgrad(f"{n}.skip.weight", sv.x, dy, 1)
+            if skip is None:
+                self._wgrad(f"{n}.skip.weight", x, dy, 1)
             else:                            # the projection's input is the concatenation: one gradient per source
-                gsk, c1 = self.grads[f"{n}.skip.weight"], sv.x.shape[3]
-                for sl, src in ((slice(0, c1), sv.x), (slice(c1, None), sv.skip)):
+                gsk, c1 = self.grads[f"{n}.skip.weight"], x.shape[3]
+                for sl, src in ((slice(0, c1), x), (slice(c1, None), skip)):
                     g = ops.conv_wgrad(src, dy, 1)
                     if self._accumulating:
                         gsk[:, sl].add_(g)
@@ -459,13 +548,13 @@ class UNetTrainer:
             dres, res_mode = dy, mode0
         add2 = None
         if dskip_of_x is not None:
-            if sv.skip is not None:          # the extra gradient covers x's channels only: widen it with zeros
-                pad = torch.zeros_like(sv.skip)
+            if skip is not None:          # the extra gradient covers x's channels only: widen it with zeros
+                pad = torch.zeros_like(skip)
                 add2 = torch.cat([dskip_of_x, pad], dim=-1)
             else:
                 add2 = dskip_of_x
-        dx, dskip, dg, db = ops.gn_backward(sv.x, dh0, sv.c0, sv.x_part, e["norm0.g"], e["norm0.b"],
-                                            gn_groups(b.in_channels), GN_EPS, act=True, x2=sv.skip,
+        dx, dskip, dg, db = ops.gn_backward(x, dh0, sv.c0, sv.x_part, e["norm0.g"], e["norm0.b"],
+                                            gn_groups(b.in_channels), GN_EPS, act=True, x2=skip,
                                             stat2=sv.skip_part, dy_mode=mode0, add1=dres, add1_mode=res_mode,
                                             add2=add2,
                                             dgamma=self.grads[f"{n}.norm0.weight"], dbeta=self.grads[f"{n}.norm0.bias"],
@@ -482,6 +571,7 @@ class UNetTrainer:
         B = dpred.shape[0]
         total = P["aff.total"]
         dev = dpred.device
+        h_last, hact = self._restore(tape["h_last"], tape["hact"], tape["c_out"], True)
         # out_conv: weight gradient on the generic kernel, data gradient through the 3x3 kernel on a
         # channel-padded NHWC copy of dpred
         self._set("out_conv.bias", dpred.sum((0, 2, 3)))
@@ -491,18 +581,19 @@ class UNetTrainer:
         dp[..., :Co] = dpred.permute(0, 2, 3, 1).to(dt)
         if dt == torch.bfloat16:
             # the 3 image channels zero-padded to one 32-channel MFMA block: the general weight-gradient kernel
-            self._set("out_conv.weight", ops.conv_wgrad(tape["hact"], dp, 3)[:Co])
+            self._set("out_conv.weight", ops.conv_wgrad(hact, dp, 3)[:Co])
         else:
-            self._set("out_conv.weight", ops.conv_wgrad_edge(tape["hact"], False, dpred, True, 3))
+            self._set("out_conv.weight", ops.conv_wgrad_edge(hact, False, dpred, True, 3))
         wT = torch.zeros((Cf, 3, 3, pad_c), dtype=dt, device=dev)
         wT[..., :Co] = P["out.w"].flip(1, 2).permute(3, 1, 2, 0).to(dt)
-        dhact, gs = self._dgrad3_sums(dp, wT, tape["h_last"], tape["c_out"])
-        dh, _, dg, db = ops.gn_backward(tape["h_last"], dhact, tape["c_out"], tape["h_last_part"], P["out_norm.g"],
+        dhact, gs = self._dgrad3_sums(dp, wT, h_last, tape["c_out"])
+        dh, _, dg, db = ops.gn_backward(h_last, dhact, tape["c_out"], tape["h_last_part"], P["out_norm.g"],
                                         P["out_norm.b"], gn_groups(Cf), GN_EPS, act=True,
                                         dgamma=self.grads["out_norm.weight"], dbeta=self.grads["out_norm.bias"],
                                         accumulate=self._accumulating, gsum=gs)
         self._mark("out_norm.weight")
         self._mark("out_norm.bias")
+        del h_last, hact, dhact
 
         dada = torch.zeros_like(tape["ada"])
         saved: List[_Saved] = tape["saved"]

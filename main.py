@@ -38,6 +38,8 @@ def parse_args(argv=None):
     parser.add_argument("--save-file-name", default="generated.png", type=str)
     parser.add_argument("--synthetic", default=0, type=int, help="train on this many generated images")
     parser.add_argument("--precision", default="bf16", choices=["bf16", "fp32"])
+    parser.add_argument("--checkpoints", default=None, choices=["fp8"], help="keep activations for the backward in 8 bits")
+    parser.add_argument("--products", default=None, choices=["fp8"], help="attention projections on 8-bit operands")
     parser.add_argument("--seed", default=0, type=int)
     parser.add_argument("--opts", nargs=argparse.REMAINDER, default=None, type=str)
     return parser.parse_args(argv)
@@ -236,7 +238,8 @@ def main(argv=None):
     if cfg.TRAIN.NOISE_SCHEDULER.PRED_TYPE != "epsilon":
         raise ValueError("Not supported prediction type.")                      # main.py:242-245
     trainer = UNetTrainer(model.unet, lr=cfg.TRAIN.LR, dropout=0.10, ema_max_decay=cfg.TRAIN.EMA_MAX_DECAY,
-                          ema_inv_gamma=cfg.TRAIN.EMA_INV_GAMMA, ema_power=cfg.TRAIN.EMA_POWER, seed=args.seed * 64 + rank)
+                          ema_inv_gamma=cfg.TRAIN.EMA_INV_GAMMA, ema_power=cfg.TRAIN.EMA_POWER, seed=args.seed * 64 + rank,
+                          checkpoints=args.checkpoints, products=args.products)
     start_iter = 0
     if cfg.TRAIN.RESUME is not None:
         assert osp.exists(cfg.TRAIN.RESUME), "Resume file not found."

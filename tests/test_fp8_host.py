@@ -73,6 +73,14 @@ def test_weights_that_do_not_fit_are_refused():
         ops.linear_fp8(torch.zeros(4, 40), w._replace(q=w.q.view(torch.float8_e5m2)))
 
 
+def test_trainer_options_are_checked():
+    from mad_amd.train import UNetTrainer
+    with pytest.raises(ValueError, match="checkpoints"):
+        UNetTrainer(None, checkpoints="fp4")
+    with pytest.raises(ValueError, match="products"):
+        UNetTrainer(None, products="int8")
+
+
 # ------------------------------------------------------------------ refusals of the C entry points (nothing is launched)
 def _lib():
     from mad_amd import _lib
