@@ -475,6 +475,14 @@ int mad_pack_weight_fp8(const void* w, int dtype, int N, int K, void* q, void* s
 int mad_linear_fp8(const void* x, int x_type, const void* x_scale, const void* w, const void* w_scale,
                    const float* bias, const void* residual, void* y, int dtype, long rows, int K, int N, void* stream);
 
+/* mad_pack_fp8 of x in `fmt` and mad_linear_fp8 of the result in one call: y, and the packed x in q, scale.  Long inputs of
+ * few columns (bf16, MAD_E4M3) are read once, by one launch.
+ * mad_linear_fp8_needs_pack: 1 where mad_linear_fp8 of an unpacked x would round it many times over and this call, with q and
+ * scale as scratch, is the faster one; 0 where mad_linear_fp8 needs no packed x. */
+int mad_linear_fp8_needs_pack(const void* x, int dtype, long rows, int K, int N);
+int mad_linear_fp8_save(const void* x, int dtype, int fmt, const void* w, const void* w_scale, const float* bias,
+                        const void* residual, void* y, void* q, void* scale, long rows, int K, int N, void* stream);
+
 /* dw (N, K) (+)= dy^T . x and db (N) (+)= column sums of dy (db may be NULL), fp32; x packed (rows, K), dy (rows, N) in
  * `dtype`, unrounded.  Partial sums are added in a fixed order (deterministic).  The data gradient is mad_linear_fp8 of the
  * packed dy and the transposed weight. */

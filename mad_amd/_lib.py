@@ -114,6 +114,8 @@ SIGNATURES = {
     "mad_gn_apply_restore_fp8": (c_int, [c_void_p] * 5 + [c_int] * 5 + [ctypes.c_ulonglong, c_float, c_void_p]),
     "mad_pack_weight_fp8": (c_int, [c_void_p, c_int, c_int, c_int] + [c_void_p] * 5),
     "mad_linear_fp8": (c_int, [c_void_p, c_int] + [c_void_p] * 6 + [c_int, ctypes.c_long, c_int, c_int, c_void_p]),
+    "mad_linear_fp8_needs_pack": (c_int, [c_void_p, c_int, ctypes.c_long, c_int, c_int]),
+    "mad_linear_fp8_save": (c_int, [c_void_p, c_int, c_int] + [c_void_p] * 7 + [ctypes.c_long, c_int, c_int, c_void_p]),
     "mad_linear_fp8_wgrad_workspace": (ctypes.c_size_t, [ctypes.c_long, c_int, c_int]),
     "mad_linear_fp8_wgrad": (c_int, [c_void_p, c_int, c_void_p, c_int] + [c_void_p] * 4 +
                              [ctypes.c_size_t, ctypes.c_long] + [c_int] * 4 + [c_void_p]),

@@ -407,6 +407,204 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
     }
 }
 
+// Row form: x in bf16 with rows of whole 16-byte pieces and at most four blocks, many rows.  A workgroup of four waves rounds its 128
+// rows once, through LDS into the fragments' registers (and to memory, if the packed x is wanted), and then walks the columns in
+// strips of 64, whose weights all waves read from LDS; LDS-DMA brings the next strip while one is multiplied and stored.  Bound
+// by HBM: x is read once, where packing first writes and reads a byte more per element, in another launch.
+struct F8RowArgs {
+    const bf16_t* x; const unsigned char* w; const unsigned char* ws; const float* bias; const bf16_t* residual; bf16_t* y;
+    unsigned char* q; unsigned char* scale;        // the packed x, or null
+    long M;
+    int K, N, shares;                              // shares of the columns: workgroups that round the same rows
+};
+
+template <int KB>
+__global__ __launch_bounds__(256, 2) void linear_fp8_rows_kernel(F8RowArgs a) {
+    constexpr int MF = 2, ROWS = 64 * MF, STRIP = 64 * KB * F8_BLOCK;      // rows of a workgroup, bytes of a strip
+    static_assert(2 * STRIP == ROWS * KB * F8_BLOCK, "the strips take the place of the rounded rows");
+    __shared__ __attribute__((aligned(16))) unsigned char xs[2 * STRIP];
+    __shared__ unsigned sc[ROWS];                  // the row's scales, a byte per block
+    __shared__ __attribute__((aligned(16))) float extra[2][2][64];         // of a strip: its bias, and the scales of its weights
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const long mt = blockIdx.x / a.shares;
+    const int share = (int)(blockIdx.x - mt * a.shares);
+    const long m0 = mt * ROWS;
+    const int mrem = a.M - m0 < ROWS ? (int)(a.M - m0) : ROWS;
+    const int pitch = f8_pitch(a.K), sp = f8_scale_pitch(a.K);
+
+    // ---- rounding: 16 lanes to a block, a pass of the workgroup is 16 rows
+    {
+        const int l = tid & 15, row0 = tid >> 4;
+        const auto xbuf = f8_resource(a.x + (size_t)m0 * a.K, mrem * a.K * 2);
+        const bool keep = a.q && share == 0;
+        constexpr int H = KB > 2 ? 4 : 8;                                  // passes whose loads are in flight together
+#pragma unroll
+        for (int h0 = 0; h0 < ROWS / 16; h0 += H) {
+            uint4 v[KB][H];
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int b = 0; b < KB; ++b) {
+                    const int c = b * F8_BLOCK + 8 * l;
+                    v[b][h] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
+                        xbuf, c < a.K ? ((row0 + 16 * (h0 + h)) * a.K + c) * 2 : (int)F8_OUTSIDE, 0, 0));
+                }
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                const int row = row0 + 16 * (h0 + h);
+                unsigned scales = 0;
+#pragma unroll
+                for (int b = 0; b < KB; ++b) {
+                    const unsigned* w = &v[b][h].x;
+                    unsigned m = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const unsigned lo = w[e] & 0x7fffu, hi = w[e] >> 16 & 0x7fffu;
+                        m = lo < 0x7f80u && lo > m ? lo : m;
+                        m = hi < 0x7f80u && hi > m ? hi : m;
+                    }
+                    const unsigned s = f8_scale_byte<F8_E4M3>(row16_umax(m) << 16);
+                    const float scale = f8_scale(s);
+                    uint2 o;
+                    o.x = f8_cvt4_bf16<F8_E4M3>(w[0], w[1], scale);
+                    o.y = f8_cvt4_bf16<F8_E4M3>(w[2], w[3], scale);
+                    *reinterpret_cast<uint2*>(xs + (b * ROWS + row) * F8_BLOCK + (((l >> 1) ^ (row >> 1 & 7)) << 4) + (l & 1) * 8) = o;
+                    scales |= s << (8 * b);
+                    if (keep && row < mrem && b * F8_BLOCK + 8 * l < pitch)
+                        *reinterpret_cast<uint2*>(a.q + (size_t)(m0 + row) * pitch + b * F8_BLOCK + 8 * l) = o;
+                }
+#pragma unroll
+                for (int b = KB; b < 4; ++b) scales |= 127u << (8 * b);
+                if (l == 0) sc[row] = scales;
+                if (keep && l == 0 && row < mrem) *reinterpret_cast<unsigned*>(a.scale + (size_t)(m0 + row) * sp) = scales;
+            }
+        }
+    }
+    __syncthreads();
+
+    // ---- this wave's rows as fragments: chunks g and g + 4 of row r, as in the tiled form
+    i32x8 xf[KB][MF];
+    unsigned xsc[MF];
+    const int c_lo = (g ^ (r >> 1)) << 4, c_hi = c_lo ^ 64;
+#pragma unroll
+    for (int i = 0; i < MF; ++i) {
+        xsc[i] = sc[16 * (MF * wave + i) + r];
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            const unsigned char* p = xs + (b * ROWS + 16 * (MF * wave + i) + r) * F8_BLOCK;
+            xf[b][i] = pair16(*reinterpret_cast<const uint4*>(p + c_lo), *reinterpret_cast<const uint4*>(p + c_hi));
+        }
+    }
+
+    // ---- strips of 64 columns; this share's are a run of them.  In LDS: [block][64 rows of w][128 bytes]
+    const int strips = (a.N + 63) / 64, per = (strips + a.shares - 1) / a.shares;
+    const int first = share * per, end = first + per < strips ? first + per : strips;
+    const int lr = lane >> 3, chunk = (lane & 7) ^ ((4 * wave + (lr >> 1)) & 7);
+    const unsigned lds0 = lds_addr(xs), ex0 = lds_addr(extra);
+    auto load_strip = [&](int t, int buf) {        // a strip's 8 KB groups of 8 rows: each wave two of every block
+        const int nrem = a.N - 64 * t < 64 ? a.N - 64 * t : 64;
+        const u32x4 wb = f8_buffer(a.w + (size_t)(64 * t) * pitch, t < end ? (unsigned)(nrem * pitch) : 0u);
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            const unsigned off = b * F8_BLOCK + 16 * chunk < pitch ? (unsigned)((8 * wave + lr) * pitch + 16 * chunk) : F8_OUTSIDE;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                buf_lds16(wb, off + j * 32 * pitch, b * F8_BLOCK, lds0 + buf * STRIP + b * 64 * F8_BLOCK + (4 * j + wave) * 1024);
+        }
+        // by LDS-DMA as well: the wait for an ordinary load would wait for the strip in front of it
+        if (wave == 2) buf_lds4(f8_buffer((const unsigned char*)(a.bias + 64 * t), a.bias && t < end ? (unsigned)(nrem * 4) : 0u), lane * 4, 0, ex0 + buf * 512);
+        if (wave == 3) buf_lds4(f8_buffer(a.ws + (size_t)(64 * t / F8_BLOCK) * sp, t < end ? 4u : 0u), 0, 0, ex0 + buf * 512 + 256);
+    };
+    constexpr int STORES = MF * 2;
+    __syncthreads();                               // every wave has its rows: the strips may take their place
+    load_strip(first, 0);
+    bool counted = false;
+    for (int t = first; t < end; ++t) {
+        const int buf = (t - first) & 1;
+        if (counted) dma_wait_upto<STORES>(); else dma_wait_all();         // the strip is older than the stores of the one before
+        __syncthreads();
+        load_strip(t + 1, buf ^ 1);
+        const unsigned wsc = __float_as_uint(extra[buf][1][0]);
+        const int n = 64 * t + (g & 1) * 16 + (g >> 1) * 8;                 // this lane's first column when it stores, pair 0
+        float bias[2][8];
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int e = 0; e < 8; e += 4)
+                *reinterpret_cast<f32x4*>(&bias[p][e]) = *reinterpret_cast<const f32x4*>(&extra[buf][0][(n & 63) + 32 * p + e]);
+        const bool whole = 64 * t + 64 <= a.N && mrem == ROWS;
+        const long mb = m0 + 16 * MF * wave + r;
+        Piece8<bf16_t> res[MF][2];
+        if (a.residual && whole) {
+#pragma unroll
+            for (int i = 0; i < MF; ++i)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) res[i][p].load(a.residual + (mb + 16 * i) * a.N + n + 32 * p);
+        }
+        f32x4 acc[4][MF];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < MF; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        const unsigned char* st = xs + buf * STRIP + r * F8_BLOCK;
+        auto wfrag = [&](int b, int j) {
+            const unsigned char* p = st + (b * 64 + 16 * j) * F8_BLOCK;
+            return pair16(*reinterpret_cast<const uint4*>(p + c_lo), *reinterpret_cast<const uint4*>(p + c_hi));
+        };
+#define BLOCK(b)                                                                                                                     \
+    if constexpr (b < KB) {                                                                                                          \
+        _Pragma("unroll") for (int j = 0; j < 4; ++j) {                                                                              \
+            const i32x8 wf = wfrag(b, j);                                                                                            \
+            _Pragma("unroll") for (int i = 0; i < MF; ++i) acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(             \
+                wf, xf[b < KB ? b : 0][i], acc[j][i], F8_E4M3, F8_E4M3, b, (int)wsc, b, (int)xsc[i]);                                \
+        }                                                                                                                            \
+    }
+        BLOCK(0) BLOCK(1) BLOCK(2) BLOCK(3)
+#undef BLOCK
+        auto piece = [&](int i, int p, float* v) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[2 * p][i][e]), __float_as_uint(acc[2 * p + 1][i][e]),
+                                                                 false, false);
+                v[e] = __uint_as_float(sw[0]) + bias[p][e];
+                v[4 + e] = __uint_as_float(sw[1]) + bias[p][4 + e];
+            }
+        };
+        counted = whole;
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < MF; ++i)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    float v[8];
+                    piece(i, p, v);
+                    if (a.residual) res[i][p].add(v);
+                    store8<bf16_t>(a.y + (mb + 16 * i) * a.N + n + 32 * p, v);
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < MF; ++i)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    float v[8];
+                    piece(i, p, v);
+                    const int c = n + 32 * p;
+                    if (mb + 16 * i < a.M && c < a.N) {
+                        if (a.residual) {
+                            float f[8];
+                            load8_tail<bf16_t>(a.residual + (mb + 16 * i) * a.N + c, c, a.N, f);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) v[e] += f[e];
+                        }
+                        store8_tail<bf16_t>(a.y + (mb + 16 * i) * a.N + c, c, a.N, v);
+                    }
+                }
+        }
+    }
+    dma_wait_all();                                // the copies of the strip behind the last
+}
+
 template <int XK, typename TO, int MF, int NF, int NW> static int launch_direct(F8LinArgs a, hipStream_t s) {
     const long mtiles = (a.M + 16 * MF - 1) / (16 * MF);
     a.ntiles = (a.N + 16 * NF - 1) / (16 * NF);
@@ -459,6 +657,38 @@ template <int XK, typename TO> static int launch_linear(F8LinArgs a, hipStream_t
     }
 }
 
+// Where the row form serves: bf16 rows of whole pieces, four blocks at most (their fragments live in registers), rows enough for one
+// workgroup to a unit, and no more columns than pay (us, packing first / rows: 32768 x 256 -> 768 27 / 21, 65536 x 384 -> 384
+// 36 / 25, 32768 x 512 -> 2048 67 / 49, 40000 x 512 -> 4096 147 / 153).
+static bool rows_form_ok(const void* x, int dtype, long rows, int K, int N) {
+    return dtype == MAD_BF16 && K % 8 == 0 && K <= 4 * F8_BLOCK && ((uintptr_t)x & 15) == 0 && (rows + 127) / 128 >= f8_cus() && N <= 2048;
+}
+
+static F8RowArgs row_args(const void* x, const void* w, const void* ws, const float* bias, const void* residual, void* y, void* q,
+                          void* scale, long rows, int K, int N) {
+    F8RowArgs a;
+    a.x = (const bf16_t*)x; a.w = (const unsigned char*)w; a.ws = (const unsigned char*)ws; a.bias = bias;
+    a.residual = (const bf16_t*)residual; a.y = (bf16_t*)y; a.q = (unsigned char*)q; a.scale = (unsigned char*)scale;
+    a.M = rows; a.K = K; a.N = N; a.shares = 1;
+    return a;
+}
+
+static int launch_rows(F8RowArgs a, hipStream_t s) {
+    const long mtiles = (a.M + 127) / 128;
+    // with one workgroup to a unit its rounding, products and stores follow one another: two, of half the columns each, overlap
+    // (32768 x 256 -> 768 25 us with one share, 22 with two); with more, rounding twice costs more (65536 x 384 -> 384 25 / 36)
+    a.shares = mtiles < 2 * f8_cus() && a.N >= 256 ? 2 : 1;
+    MAD_REQUIRE(mtiles <= 0x7fffffffL, "mad_linear_fp8: %ld rows need more workgroups than a launch holds", a.M);
+    const dim3 grid((unsigned)(mtiles * a.shares));
+    switch (f8_blocks(a.K)) {
+        case 1: hipLaunchKernelGGL(linear_fp8_rows_kernel<1>, grid, dim3(256), 0, s, a); break;
+        case 2: hipLaunchKernelGGL(linear_fp8_rows_kernel<2>, grid, dim3(256), 0, s, a); break;
+        case 3: hipLaunchKernelGGL(linear_fp8_rows_kernel<3>, grid, dim3(256), 0, s, a); break;
+        default: hipLaunchKernelGGL(linear_fp8_rows_kernel<4>, grid, dim3(256), 0, s, a); break;
+    }
+    return check_launch("mad_linear_fp8");
+}
+
 }  // namespace mad
 
 using namespace mad;
@@ -476,6 +706,8 @@ extern "C" int mad_linear_fp8(const void* x, int x_type, const void* x_scale, co
     MAD_REQUIRE(x && w && w_scale && y && (!packed || x_scale), "mad_linear_fp8: null pointer");
     MAD_REQUIRE(f8_aligned(w, w_scale) && (!packed || f8_aligned(x, x_scale)),
                 "mad_linear_fp8: packed bytes must be 16-byte, scales 4-byte aligned");
+    if (!packed && rows_form_ok(x, dtype, rows, K, N))
+        return launch_rows(row_args(x, w, w_scale, bias, residual, y, nullptr, nullptr, rows, K, N), (hipStream_t)stream);
     F8LinArgs a;
     a.x = x; a.xs = (const unsigned char*)x_scale; a.w = (const unsigned char*)w; a.ws = (const unsigned char*)w_scale;
     a.bias = bias; a.residual = residual; a.y = y; a.M = rows; a.K = K; a.N = N; a.mtiles = a.ntiles = 0;
@@ -488,4 +720,24 @@ extern "C" int mad_linear_fp8(const void* x, int x_type, const void* x_scale, co
     if (x_type == MAD_E4M3) return launch_linear<X_E4M3, float>(a, s);
     if (x_type == MAD_E5M2) return launch_linear<X_E5M2, float>(a, s);
     return launch_linear<X_F32, float>(a, s);
+}
+
+// up to this many rows the direct form rounds x on its way in for less than a launch costs
+static constexpr long F8_FUSED_ROWS = 32;
+
+extern "C" int mad_linear_fp8_needs_pack(const void* x, int dtype, long rows, int K, int N) {
+    return rows > F8_FUSED_ROWS && !rows_form_ok(x, dtype, rows, K, N);
+}
+
+extern "C" int mad_linear_fp8_save(const void* x, int dtype, int fmt, const void* w, const void* w_scale, const float* bias,
+                                   const void* residual, void* y, void* q, void* scale, long rows, int K, int N, void* stream) {
+    MAD_REQUIRE(rows >= 0 && N > 0 && N <= MAD_FP8_MAX_WIDTH, "mad_linear_fp8_save: bad shape rows=%ld N=%d", rows, N);
+    if (fmt == MAD_E4M3 && K > 0 && rows_form_ok(x, dtype, rows, K, N)) {
+        MAD_REQUIRE(x && w && w_scale && y && q && scale, "mad_linear_fp8_save: null pointer");
+        MAD_REQUIRE(f8_aligned(w, w_scale) && f8_aligned(q, scale),
+                    "mad_linear_fp8_save: packed bytes must be 16-byte, scales 4-byte aligned");
+        return launch_rows(row_args(x, w, w_scale, bias, residual, y, q, scale, rows, K, N), (hipStream_t)stream);
+    }
+    if (int rc = mad_pack_fp8(x, dtype, fmt, rows, K, q, scale, stream)) return rc;
+    return mad_linear_fp8(q, fmt, scale, w, w_scale, bias, residual, y, dtype, rows, K, N, stream);
 }

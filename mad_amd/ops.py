@@ -942,29 +942,33 @@ def pack_weight_fp8(w: Tensor, transposed: bool = False) -> Fp8Weight:
     return Fp8Weight(q, scale, (N, K), qt, scale_t)
 
 
-# Rows up to which linear_fp8 rounds x inside the product's own launch: every workgroup rounds the rows it reads again, which
-# costs less than a launch while there are few.
-FP8_FUSED_ROWS = 32
-
-
-def _linear_fp8(x: Union[Tensor, Fp8Tensor], rows: int, k: int, dtype: torch.dtype, q: Tensor, scale: Tensor, n: int,
-                bias: Optional[Tensor], residual: Optional[Tensor], what: str) -> Tensor:
-    """y (rows, n) in ``dtype`` of an x whose parts are checked."""
+def _linear_fp8(x: Union[Tensor, Fp8Tensor], rows: int, k: int, fmt: str, keep: bool, q: Tensor, scale: Tensor, n: int,
+                bias: Optional[Tensor], residual: Optional[Tensor], what: str):
+    """(y (rows, n), x packed if ``keep``) of an x whose parts are checked."""
     packed = isinstance(x, Fp8Tensor)
-    xq, xs = (x.q, x.scale) if packed else (x, None)
-    _dev(xq, xs, q, scale, bias, residual)
+    xq = x.q if packed else x
+    _dev(xq, q, scale, bias, residual)
     if bias is not None and (bias.dtype != torch.float32 or bias.numel() != n):
         raise ValueError(f"{what}: bias must be fp32 with {n} elements")
-    y = torch.empty((rows, n), dtype=dtype, device=xq.device)
-    if residual is not None and (residual.dtype != dtype or residual.numel() != y.numel()):
-        raise ValueError(f"{what}: residual must be {dtype} with {y.numel()} elements")
+    y = torch.empty((rows, n), dtype=x.dtype, device=xq.device)
+    if residual is not None and (residual.dtype != x.dtype or residual.numel() != rows * n):
+        raise ValueError(f"{what}: residual must be {x.dtype} with {rows * n} elements")
     code = _dtype_code(y)
     end = TIMER.bracket("linear_fp8", 2.0 * rows * k * n)
-    _fp8_call("mad_linear_fp8", y, _ptr(xq), _FP8_CODES[xq.dtype] if packed else code, _ptr(xs), _ptr(q), _ptr(scale), _ptr(bias),
-              _ptr(residual), _ptr(y), code, rows, k, n)
+    if packed:
+        _fp8_call("mad_linear_fp8", y, xq.data_ptr(), _FP8_CODES[xq.dtype], x.scale.data_ptr(), q.data_ptr(), scale.data_ptr(), _ptr(bias),
+                  _ptr(residual), y.data_ptr(), code, rows, k, n)
+    elif keep or fmt != "e4m3" or lib.mad_linear_fp8_needs_pack(x.data_ptr(), code, rows, k, n):
+        pq, ps = _fp8_empty(rows, k, fmt, xq.device)
+        _fp8_call("mad_linear_fp8_save", y, x.data_ptr(), code, _FP8_TYPES[fmt][1], q.data_ptr(), scale.data_ptr(), _ptr(bias),
+                  _ptr(residual), y.data_ptr(), pq.data_ptr(), ps.data_ptr(), rows, k, n)
+        x = Fp8Tensor(pq, ps, x.shape, x.dtype)
+    else:
+        _fp8_call("mad_linear_fp8", y, x.data_ptr(), code, None, q.data_ptr(), scale.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(),
+                  code, rows, k, n)
     if end is not None:
         end.record()
-    return y
+    return y, x
 
 
 def linear_fp8(x: Union[Tensor, Fp8Tensor], w: Fp8Weight, bias: Optional[Tensor] = None, residual: Optional[Tensor] = None,
@@ -982,17 +986,13 @@ def linear_fp8(x: Union[Tensor, Fp8Tensor], w: Fp8Weight, bias: Optional[Tensor]
         rows, c = _fp8_rows(x.shape, "linear_fp8")
     if c != K:
         raise ValueError(f"linear_fp8: x has {c} columns, the weight {K}")
-    shape, dtype = (*x.shape[:-1], N), x.dtype
+    shape = (*x.shape[:-1], N)
     if residual is not None and residual.shape != shape:
         raise ValueError(f"linear_fp8: residual has shape {tuple(residual.shape)}, y {shape}")
-    if not isinstance(x, Fp8Tensor) and (save or rows > FP8_FUSED_ROWS):
-        x = pack_fp8(x)
-    y = _linear_fp8(x, rows, K, dtype, w.q, w.scale, N, bias, residual, "linear_fp8")
+    y, x = _linear_fp8(x, rows, K, "e4m3", save, w.q, w.scale, N, bias, residual, "linear_fp8")
     if len(shape) != 2:
         y = y.view(shape)
-    if not save:
-        return y
-    return y, x
+    return (y, x) if save else y
 
 
 def linear_fp8_backward(dy: Tensor, x: Fp8Tensor, w: Optional[Fp8Weight] = None, need_dx: bool = True, grad_fmt: str = "e4m3",
@@ -1021,8 +1021,8 @@ def linear_fp8_backward(dy: Tensor, x: Fp8Tensor, w: Optional[Fp8Weight] = None,
         if w is None or tuple(w.shape) != (N, K):
             raise ValueError(f"linear_fp8_backward: dx needs the packed weight ({N}, {K})")
         _fp8_weight_check(w.qt, w.scale_t, K, N, "linear_fp8_backward")
-        g = pack_fp8(dy, grad_fmt)
-        dx = _linear_fp8(g, rows, N, dy.dtype, w.qt, w.scale_t, K, None, None, "linear_fp8_backward").view(x.shape)
+        dx, _ = _linear_fp8(dy, rows, N, grad_fmt, False, w.qt, w.scale_t, K, None, None, "linear_fp8_backward")
+        dx = dx.view(x.shape)
     if dw is None:
         dw = torch.empty((N, K), dtype=torch.float32, device=dy.device)
     if dbias is None and need_dbias:

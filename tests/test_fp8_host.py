@@ -163,6 +163,28 @@ def test_c_linear_refusals():
     assert call(rows=0) == 0
 
 
+def test_c_linear_save_refusals():
+    lib, L = _lib()
+
+    def call(x=P, dt=L.MAD_BF16, fmt=L.MAD_E4M3, w=P, ws=P, y=P, q=P, s=P, rows=1 << 20, K=32, N=8):
+        return lib.mad_linear_fp8_save(x, dt, fmt, w, ws, None, None, y, q, s, rows, K, N, None)
+    _refused(call(dt=5), "dtype")
+    _refused(call(fmt=L.MAD_BF16), "8-bit type")
+    _refused(call(rows=-1), "bad shape")
+    _refused(call(N=0), "bad shape")
+    _refused(call(K=0), "bad shape")
+    _refused(call(w=None), "null")
+    _refused(call(q=None), "null")
+    _refused(call(q=ODD), "aligned")
+    _refused(call(w=ODD), "aligned")
+    _refused(call(rows=4, q=None), "null")
+    assert call(rows=0) == 0
+    assert lib.mad_linear_fp8_needs_pack(P, L.MAD_BF16, 8, 4096, 4096) == 0
+    assert lib.mad_linear_fp8_needs_pack(P, L.MAD_BF16, 4096, 4096, 4096) == 1
+    assert lib.mad_linear_fp8_needs_pack(P, L.MAD_BF16, 1 << 20, 256, 256) == 0
+    assert lib.mad_linear_fp8_needs_pack(P, L.MAD_F32, 1 << 20, 256, 256) == 1
+
+
 def test_c_wgrad_refusals():
     lib, L = _lib()
 

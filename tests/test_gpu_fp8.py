@@ -277,6 +277,39 @@ def test_linear_over_many_tiles(dev, rows, k, n, dt):
     assert torch.equal(buf[:rows], got) and bool((buf[rows:] == 7.0).all())
 
 
+# bf16 inputs long enough for the form that rounds them on the way in, of one to four blocks, whole and partial, and around its limits
+ROWS_FORM = [(33000, 64, 200), (32768, 128, 128), (32769, 136, 513), (40001, 256, 768), (33333, 384, 66), (65600, 392, 384), (33000, 512, 2048),
+             (33000, 512, 2056), (33000, 520, 64), (33000, 60, 64)]
+
+
+@pytest.mark.parametrize("rows,k,n", ROWS_FORM)
+def test_one_launch_is_packing_and_product(dev, rows, k, n):
+    """The rounded x, if wanted, and y are those of the two calls, bit for bit; rows that are not finite included."""
+    from mad_amd import _lib, ops
+    g = torch.Generator(device=dev).manual_seed(rows + k + n)
+    rand = lambda *s: torch.randn(s, generator=g, device=dev)
+    x = (rand(rows, k) * torch.exp(2 * rand(rows, 1))).to(torch.bfloat16)
+    x[1, 3], x[5] = float("nan"), 0.0
+    x[rows - 1, k // 2], x[7] = float("inf"), float("-inf")
+    x[9] *= 2.0 ** -120
+    pw = ops.pack_weight_fp8(rand(n, k) / math.sqrt(k))
+    bias, res = rand(n), rand(rows, n).to(torch.bfloat16)
+    x8 = ops.pack_fp8(x)
+    for b, r in ((None, None), (bias, res)):
+        want = ops.linear_fp8(x8, pw, bias=b, residual=r)
+        y = ops.linear_fp8(x, pw, bias=b, residual=r)
+        ys, kept = ops.linear_fp8(x, pw, bias=b, residual=r, save=True)
+        assert _same(y, want) and _same(ys, want)
+        assert _same(kept.q.float(), x8.q.float()) and torch.equal(kept.scale, x8.scale)
+        assert not bool(_bytes(kept.q)[:, k:].any())
+    buf = torch.full((rows + 2, n), 7.0, dtype=torch.bfloat16, device=dev)
+    q, s = torch.full((rows + 2, x8.q.shape[1]), 0x11, dtype=torch.uint8, device=dev), torch.full((rows + 2, x8.scale.shape[1]), 0x11, dtype=torch.uint8, device=dev)
+    ops.check(_lib.lib.mad_linear_fp8_save(x.data_ptr(), _lib.MAD_BF16, _lib.MAD_E4M3, pw.q.data_ptr(), pw.scale.data_ptr(), bias.data_ptr(),
+                                           res.data_ptr(), buf.data_ptr(), q.data_ptr(), s.data_ptr(), rows, k, n,
+                                           torch.cuda.current_stream().cuda_stream), "mad_linear_fp8_save")
+    assert _same(buf[:rows], want) and bool((buf[rows:] == 7.0).all()) and bool((q[rows:] == 0x11).all()) and bool((s[rows:] == 0x11).all())
+
+
 @pytest.mark.parametrize("rows", [3, 300])
 def test_rows_do_not_touch_each_other(dev, rows):
     """NaN and infinities in one row reach that row of y alone, and zero rows give the bias."""
