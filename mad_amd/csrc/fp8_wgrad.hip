@@ -12,6 +12,7 @@
 // db is the gradient of an input column of ones: one more product per fragment of dy.  A workgroup makes it for every
 // ktiles-th step only (kt = step mod ktiles), so that no tile of dw has more work than another; the parts are joined.
 #include "fp8.h"
+#include <math.h>
 
 namespace mad {
 
@@ -158,7 +159,7 @@ __global__ __launch_bounds__(256) void wgrad_fp8_kernel(F8WgradArgs a) {
 // what lies there, which only reaches results that are not stored; rows past the share are zeros (reads outside their buffer).
 template <int BN, int BK> struct F8Wg {
     static constexpr int ROWS = 64, DY = ROWS * BN * 2, STAGE = DY + ROWS * BK * 2;
-    static constexpr int RAW = ROWS * BK, SCALES = 2 * ROWS * 4;          // x as it comes; scales of two steps, a dword per row
+    static constexpr int RAW = ROWS * BK, SCALES = 2 * ROWS * 8;          // x as it comes; scales of two steps, two dwords per row
     static constexpr int LDS = 2 * STAGE + RAW + SCALES;
 };
 
@@ -173,7 +174,8 @@ __global__ __launch_bounds__(64 * WN * WK) void wgrad_fp8_tile_kernel(F8WgradArg
     constexpr int FB = FN / WK;                                           // column sums: the waves of a row share its fragments
     constexpr int DPW = BN / 8 / NW;                                      // dy copies per wave and step (4 rows x 128 columns each)
     constexpr int XPT = 64 * BK / 16 / (64 * NW);                         // 16-byte pieces of x per thread and step
-    static_assert(BK <= 512 && NW % 2 == 0 && (64 * NW / (BK / 16)) % 8 == 0 && BN % 128 == 0 && BK % 128 == 0 && BN % (8 * NW) == 0 && XPT * 16 * NW == BK && FN % WK == 0, "tile");
+    static_assert(BK <= 512 && (BK <= 256 || BK == 384) && NW % 2 == 0 && BN % 128 == 0 && BK % 128 == 0 && BN % (8 * NW) == 0 &&
+                  XPT * 16 * NW == BK && FN % WK == 0, "tile");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wn = wave / WK, wk = wave % WK;
@@ -201,13 +203,15 @@ __global__ __launch_bounds__(64 * WN * WK) void wgrad_fp8_tile_kernel(F8WgradArg
         doff[j] = (unsigned)((4 * (c & 15) + lr) * a.N * 2 + (n0 + (c >> 4) * 128) * 2 + (((lane & 15) ^ swizzle(4 * wave + lr)) << 4));   // NW is even
     }
     unsigned xoff[XPT];
-    int xdst[XPT], sbyte[XPT];
+    int xdst[XPT], sbyte[XPT], odd = 0;
 #pragma unroll
     for (int u = 0; u < XPT; ++u) {
         const int i = u * 64 * NW + tid, row = i / (BK / 16), piece = i % (BK / 16), half = piece >> 3;
         xoff[u] = (unsigned)(row * xp + k0 + 16 * piece);
-        const int block = k0 / F8_BLOCK + half;
-        sbyte[u] = row * 4 + (block & 3);
+        // the row's dword of scales that holds the block: the first of the tile's, or the one behind it
+        const int block = (k0 / F8_BLOCK & 3) + half;
+        sbyte[u] = (block >> 2) * L::ROWS * 4 + row * 4 + (block & 3);
+        odd |= (row & 1) << u;
         // odd rows write their second piece first: the pieces of a write then cover all banks
         xdst[u] = L::DY + (half * L::ROWS + row) * 256 + (((2 * (piece & 7) + (row & 1)) ^ swizzle(row)) << 4);
     }
@@ -224,11 +228,14 @@ __global__ __launch_bounds__(64 * WN * WK) void wgrad_fp8_tile_kernel(F8WgradArg
         for (int j = 0; j < DPW; ++j) buf_lds16(db, doff[j], 0, lds0 + buf * L::STAGE + (j * NW + wave) * 1024);
     };
     constexpr int RAW = 2 * L::STAGE, SCALES = RAW + L::RAW;
-    // scales of step s: the dword of each row that holds the tile's blocks (k0 is a multiple of BK, so they are in one)
+    // scales of step s: the dword of each row that holds the tile's first block and, where the tile may reach past it, the next
     auto fetch_scales = [&](int s) {
         const long m = m_begin + (long)s * L::ROWS;
         const u32x4 sb = f8_buffer(a.xs + (size_t)m * sp, (unsigned)(step_rows(s) * sp));
-        if (wave == NW - 1) buf_lds4(sb, (unsigned)(lane * sp + (k0 / F8_BLOCK & ~3)), 0, lds0 + SCALES + (s & 1) * 256);
+        const int first = k0 / F8_BLOCK & ~3;
+        const unsigned dst = lds0 + SCALES + (s & 1) * L::ROWS * 8;
+        if (wave == NW - 1) buf_lds4(sb, (unsigned)(lane * sp + first), 0, dst);
+        if (BK > 256 && wave == NW - 2) buf_lds4(sb, first + 4 < sp ? (unsigned)(lane * sp + first + 4) : F8_OUTSIDE, 0, dst + L::ROWS * 4);
     };
     auto fetch_x = [&](int s) {                                           // x of step s into this lane's slots
         const long m = m_begin + (long)s * L::ROWS;
@@ -239,13 +246,13 @@ __global__ __launch_bounds__(64 * WN * WK) void wgrad_fp8_tile_kernel(F8WgradArg
         }
     };
     auto widen = [&](int s, int buf) {                                    // the fetched x of step s into the stage
-        const bool odd = tid / (BK / 16) & 1;                            // of the row: 64 NW / (BK / 16) rows apart is even
         unsigned char* d = smem + buf * L::STAGE;
 #pragma unroll
         for (int u = 0; u < XPT; ++u) {
             const uint4 v = *reinterpret_cast<const uint4*>(smem + RAW + (u * 64 * NW + tid) * 16);
-            const float sc = f8_scale(smem[SCALES + (s & 1) * 256 + sbyte[u]]);
-            const unsigned a0 = odd ? v.z : v.x, a1 = odd ? v.w : v.y, b0 = odd ? v.x : v.z, b1 = odd ? v.y : v.w;
+            const float sc = f8_scale(smem[SCALES + (s & 1) * L::ROWS * 8 + sbyte[u]]);
+            const bool o = odd >> u & 1;
+            const unsigned a0 = o ? v.z : v.x, a1 = o ? v.w : v.y, b0 = o ? v.x : v.z, b1 = o ? v.y : v.w;
             *reinterpret_cast<bf16x8*>(d + xdst[u]) = f8_bf16x8<FMT>(a0, a1, sc);
             *reinterpret_cast<bf16x8*>(d + (xdst[u] ^ 16)) = f8_bf16x8<FMT>(b0, b1, sc);
         }
@@ -374,22 +381,36 @@ __global__ __launch_bounds__(256) void wgrad_fp8_join_kernel(F8JoinArgs a) {
     }
 }
 
-// How a gradient is cut: the form, its tiles and the shares of the rows.
-struct F8WgradPlan { int tile, ntiles, ktiles, splits; long per; };
+// How a gradient is cut: the form, its tiles and the shares of the rows.  A step of 64 rows takes a workgroup about 1.5 us with tiles of
+// 128 x 128 (two workgroups to a unit), 1.9 with 128 x 384 and 1.85 with 256 x 256; a share more shortens the rows of each and
+// adds a partial sum to write and join.  The shares that balance the two, or fill the units once, and of the tiles the ones
+// that come out shortest (us, 128 x 128 / 128 x 384 / 256 x 256: 65536 x 384 -> 1152 99 / 86 / 105, 16384 x 768 -> 2304
+// 91 / 77 / 77, 8192 x 4096 -> 4096 319 / 388 / 234, 32768 x 256 -> 768 33 / 38 / 40).
+struct F8WgradPlan { int bn, bk, ntiles, ktiles, splits; long per; double us; };
 
 static F8WgradPlan wgrad_plan(long rows, int N, int K, bool tiled) {
-    F8WgradPlan p;
-    auto tiles = [&](int t) { return (long)((N + t - 1) / t) * ((K + t - 1) / t); };
-    const int cus = f8_cus();
-    p.tile = tiled && tiles(256) >= cus ? 256 : 128;
-    p.ntiles = (N + p.tile - 1) / p.tile; p.ktiles = (K + p.tile - 1) / p.tile;
-    // two workgroups of the small tile fit a unit at a time: no more shares than fill them once
-    long s = p.tile == 256 ? 1 : 2 * cus / tiles(p.tile);
-    const long most = (rows + 63) / 64;
-    if (s > most) s = most;
-    p.splits = (int)(s < 1 ? 1 : s);
-    p.per = ((rows + p.splits - 1) / p.splits + 63) / 64 * 64;
-    return p;
+    const long cus = f8_cus();
+    auto plan = [&](int bn, int bk, int resident, double step_us) {
+        F8WgradPlan p;
+        p.bn = bn; p.bk = bk;
+        p.ntiles = (N + bn - 1) / bn; p.ktiles = (K + bk - 1) / bk;
+        const long tiles = (long)p.ntiles * p.ktiles, steps = (rows + 63) / 64;
+        const double share_us = (double)N * K * 2.0e-6;                     // 8 bytes an element at 4 TB/s: written, then joined
+        long s = (long)sqrt((double)steps * step_us / share_us + 1.0);
+        const long most = resident * cus / tiles;
+        if (s > most) s = most;
+        if (s > steps) s = steps;
+        p.splits = (int)(s < 1 ? 1 : s);
+        p.per = ((rows + p.splits - 1) / p.splits + 63) / 64 * 64;
+        const double rounds = (double)((tiles * p.splits + resident * cus - 1) / (resident * cus));
+        p.us = rounds * (double)(p.per / 64) * step_us + (p.splits > 1 ? 3.0 + p.splits * share_us : 0.0);
+        return p;
+    };
+    F8WgradPlan best = plan(128, 128, 2, 1.5);
+    if (!tiled) return best;
+    for (const F8WgradPlan& p : {plan(128, 384, 1, 1.9), plan(256, 256, 1, 1.85)})
+        if (p.us < best.us) best = p;
+    return best;
 }
 
 }  // namespace mad
@@ -417,13 +438,13 @@ extern "C" size_t mad_linear_fp8_wgrad_workspace(long rows, int N, int K) {
     return a > b ? a : b;                       // whichever form the operands' alignment allows
 }
 
-template <int FMT, int T, int WN, int WK> static int launch_wgrad_tile(const F8WgradArgs& a, unsigned wgs, hipStream_t s) {
-    constexpr int lds = F8Wg<T, T>::LDS;
+template <int FMT, int BN, int BK, int WN, int WK> static int launch_wgrad_tile(const F8WgradArgs& a, unsigned wgs, hipStream_t s) {
+    constexpr int lds = F8Wg<BN, BK>::LDS;
     static int lds_dev = -1;
-    auto kernel = &wgrad_fp8_tile_kernel<FMT, T, T, WN, WK>;
+    auto kernel = &wgrad_fp8_tile_kernel<FMT, BN, BK, WN, WK>;
     MAD_REQUIRE(raise_lds_limit(reinterpret_cast<const void*>(kernel), lds, &lds_dev),
                 "mad_linear_fp8_wgrad: cannot raise the dynamic LDS limit to %d", lds);
-    hipLaunchKernelGGL((wgrad_fp8_tile_kernel<FMT, T, T, WN, WK>), dim3(wgs), dim3(64 * WN * WK), lds, s, a);
+    hipLaunchKernelGGL((wgrad_fp8_tile_kernel<FMT, BN, BK, WN, WK>), dim3(wgs), dim3(64 * WN * WK), lds, s, a);
     return check_launch("mad_linear_fp8_wgrad");
 }
 
@@ -455,10 +476,13 @@ extern "C" int mad_linear_fp8_wgrad(const void* dy, int dtype, const void* x, in
     a.acc_w = accumulate; a.acc_b = !join_b && bias_accumulate;
     hipStream_t s = (hipStream_t)stream;
     int rc;
-    if (tiled && p.tile == 256)
-        rc = x_type == MAD_E4M3 ? launch_wgrad_tile<F8_E4M3, 256, 2, 4>(a, (unsigned)wgs, s) : launch_wgrad_tile<F8_E5M2, 256, 2, 4>(a, (unsigned)wgs, s);
-    else if (tiled)
-        rc = x_type == MAD_E4M3 ? launch_wgrad_tile<F8_E4M3, 128, 2, 2>(a, (unsigned)wgs, s) : launch_wgrad_tile<F8_E5M2, 128, 2, 2>(a, (unsigned)wgs, s);
+#define TILE(BN, BK, WN, WK)                                                                                             \
+    (x_type == MAD_E4M3 ? launch_wgrad_tile<F8_E4M3, BN, BK, WN, WK>(a, (unsigned)wgs, s)                                \
+                        : launch_wgrad_tile<F8_E5M2, BN, BK, WN, WK>(a, (unsigned)wgs, s))
+    if (tiled && p.bn == 256) rc = TILE(256, 256, 2, 4);
+    else if (tiled && p.bk == 384) rc = TILE(128, 384, 2, 4);
+    else if (tiled) rc = TILE(128, 128, 2, 2);
+#undef TILE
     else {
 #define LAUNCH(T, F) hipLaunchKernelGGL((wgrad_fp8_kernel<T, F>), dim3((unsigned)wgs), dim3(256), 0, s, a)
         if (dtype == MAD_BF16) { if (x_type == MAD_E4M3) LAUNCH(bf16_t, F8_E4M3); else LAUNCH(bf16_t, F8_E5M2); }

@@ -142,6 +142,8 @@ def test_c_norm_refusals(name):
     _refused(call(p=1.0), "out of [0,1)")
     _refused(call(coef=None), "null")
     _refused(call(q=ODD), "aligned")
+    _refused(call(y=ODD), "aligned")
+    _refused(call(x=P + 2), "aligned")
     assert call(B=0) == 0 and call(HW=0) == 0
 
 

@@ -440,7 +440,8 @@ def test_linear_backward(dev, rows, k, n, fmt, dt):
 
 
 # rows, K, N: many shares of the rows, tiles of 128 and of 256, ragged in every direction, rows of dy that are no whole 16 bytes
-WGRAD_LARGE = [(66000, 272, 136), (333, 4000, 4104), (20001, 384, 1152), (5000, 16, 8), (3000, 1040, 131), (64, 4096, 4096), (129, 130, 264)]
+WGRAD_LARGE = [(66000, 272, 136), (333, 4000, 4104), (20001, 384, 1152), (5000, 16, 8), (3000, 1040, 131), (64, 4096, 4096), (129, 130, 264),
+               (30000, 768, 2304), (9000, 640, 520), (2000, 1152, 1536), (40000, 200, 1152)]
 
 
 @pytest.mark.parametrize("dt", DTYPES)
