@@ -7,7 +7,8 @@
 // step, so x is rounded once.  NaN stays NaN; an infinity becomes NaN in e4m3, which has none, and stays one in e5m2.
 // The scale is a power of two because the matrix instruction applies such scales itself (E8M0 operands of
 // v_mfma_scale_f32_16x16x128_f8f6f4, whose reduction length is exactly one block): no multiplication is left for the
-// vector unit, and bf16 holds every restored value exactly (4 significant bits at most).
+// vector unit, and bf16 holds every restored value exactly (4 significant bits at most; of blocks with scales under 2^-124, e5m2
+// 2^-117, the smallest elements are rounded to its smallest step, 2^-133).
 // Rows of bytes are padded with zeros to whole 16-byte pieces, rows of scales with 127 to whole groups of four.
 #pragma once
 #include "mma.h"
@@ -81,7 +82,7 @@ template <int FMT> __device__ __forceinline__ void f8_values4(unsigned q, float 
     f[0] = lo[0] * scale; f[1] = lo[1] * scale; f[2] = hi[0] * scale; f[3] = hi[1] * scale;
 }
 
-// eight bytes times a power of two as bf16: exact (4 significant bits)
+// eight bytes times a power of two as bf16: exact (4 significant bits) down to bf16's smallest step
 template <int FMT> __device__ __forceinline__ bf16x8 f8_bf16x8(unsigned lo, unsigned hi, float scale = 1.0f) {
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
     bf16x2 a, b, c, d;

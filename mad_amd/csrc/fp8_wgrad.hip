@@ -3,7 +3,7 @@
 //   dw[n][k] (+)= sum_m dy[m][n] * x[m][k]      db[n] (+)= sum_m dy[m][n]
 //
 // The scale of x changes along the reduction (one per row m), so the product cannot run on 8-bit operands; but bf16 holds
-// every restored value exactly, so x is widened on its way into LDS and the product runs on v_mfma_f32_16x16x32_bf16 without a
+// every restored value exactly (to 2^-133, its smallest step), so x is widened on its way into LDS and the product runs on v_mfma_f32_16x16x32_bf16 without a
 // further rounding.  dy is bf16, or fp32 cut into three bf16 terms whose sum is dy to 24 bits (x is exact, so three
 // products give fp32 accuracy).  Both operands are stored with the reduction index slow and read with the transposing LDS
 // read (ds_read_b64_tr_b16: a row of 16 lanes fetches 4 rows m x 16 columns, lane i receives column i).

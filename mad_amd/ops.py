@@ -889,7 +889,7 @@ def unpack_fp8(p: Fp8Tensor) -> Tensor:
 def _coef_check(coef: Tensor, shape: Sequence[int], what: str) -> None:
     if len(shape) != 4:
         raise ValueError(f"{what}: needs an NHWC tensor, got shape {tuple(shape)}")
-    if coef.dtype != torch.float32 or tuple(coef.shape) != (shape[0], shape[3], 2):
+    if coef.dtype != torch.float32 or coef.shape != (shape[0], shape[3], 2):
         raise ValueError(f"{what}: coef must be fp32 ({shape[0]}, {shape[3]}, 2), got {coef.dtype} {tuple(coef.shape)}")
 
 

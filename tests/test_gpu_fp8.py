@@ -108,6 +108,8 @@ def test_pack_keeps_leading_axes_and_takes_no_rows(dev):
     p = ops.pack_fp8(x)
     flat = ops.pack_fp8(x.view(30, 40))
     assert torch.equal(_bytes(p.q), _bytes(flat.q)) and torch.equal(ops.unpack_fp8(p).view(30, 40), ops.unpack_fp8(flat))
+    y = ops.linear_fp8(x[0, 0, 0, :].contiguous(), ops.pack_weight_fp8(_rand((24, 40), 2).to(dev)))
+    assert tuple(y.shape) == (24,)
     one = ops.pack_fp8(x[0, 0, 0, :].contiguous())
     assert torch.equal(_bytes(one.q)[0, :40], _bytes(flat.q)[0, :40])
     e = ops.pack_fp8(torch.empty((0, 40), device=dev))
@@ -343,6 +345,41 @@ def test_scales_far_apart(dev):
             _close(y, xv @ wv.t(), xv.abs() @ wv.abs().t(), 512, dt, _eights(xv, wv))
 
 
+@pytest.mark.parametrize("rows", [2, 70, 5000, 33000])
+def test_weights_that_are_not_finite(dev, rows):
+    """A NaN or an infinity of the weight makes its column of y NaN and no other."""
+    from mad_amd import ops
+    k, n = 200, 300
+    g = torch.Generator(device=dev).manual_seed(4)
+    w = torch.randn((n, k), generator=g, device=dev)
+    x = torch.randn((rows, k), generator=g, device=dev).to(torch.bfloat16)
+    clean = ops.linear_fp8(x, ops.pack_weight_fp8(w))
+    w[7, 3], w[200, 199] = float("nan"), float("inf")
+    y = ops.linear_fp8(x, ops.pack_weight_fp8(w))
+    keep = [i for i in range(n) if i not in (7, 200)]
+    assert torch.equal(y[:, keep], clean[:, keep]) and bool(torch.isnan(y[:, [7, 200]]).all())
+
+
+def test_values_at_the_floor_of_the_exponents(dev):
+    """Activations whose scale is the smallest there is (their values are subnormal in bf16): products and gradients keep them."""
+    from mad_amd import ops
+    for dt in DTYPES:
+        x = (_rand((96, 256), 1) * 2.0 ** -124).to(dt)
+        x8 = ops.pack_fp8(x.to(dev))
+        assert bool((x8.scale[:, :2] == 1).all())
+        xv = R.pack_rows(x)[0]
+        assert _same(ops.unpack_fp8(x8).cpu(), xv.float().to(dt))
+        w = _rand((48, 256), 2) * 2.0 ** 60
+        wv = R.pack_weight(w)[0]
+        _close(ops.linear_fp8(x8, ops.pack_weight_fp8(w.to(dev))), xv @ wv.t(), xv.abs() @ wv.abs().t(), 256, dt, _eights(xv, wv))
+        dy = (_rand((96, 64), 3) * 2.0 ** 60).to(dt)
+        _, dw, _ = ops.linear_fp8_backward(dy.to(dev), x8, need_dx=False)
+        # the gradient takes x in bf16: 2^-126 times an 8-bit value may lie between two multiples of 2^-133, bf16's smallest step, and is
+        # then off by at most half of it, so dw by at most 2^-134 * sum |dy|, added to S as (sum |dy| * 2^-134) / (100 * 2^-23)
+        size = dy.double().abs().t() @ xv.abs() + dy.double().abs().sum(0)[:, None] * (2.0 ** -134 / (100 * 2.0 ** -23))
+        _close(dw, dy.double().t() @ xv, size, 96, torch.float32)
+
+
 def test_linear_of_unaligned_operands(dev):
     """A bias, a residual and an input that start at any element."""
     from mad_amd import ops
@@ -536,6 +573,24 @@ def test_chain_is_deterministic_and_independent_of_the_stream(dev):
         b = _chain(ops, *args)
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_two_streams_at_once(dev):
+    """Calls that overlap on two streams share nothing."""
+    from mad_amd import ops
+    args = [_chain_inputs(dev, s) for s in (1, 30)]
+    want = [_chain(ops, *a) for a in args]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(_chain(ops, *args[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(u, v) for u, v in zip(out, want[i]))
 
 
 def test_chain_in_a_graph(dev):
