@@ -3,9 +3,9 @@
 //   dw[n][k] (+)= sum_m dy[m][n] * x[m][k]      db[n] (+)= sum_m dy[m][n]
 //
 // The scale of x changes along the reduction (one per row m), so the product cannot run on 8-bit operands; but bf16 holds
-// every restored value exactly (to 2^-133, its smallest step), so x is widened on its way into LDS and the product runs on v_mfma_f32_16x16x32_bf16 without a
-// further rounding.  dy is bf16, or fp32 cut into three bf16 terms whose sum is dy to 24 bits (x is exact, so three
-// products give fp32 accuracy).  Both operands are stored with the reduction index slow and read with the transposing LDS
+// every restored value exactly (to 2^-133, its smallest step), so x is widened on its way into LDS and the product runs on
+// v_mfma_f32_16x16x32_bf16 without a further rounding.  dy is bf16, or fp32 cut into three bf16 terms whose sum is dy (x is
+// exact, so three products give fp32 accuracy).  Both operands are stored with the reduction index slow and read with the transposing LDS
 // read (ds_read_b64_tr_b16: a row of 16 lanes fetches 4 rows m x 16 columns, lane i receives column i).
 // Shares of the rows write partial sums that a second kernel adds in share order: the result does not depend on timing.
 //
@@ -32,101 +32,174 @@ __device__ __forceinline__ bf16x8 tr_pair(const unsigned char* lo, const unsigne
     return bf16x8{l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3]};
 }
 
-__device__ __forceinline__ uint4 pack8_bf16(const float* f) {
-    uint4 o;
-    unsigned* w = &o.x;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = (unsigned)f32_to_bf16(f[2 * i]) | ((unsigned)f32_to_bf16(f[2 * i + 1]) << 16);
-    return o;
-}
+// The 16-byte chunk c of row m lies at c ^ swizzle(m): the eight rows that two lane groups read at a time, 32 bytes each, are in
+// eight different parts of the 256 bytes that the banks span (with (m & 3) << 2 alone every read took twice as long).
+__device__ __forceinline__ int swizzle(int m) { return ((m & 3) << 2) | ((m >> 2 & 1) << 1); }
 
-// T: type of dy; FMT: 8-bit type of x.  A workgroup owns 128 (n) x 128 (k) of dw and a share of the rows; four waves 2 x 2
-// of 64 x 64.  LDS tiles [32 rows m][128 columns] bf16; the 16-byte chunk c of row m lies at c ^ ((m & 3) << 2), so the four
-// rows a transposing read touches are in different banks.
-template <typename T, int FMT>
-__global__ __launch_bounds__(256) void wgrad_fp8_kernel(F8WgradArgs a) {
-    constexpr int NP = sizeof(T) == 4 ? 3 : 1;               // bf16 terms of dy
-    constexpr int TILE = 32 * 256;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[(NP + 1) * TILE];
+// Eight elements of dy on their way to bf16.  fp32 is cut into three terms by truncation, 8 bits of the 24 each, so that every
+// difference is exact; of a value that is not finite the first term is all (truncated, a NaN keeps a set bit).
+template <typename T> struct DyPiece;
+template <> struct DyPiece<bf16_t> {
+    uint4 v;
+    __device__ __forceinline__ void clear() { v = uint4{0, 0, 0, 0}; }
+    __device__ __forceinline__ void load(const bf16_t* p) { Piece8<bf16_t> t; t.load(p); v = __builtin_bit_cast(uint4, t.v); }
+    __device__ __forceinline__ void load_some(const bf16_t* p, int n) {
+        unsigned w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            w[e] = (2 * e < n ? (unsigned)p[2 * e] : 0u) | (2 * e + 1 < n ? (unsigned)p[2 * e + 1] << 16 : 0u);
+        v = uint4{w[0], w[1], w[2], w[3]};
+    }
+    __device__ __forceinline__ void terms(uint4* o) const { o[0] = v; }
+};
+template <> struct DyPiece<float> {
+    float f[8];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = 0.0f;
+    }
+    __device__ __forceinline__ void load(const float* p) { load8<float>(p, f); }
+    __device__ __forceinline__ void load_some(const float* p, int n) { load8_tail<float>(p, 0, n, f); }
+    __device__ __forceinline__ void terms(uint4* o) const {
+        unsigned t[3][8], top = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { const unsigned u = __float_as_uint(f[e]) & 0x7fffffffu; top = u > top ? u : top; }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            t[0][e] = __float_as_uint(f[e]);
+            const float r = f[e] - __uint_as_float(t[0][e] & 0xffff0000u);
+            t[1][e] = __float_as_uint(r);
+            t[2][e] = __float_as_uint(r - __uint_as_float(t[1][e] & 0xffff0000u));
+        }
+        if (__any(top >= 0x7f800000u)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const unsigned u = t[0][e] & 0x7fffffffu;
+                if (u >= 0x7f800000u) { t[0][e] |= u > 0x7f800000u ? 0x400000u : 0u; t[1][e] = t[2][e] = 0; }
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            unsigned* w = &o[p].x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_perm(t[p][2 * e + 1], t[p][2 * e], 0x07060302u);
+        }
+    }
+};
+
+// General form: dy in fp32, or in bf16 with rows that start anywhere.  128 (n) x BK (k) of dw per workgroup, 32 rows m per step,
+// waves of 64 x 64; LDS [32 rows][128 columns] bf16 per term of dy and per 128 columns of x, two stages.  Both operands pass
+// through registers: loaded a step and a half ahead, cut or widened between the two halves of the products of the step before.
+// As in the tiled form below, columns past the end hold whatever follows in memory, rows past the share zeros.
+// 8192 x 4096 -> 4096: fp32 808 us (three products: 1020 TFLOP/s of the matrix units; with one stage, loads inside the step and
+// terms rounded to nearest 1677), bf16 into 4095 columns 438 (1394).
+template <typename T, int BK> struct F8WgGeneral {
+    static constexpr int NP = sizeof(T) == 4 ? 3 : 1, TILE = 32 * 256, STAGE = (NP + BK / 128) * TILE, LDS = 2 * STAGE;
+};
+
+template <typename T, int FMT, int BK>
+__global__ __launch_bounds__(2 * BK) void wgrad_fp8_kernel(F8WgradArgs a) {
+    using L = F8WgGeneral<T, BK>;
+    constexpr int NP = L::NP, TILE = L::TILE, WK = BK / 64, FB = 4 / WK, DP = 256 / BK;
+    static_assert(BK == 128 || BK == 256, "tile");
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wn = wave >> 1, wk = wave & 1;
+    const int wn = wave / WK, wk = wave % WK;
     const int tiles = a.ntiles * a.ktiles;
     const int split = blockIdx.x / tiles, t = blockIdx.x - split * tiles;
     const int nt = t / a.ktiles, kt = t - nt * a.ktiles;
-    const int n0 = nt * 128, k0 = kt * 128;
+    const int n0 = nt * 128, k0 = kt * BK;
     const long m_begin = (long)split * a.per, m_end = m_begin + a.per < a.M ? m_begin + a.per : a.M;
+    const int steps = (int)((m_end - m_begin + 31) / 32);
     const int xp = f8_pitch(a.K), sp = f8_scale_pitch(a.K);
-    const T* dy = (const T*)a.dy;
+    const size_t total = (size_t)a.M * a.N;
 
-    f32x4 acc[4][4], accb[4];                                 // [k fragment][n fragment]
+    // this thread's pieces of a step: DP times eight columns of dy, sixteen of x
+    const int dr = tid >> 4, dc = 8 * (tid & 15), xr = tid / (BK / 16), xc = 16 * (tid % (BK / 16));
+    DyPiece<T> dv[DP];
+    uint4 xv;
+    float sc;
+    auto fetch = [&](int s) {
+        const long m = m_begin + 32L * s;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        accb[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int h = 0; h < DP; ++h) {
+            const long mr = m + dr + 16 * h;
+            const size_t at = (size_t)mr * a.N + n0 + dc;
+            dv[h].clear();
+            if (mr < m_end && n0 + dc < a.N) {
+                if (at + 8 <= total) dv[h].load((const T*)a.dy + at);
+                else dv[h].load_some((const T*)a.dy + at, a.N - n0 - dc);
+            }
+        }
+        xv = uint4{0, 0, 0, 0};
+        sc = 1.0f;
+        if (m + xr < m_end && k0 + xc < xp) {
+            xv = *reinterpret_cast<const uint4*>(a.x + (size_t)(m + xr) * xp + k0 + xc);
+            sc = f8_scale(a.xs[(size_t)(m + xr) * sp + (k0 + xc) / F8_BLOCK]);
+        }
+    };
+    auto put = [&](int buf) {
+        unsigned char* st = smem + buf * L::STAGE;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    const bool with_bias = a.db && wk == 0;
-    int turn = 0;                                             // step mod ktiles
-    const __bf16 one = (__bf16)1.0f;
-    const bf16x8 ones = {one, one, one, one, one, one, one, one};
-
-    const int lr = tid >> 4, lc = tid & 15;                   // loader: row within 16, 8-column piece
-    const int g = lane >> 4, q = (lane >> 2) & 3, pp = lane & 3;
-    auto frag = [&](const unsigned char* tile, int col) {     // 16 columns from col, all 32 rows
-        const int chunk = (col >> 3) + (pp >> 1);
-        const int off = ((chunk ^ (q << 2)) << 4) + (pp & 1) * 8;
-        return tr_pair(tile + (4 * g + q) * 256 + off, tile + (16 + 4 * g + q) * 256 + off);
+        for (int h = 0; h < DP; ++h) {
+            const int row = dr + 16 * h;
+            unsigned char* d = st + row * 256 + (((dc >> 3) ^ swizzle(row)) << 4);
+            uint4 o[NP];
+            dv[h].terms(o);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) *reinterpret_cast<uint4*>(d + p * TILE) = o[p];
+        }
+        unsigned char* d = st + (NP + xc / 128) * TILE + xr * 256;
+        const int chunk = (xc % 128 >> 3) ^ swizzle(xr);
+        *reinterpret_cast<bf16x8*>(d + (chunk << 4)) = f8_bf16x8<FMT>(xv.x, xv.y, sc);
+        *reinterpret_cast<bf16x8*>(d + ((chunk ^ 1) << 4)) = f8_bf16x8<FMT>(xv.z, xv.w, sc);
     };
 
-    for (long m = m_begin; m < m_end; m += 32) {
-        __syncthreads();
+    f32x4 acc[4][4], accb[FB];                                // [k fragment][n fragment]
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int row = 16 * h + lr;
-            const long mr = m + row;
-            const bool live = mr < m_end;
-            unsigned char* dst = smem + row * 256 + ((lc ^ ((row & 3) << 2)) << 4);
-            float f[8];
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = 0.0f;
-            const int n = n0 + 8 * lc, c = k0 + 8 * lc;
-            if (live && n < a.N) load8_tail<T>(dy + (size_t)mr * a.N + n, n, a.N, f);
+        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int p = 0; p < NP; ++p) {
-                *reinterpret_cast<uint4*>(dst + p * TILE) = pack8_bf16(f);
-                if (p + 1 < NP) {
+    for (int j = 0; j < FB; ++j) accb[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const __bf16 one = (__bf16)1.0f;
+    const bf16x8 ones = {one, one, one, one, one, one, one, one};
+    int turn = a.db ? 0 : -1;                                 // step mod ktiles
+
+    const int g = lane >> 4, q = (lane >> 2) & 3, pp = lane & 3;
+    const int frow = (4 * g + q) * 256 + (pp & 1) * 8, fswz = swizzle(4 * g + q);
+    auto frag = [&](const unsigned char* tile, int col) {     // 16 columns from col, all 32 rows
+        const unsigned char* p = tile + frow + ((((col >> 3) + (pp >> 1)) ^ fswz) << 4);
+        return tr_pair(p, p + 16 * 256);
+    };
+
+    fetch(0);
+    put(0);
+    fetch(1);
+    for (int s = 0; s < steps; ++s) {
+        __syncthreads();                   // step s is visible; every wave is done with the stage refilled below
+        const unsigned char* st = smem + (s & 1) * L::STAGE;
+        if (turn == kt) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {              // what the terms so far leave (nothing of an infinity or NaN)
-                        const float hi = bf16_to_f32(f32_to_bf16(f[e]));
-                        f[e] = f8_mag(hi) || hi == 0.0f ? f[e] - hi : 0.0f;
-                    }
-                }
-            }
+            for (int p = 0; p < NP; ++p)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = 0.0f;
-            if (live && c < xp) {
-                const uint2 v = *reinterpret_cast<const uint2*>(a.x + (size_t)mr * xp + c);
-                const float s = f8_scale(a.xs[(size_t)mr * sp + kt]);
-                f8_values4<FMT>(v.x, s, f);
-                f8_values4<FMT>(v.y, s, f + 4);
-            }
-            *reinterpret_cast<uint4*>(dst + NP * TILE) = pack8_bf16(f);
+                for (int j = 0; j < FB; ++j)
+                    accb[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, frag(st + p * TILE, wn * 64 + 16 * (wk * FB + j)), accb[j], 0, 0, 0);
         }
-        __syncthreads();
-        const bool mine = with_bias && turn == kt;
-        turn = turn + 1 == a.ktiles ? 0 : turn + 1;
+        if (a.db) turn = turn + 1 == a.ktiles ? 0 : turn + 1;
         bf16x8 xf[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) xf[i] = frag(smem + NP * TILE, wk * 64 + 16 * i);
+        for (int i = 0; i < 4; ++i) xf[i] = frag(st + (NP + wk / 2) * TILE, wk % 2 * 64 + 16 * i);
 #pragma unroll
-        for (int p = 0; p < NP; ++p)
+        for (int j = 0; j < 4; ++j) {
+            if (j == 2) { put((s + 1) & 1); fetch(s + 2); }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bf16x8 d = frag(smem + p * TILE, wn * 64 + 16 * j);
-                if (mine) accb[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, d, accb[j], 0, 0, 0);
+            for (int p = 0; p < NP; ++p) {
+                const bf16x8 d = frag(st + p * TILE, wn * 64 + 16 * j);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[i], d, acc[i][j], 0, 0, 0);
             }
+        }
     }
 
     // a lane holds four consecutive k of one n
@@ -140,12 +213,18 @@ __global__ __launch_bounds__(256) void wgrad_fp8_kernel(F8WgradArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int k = k0 + wk * 64 + 16 * i + 4 * g;
+            if (k >= a.K) continue;
             float* p = dw + (size_t)n * a.K + k;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (k + e < a.K) p[e] = (direct && a.acc_w ? p[e] : 0.0f) + acc[i][j][e];
+            f32x4 v = acc[i][j];
+            if (direct && a.acc_w) v += load4_tail<float>(p, k, a.K);
+            store4_tail<float>(p, k, a.K, v);
         }
-        if (with_bias && g == 0) {
+    }
+    if (a.db && g == 0) {
+#pragma unroll
+        for (int j = 0; j < FB; ++j) {
+            const int n = n0 + wn * 64 + 16 * (wk * FB + j) + r;
+            if (n >= a.N) continue;
             float* p = a.db + ((size_t)split * a.ktiles + kt) * a.N + n;
             *p = (a.acc_b ? *p : 0.0f) + accb[j][0];
         }
@@ -162,10 +241,6 @@ template <int BN, int BK> struct F8Wg {
     static constexpr int RAW = ROWS * BK, SCALES = 2 * ROWS * 8;          // x as it comes; scales of two steps, two dwords per row
     static constexpr int LDS = 2 * STAGE + RAW + SCALES;
 };
-
-// The 16-byte chunk c of row m lies at c ^ swizzle(m): the eight rows that two lane groups read at a time, 32 bytes each, are in
-// eight different parts of the 256 bytes that the banks span (with (m & 3) << 2 alone every read took twice as long).
-__device__ __forceinline__ int swizzle(int m) { return ((m & 3) << 2) | ((m >> 2 & 1) << 1); }
 
 template <int FMT, int BN, int BK, int WN, int WK>
 __global__ __launch_bounds__(64 * WN * WK) void wgrad_fp8_tile_kernel(F8WgradArgs a) {
@@ -383,12 +458,14 @@ __global__ __launch_bounds__(256) void wgrad_fp8_join_kernel(F8JoinArgs a) {
 
 // How a gradient is cut: the form, its tiles and the shares of the rows.  A step of 64 rows takes a workgroup about 1.5 us with tiles of
 // 128 x 128 (two workgroups to a unit), 1.9 with 128 x 384 and 1.85 with 256 x 256; a share more shortens the rows of each and
-// adds a partial sum to write and join.  The shares that balance the two, or fill the units once, and of the tiles the ones
-// that come out shortest (us, 128 x 128 / 128 x 384 / 256 x 256: 65536 x 384 -> 1152 99 / 86 / 105, 16384 x 768 -> 2304
+// adds a partial sum to write and join.  The general form takes 1.7 us (bf16; 128 x 256 is no faster there) and 3.5 (fp32; 3.15 with 128 x
+// 256, one workgroup: 16384 x 2048 -> 2048 483 / 428 us, 65536 x 128 -> 384 48 / 53).  The shares that balance the two, or fill the units
+// once, and of the tiles the ones that come out shortest (us, 128 x 128 / 128 x 384 / 256 x 256: 65536 x 384 -> 1152 99 / 86 / 105, 16384 x 768 -> 2304
 // 91 / 77 / 77, 8192 x 4096 -> 4096 319 / 388 / 234, 32768 x 256 -> 768 33 / 38 / 40).
+enum F8WgradForm { WG_TILED, WG_BF16, WG_F32 };
 struct F8WgradPlan { int bn, bk, ntiles, ktiles, splits; long per; double us; };
 
-static F8WgradPlan wgrad_plan(long rows, int N, int K, bool tiled) {
+static F8WgradPlan wgrad_plan(long rows, int N, int K, F8WgradForm form) {
     const long cus = f8_cus();
     auto plan = [&](int bn, int bk, int resident, double step_us) {
         F8WgradPlan p;
@@ -406,8 +483,12 @@ static F8WgradPlan wgrad_plan(long rows, int N, int K, bool tiled) {
         p.us = rounds * (double)(p.per / 64) * step_us + (p.splits > 1 ? 3.0 + p.splits * share_us : 0.0);
         return p;
     };
+    if (form == WG_BF16) return plan(128, 128, 2, 1.7);
+    if (form == WG_F32) {
+        const F8WgradPlan small = plan(128, 128, 2, 3.5), wide = plan(128, 256, 1, 3.15);
+        return wide.us < small.us ? wide : small;
+    }
     F8WgradPlan best = plan(128, 128, 2, 1.5);
-    if (!tiled) return best;
     for (const F8WgradPlan& p : {plan(128, 384, 1, 1.9), plan(256, 256, 1, 1.85)})
         if (p.us < best.us) best = p;
     return best;
@@ -427,25 +508,41 @@ static size_t wgrad_workspace(const F8WgradPlan& p, int N, int K) {
     return (w + b) * sizeof(float);
 }
 
-// the form with LDS-DMA of dy needs whole 16-byte pieces, and 64 rows within a buffer's 32-bit offsets
-static bool wgrad_tiled(const void* dy, int dtype, int N) {
-    return dtype == MAD_BF16 && N % 8 == 0 && !((uintptr_t)dy & 15);
+// LDS-DMA of dy needs rows of whole 16-byte pieces
+static F8WgradForm wgrad_form(const void* dy, int dtype, int N) {
+    return dtype == MAD_F32 ? WG_F32 : N % 8 == 0 && !((uintptr_t)dy & 15) ? WG_TILED : WG_BF16;
 }
 
 extern "C" size_t mad_linear_fp8_wgrad_workspace(long rows, int N, int K) {
     if (!wgrad_shape_ok(rows, N, K)) return 0;
-    const size_t a = wgrad_workspace(wgrad_plan(rows, N, K, true), N, K), b = wgrad_workspace(wgrad_plan(rows, N, K, false), N, K);
-    return a > b ? a : b;                       // whichever form the operands' alignment allows
+    size_t most = 0;                            // of the forms: which one runs depends on the operands' type and alignment
+    for (const F8WgradForm f : {WG_TILED, WG_BF16, WG_F32}) {
+        const size_t n = wgrad_workspace(wgrad_plan(rows, N, K, f), N, K);
+        if (n > most) most = n;
+    }
+    return most;
 }
 
-template <int FMT, int BN, int BK, int WN, int WK> static int launch_wgrad_tile(const F8WgradArgs& a, unsigned wgs, hipStream_t s) {
-    constexpr int lds = F8Wg<BN, BK>::LDS;
-    static int lds_dev = -1;
-    auto kernel = &wgrad_fp8_tile_kernel<FMT, BN, BK, WN, WK>;
-    MAD_REQUIRE(raise_lds_limit(reinterpret_cast<const void*>(kernel), lds, &lds_dev),
+static int launch_wgrad(void (*kernel)(F8WgradArgs), int lds, int* lds_dev, int threads, const F8WgradArgs& a, unsigned wgs, hipStream_t s) {
+    MAD_REQUIRE(raise_lds_limit(reinterpret_cast<const void*>(kernel), lds, lds_dev),
                 "mad_linear_fp8_wgrad: cannot raise the dynamic LDS limit to %d", lds);
-    hipLaunchKernelGGL((wgrad_fp8_tile_kernel<FMT, BN, BK, WN, WK>), dim3(wgs), dim3(64 * WN * WK), lds, s, a);
+    hipLaunchKernelGGL(kernel, dim3(wgs), dim3(threads), lds, s, a);
     return check_launch("mad_linear_fp8_wgrad");
+}
+
+template <int FMT> static int launch_wgrad(F8WgradForm form, const F8WgradPlan& p, const F8WgradArgs& a, hipStream_t s) {
+    const unsigned wgs = (unsigned)(p.ntiles * p.ktiles * p.splits);
+#define TILE(BN, BK, WN, WK)                                                                                               \
+    { static int dev = -1; return launch_wgrad(&wgrad_fp8_tile_kernel<FMT, BN, BK, WN, WK>, F8Wg<BN, BK>::LDS, &dev, 64 * WN * WK, a, wgs, s); }
+#define GENERAL(T, BK)                                                                                                     \
+    { static int dev = -1; return launch_wgrad(&wgrad_fp8_kernel<T, FMT, BK>, F8WgGeneral<T, BK>::LDS, &dev, 2 * BK, a, wgs, s); }
+    if (form == WG_F32) { if (p.bk == 256) GENERAL(float, 256) else GENERAL(float, 128) }
+    if (form == WG_BF16) GENERAL(bf16_t, 128)
+    if (p.bn == 256) TILE(256, 256, 2, 4)
+    if (p.bk == 384) TILE(128, 384, 2, 4)
+    TILE(128, 128, 2, 2)
+#undef TILE
+#undef GENERAL
 }
 
 extern "C" int mad_linear_fp8_wgrad(const void* dy, int dtype, const void* x, int x_type, const void* x_scale, float* dw, float* db,
@@ -459,8 +556,8 @@ extern "C" int mad_linear_fp8_wgrad(const void* dy, int dtype, const void* x, in
     const size_t need = mad_linear_fp8_wgrad_workspace(rows, N, K);
     MAD_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "mad_linear_fp8_wgrad: workspace of %zu bytes, %zu needed",
                 workspace_bytes, need);
-    const bool tiled = wgrad_tiled(dy, dtype, N);
-    const F8WgradPlan p = wgrad_plan(rows, N, K, tiled);
+    const F8WgradForm form = wgrad_form(dy, dtype, N);
+    const F8WgradPlan p = wgrad_plan(rows, N, K, form);
     const long wgs = (long)p.ntiles * p.ktiles * p.splits;
     MAD_REQUIRE(wgs <= 0x7fffffffL, "mad_linear_fp8_wgrad: N=%d K=%d need more workgroups than a launch holds", N, K);
     const size_t nk = (size_t)N * K;
@@ -475,21 +572,7 @@ extern "C" int mad_linear_fp8_wgrad(const void* dy, int dtype, const void* x, in
     a.ntiles = p.ntiles; a.ktiles = p.ktiles; a.splits = p.splits;
     a.acc_w = accumulate; a.acc_b = !join_b && bias_accumulate;
     hipStream_t s = (hipStream_t)stream;
-    int rc;
-#define TILE(BN, BK, WN, WK)                                                                                             \
-    (x_type == MAD_E4M3 ? launch_wgrad_tile<F8_E4M3, BN, BK, WN, WK>(a, (unsigned)wgs, s)                                \
-                        : launch_wgrad_tile<F8_E5M2, BN, BK, WN, WK>(a, (unsigned)wgs, s))
-    if (tiled && p.bn == 256) rc = TILE(256, 256, 2, 4);
-    else if (tiled && p.bk == 384) rc = TILE(128, 384, 2, 4);
-    else if (tiled) rc = TILE(128, 128, 2, 2);
-#undef TILE
-    else {
-#define LAUNCH(T, F) hipLaunchKernelGGL((wgrad_fp8_kernel<T, F>), dim3((unsigned)wgs), dim3(256), 0, s, a)
-        if (dtype == MAD_BF16) { if (x_type == MAD_E4M3) LAUNCH(bf16_t, F8_E4M3); else LAUNCH(bf16_t, F8_E5M2); }
-        else { if (x_type == MAD_E4M3) LAUNCH(float, F8_E4M3); else LAUNCH(float, F8_E5M2); }
-#undef LAUNCH
-        rc = check_launch("mad_linear_fp8_wgrad");
-    }
+    const int rc = x_type == MAD_E4M3 ? launch_wgrad<F8_E4M3>(form, p, a, s) : launch_wgrad<F8_E5M2>(form, p, a, s);
     if (rc) return rc;
     if (!join_w && !join_b) return 0;
     F8JoinArgs j;
