@@ -843,8 +843,8 @@ def _fp8_rows(shape: Sequence[int], what: str) -> Tuple[int, int]:
 def _fp8_empty(rows: int, c: int, fmt: str, device) -> Tuple[Tensor, Tensor]:
     if fmt not in _FP8_TYPES:
         raise ValueError(f"unknown 8-bit type {fmt!r}: 'e4m3' or 'e5m2'")
-    return (torch.empty((rows, _pitch(c)), dtype=_FP8_TYPES[fmt][0], device=device),
-            torch.empty((rows, _scale_pitch(c)), dtype=torch.uint8, device=device))
+    return (torch.empty(rows, _pitch(c), dtype=_FP8_TYPES[fmt][0], device=device),
+            torch.empty(rows, _scale_pitch(c), dtype=torch.uint8, device=device))
 
 
 def _fp8_check(p: Fp8Tensor, what: str) -> Tuple[int, int, int]:
@@ -934,8 +934,9 @@ def pack_weight_fp8(w: Tensor, transposed: bool = False) -> Fp8Weight:
     N, K = w.shape
     for n in (N, K):
         _fp8_rows((1, n), "pack_weight_fp8")
-    new = lambda r, c: torch.empty((r, c), dtype=torch.float8_e4m3fn, device=w.device)
-    scales = lambda r, c: torch.empty((-(-r // FP8_BLOCK), _scale_pitch(c)), dtype=torch.uint8, device=w.device)
+    device = w.device
+    new = lambda r, c: torch.empty(r, c, dtype=torch.float8_e4m3fn, device=device)
+    scales = lambda r, c: torch.empty(-(-r // FP8_BLOCK), _scale_pitch(c), dtype=torch.uint8, device=device)
     q, scale = new(N, _pitch(K)), scales(N, K)
     qt, scale_t = (new(K, _pitch(N)), scales(K, N)) if transposed else (None, None)
     _fp8_call("mad_pack_weight_fp8", w, _ptr(w), code, N, K, _ptr(q), _ptr(scale), _ptr(qt), _ptr(scale_t))
@@ -950,7 +951,7 @@ def _linear_fp8(x: Union[Tensor, Fp8Tensor], rows: int, k: int, fmt: str, keep: 
     _dev(xq, q, scale, bias, residual)
     if bias is not None and (bias.dtype != torch.float32 or bias.numel() != n):
         raise ValueError(f"{what}: bias must be fp32 with {n} elements")
-    y = torch.empty((rows, n), dtype=x.dtype, device=xq.device)
+    y = torch.empty(rows, n, dtype=x.dtype, device=xq.device)
     if residual is not None and (residual.dtype != x.dtype or residual.numel() != rows * n):
         raise ValueError(f"{what}: residual must be {x.dtype} with {rows * n} elements")
     code = _dtype_code(y)
@@ -1024,11 +1025,11 @@ def linear_fp8_backward(dy: Tensor, x: Fp8Tensor, w: Optional[Fp8Weight] = None,
         dx, _ = _linear_fp8(dy, rows, N, grad_fmt, False, w.qt, w.scale_t, K, None, None, "linear_fp8_backward")
         dx = dx.view(x.shape)
     if dw is None:
-        dw = torch.empty((N, K), dtype=torch.float32, device=dy.device)
+        dw = torch.empty(N, K, dtype=torch.float32, device=dy.device)
     if dbias is None and need_dbias:
-        dbias = torch.empty((N,), dtype=torch.float32, device=dy.device)
+        dbias = torch.empty(N, dtype=torch.float32, device=dy.device)
     nbytes = lib.mad_linear_fp8_wgrad_workspace(rows, N, K)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dy.device) if nbytes else None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device) if nbytes else None
     end = TIMER.bracket("linear_fp8_wgrad", 2.0 * rows * K * N)
     _fp8_call("mad_linear_fp8_wgrad", dy, _ptr(dy), code, _ptr(x.q), fmt, _ptr(x.scale), _ptr(dw), _ptr(dbias), _ptr(ws), nbytes,
               rows, N, K, int(accumulate), int(accumulate))
