@@ -476,8 +476,8 @@ int mad_pack_weight_fp8(const void* w, int dtype, int N, int K, void* q, void* s
 int mad_linear_fp8(const void* x, int x_type, const void* x_scale, const void* w, const void* w_scale,
                    const float* bias, const void* residual, void* y, int dtype, long rows, int K, int N, void* stream);
 
-/* mad_pack_fp8 of x in `fmt` and mad_linear_fp8 of the result in one call: y, and the packed x in q, scale.  Long inputs of
- * few columns (bf16, MAD_E4M3) are read once, by one launch.
+/* mad_pack_fp8 of x in `fmt` and mad_linear_fp8 of the result in one call: y, and the packed x in q, scale.  Small inputs, and
+ * long ones of few columns (bf16, MAD_E4M3), are packed inside the product's launch.
  * mad_linear_fp8_needs_pack: 1 where mad_linear_fp8 of an unpacked x would round it many times over and this call, with q and
  * scale as scratch, is the faster one; 0 where mad_linear_fp8 needs no packed x. */
 int mad_linear_fp8_needs_pack(const void* x, int dtype, long rows, int K, int N);

@@ -24,6 +24,7 @@ struct F8LinArgs {
     const void* x; const unsigned char* xs;        // x as bytes with scales, or as bf16 / fp32 (xs null)
     const unsigned char* w; const unsigned char* ws;
     const float* bias; const void* residual; void* y;
+    unsigned char* q; unsigned char* scale;        // direct form: where the rounded x is kept, or null
     long M;
     int K, N, mtiles, ntiles;
 };
@@ -62,9 +63,10 @@ __device__ __forceinline__ void block_product(f32x4& acc, const i32x8& w, const 
 }
 
 // Direct form: operands from global memory straight into registers, (16 MF) x (16 NF) outputs per workgroup, its NW
-// waves taking every NW-th block of the reduction.  Few rows are bound by the latency of reading the weights once, so the reduction is
-// spread over many waves; their sums are joined through LDS pairwise, wave w and w + NW/2 first: a fixed order.
-template <int XK, typename TO, int MF, int NF, int NW>
+// waves taking every NW-th block of the reduction.  Few rows are bound by the latency of reading the weights once, so the reduction
+// is spread over many waves; their sums are joined through LDS pairwise, wave w and w + NW/2 first: a fixed order.  x may come
+// unpacked: it is rounded to XF on its way in, by every workgroup that needs it, and kept in memory by the first of them if asked.
+template <int XK, int XF, typename TO, int MF, int NF, int NW>
 __global__ __launch_bounds__(64 * NW) void linear_fp8_direct_kernel(F8LinArgs a) {
     __shared__ __attribute__((aligned(16))) f32x4 red[NW / 2][MF * NF][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -139,10 +141,10 @@ __global__ __launch_bounds__(64 * NW) void linear_fp8_direct_kernel(F8LinArgs a)
                             u = hi < 0x7f80u && hi > u ? hi : u;
                         }
                     }
-                    xsc = (int)f8_scale_byte<F8_E4M3>(over_block(u) << 16);
+                    xsc = (int)f8_scale_byte<XF>(over_block(u) << 16);
                     const float scale = f8_scale((unsigned)xsc);
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) xf[q] = (int)f8_cvt4_bf16<F8_E4M3>(w[2 * q], w[2 * q + 1], scale);
+                    for (int q = 0; q < 8; ++q) xf[q] = (int)f8_cvt4_bf16<XF>(w[2 * q], w[2 * q + 1], scale);
                 } else {
                     float f[32];
                     if (whole) {
@@ -160,15 +162,25 @@ __global__ __launch_bounds__(64 * NW) void linear_fp8_direct_kernel(F8LinArgs a)
                     }
 #pragma unroll
                     for (int e = 0; e < 32; ++e) { const unsigned t = f8_mag(f[e]); u = t > u ? t : u; }
-                    xsc = (int)f8_scale_byte<F8_E4M3>(over_block(u));
+                    xsc = (int)f8_scale_byte<XF>(over_block(u));
                     const float inv = f8_inv_scale((unsigned)xsc);
 #pragma unroll
                     for (int q = 0; q < 8; ++q)
-                        xf[q] = (int)f8_cvt4<F8_E4M3>(f[4 * q] * inv, f[4 * q + 1] * inv, f[4 * q + 2] * inv, f[4 * q + 3] * inv);
+                        xf[q] = (int)f8_cvt4<XF>(f[4 * q] * inv, f[4 * q + 1] * inv, f[4 * q + 2] * inv, f[4 * q + 3] * inv);
+                }
+                if (a.q && n0 == 0 && 16 * i + r < mrem) {
+                    const size_t row = (size_t)m0 + 16 * i + r;
+                    uint4* to = reinterpret_cast<uint4*>(a.q + row * wp + c);
+                    if (c < wp) to[0] = uint4{(unsigned)xf[0], (unsigned)xf[1], (unsigned)xf[2], (unsigned)xf[3]};
+                    if (c + 16 < wp) to[1] = uint4{(unsigned)xf[4], (unsigned)xf[5], (unsigned)xf[6], (unsigned)xf[7]};
+                    if (g == 0) {
+                        a.scale[row * sp + kt] = (unsigned char)xsc;
+                        for (int k = kt + 1; kt == kb - 1 && k < sp; ++k) a.scale[row * sp + k] = 127;
+                    }
                 }
             }
 #pragma unroll
-            for (int j = 0; j < NF; ++j) block_product<XK == X_E5M2 ? F8_E5M2 : F8_E4M3, sizeof(TO) == 4>(acc[j][i], wf[j], xf, wsc[j], xsc);
+            for (int j = 0; j < NF; ++j) block_product<XF, sizeof(TO) == 4>(acc[j][i], wf[j], xf, wsc[j], xsc);
         }
     }
 #pragma unroll
@@ -605,12 +617,12 @@ __global__ __launch_bounds__(256, 2) void linear_fp8_rows_kernel(F8RowArgs a) {
     dma_wait_all();                                // the copies of the strip behind the last
 }
 
-template <int XK, typename TO, int MF, int NF, int NW> static int launch_direct(F8LinArgs a, hipStream_t s) {
+template <int XK, int XF, typename TO, int MF, int NF, int NW> static int launch_direct(F8LinArgs a, hipStream_t s) {
     const long mtiles = (a.M + 16 * MF - 1) / (16 * MF);
     a.ntiles = (a.N + 16 * NF - 1) / (16 * NF);
     MAD_REQUIRE(mtiles * a.ntiles <= 0x7fffffffL, "mad_linear_fp8: %ld rows x %d columns need more workgroups than a launch holds",
                 a.M, a.N);
-    hipLaunchKernelGGL((linear_fp8_direct_kernel<XK, TO, MF, NF, NW>), dim3((unsigned)(mtiles * a.ntiles)), dim3(64 * NW), 0, s, a);
+    hipLaunchKernelGGL((linear_fp8_direct_kernel<XK, XF, TO, MF, NF, NW>), dim3((unsigned)(mtiles * a.ntiles)), dim3(64 * NW), 0, s, a);
     return check_launch("mad_linear_fp8");
 }
 
@@ -635,7 +647,7 @@ template <int XF, typename TO, int BM, int BN, int WM, int WN> static int launch
 // large tiles, 274 with small; 4096 x 4096 -> 1024 52 / 26) and nothing extra below (65536 x 384 -> 1152 51 / 47,
 // 16384 x 256 -> 4096 37 / 37).  With fewer than one small tile for each unit the direct form is as fast or faster
 // (1024 x 4096 -> 1024 23 / 24, 64 x 256 -> 4096 3.5 / 5.7; fp32 777 x 1000 -> 328 7 / 15).
-template <int XK, typename TO> static int launch_linear(F8LinArgs a, hipStream_t s) {
+template <int XK, int XF, typename TO> static int launch_linear(F8LinArgs a, hipStream_t s) {
     if constexpr (XK < X_BF16) {
         const long cus = f8_cus(), small = ((a.M + 127) / 128) * ((a.N + 127) / 128), large = ((a.M + 255) / 256) * ((a.N + 255) / 256);
         if (small >= cus) {
@@ -645,15 +657,17 @@ template <int XK, typename TO> static int launch_linear(F8LinArgs a, hipStream_t
     }
     // Of the direct form, the smaller its workgroups the more of them share the latency, until re-reading costs more.  Sixteen by
     // sixteen results each up to two workgroups for each unit, then 32 x 32, then 64 x 64 (packed x, us: 64 x 1024 -> 1024 3.6 / 4.9
-    // / 7.5, 64 x 4096 -> 4096 20.9 / 12.6 / 25, 1024 x 4096 -> 1024 73 / 39 / 23).  Where x is rounded on its way in, every
-    // workgroup rounds it again, so they get wider in n first (16 x 4096 -> 8192 19.7 / 14.9 for 16 / 32 columns).
+    // / 7.5, 64 x 4096 -> 4096 20.9 / 12.4 / 25, 1024 x 4096 -> 1024 73 / 39 / 23).  Where x is rounded on its way in, every
+    // workgroup rounds it again, so they get wider in n first (16 x 4096 -> 8192 19.7 / 14.9 for 16 / 32 columns).  Eight waves in the first
+    // two: a result is the same sum whether x came packed or is kept packed on the way (four cost as much: 1024 x 384 -> 384
+    // 4.4 / 4.7, fp32 64 x 4096 -> 4096 13.8 / 12.5).
     const long f = ((a.M + 15) / 16) * ((a.N + 15) / 16), cus = f8_cus();
     if constexpr (XK < X_BF16) {
-        if (f <= 2 * cus) return launch_direct<XK, TO, 1, 1, 8>(a, s);
-        return f <= 8 * cus ? launch_direct<XK, TO, 2, 2, 4>(a, s) : launch_direct<XK, TO, 4, 4, 4>(a, s);
+        if (f <= 2 * cus) return launch_direct<XK, XF, TO, 1, 1, 8>(a, s);
+        return f <= 8 * cus ? launch_direct<XK, XF, TO, 2, 2, 8>(a, s) : launch_direct<XK, XF, TO, 4, 4, 4>(a, s);
     } else {
-        if (f <= cus) return launch_direct<XK, TO, 1, 1, 8>(a, s);
-        return a.M <= 16 ? launch_direct<XK, TO, 1, 2, 16>(a, s) : launch_direct<XK, TO, 2, 2, 8>(a, s);
+        if (f <= cus) return launch_direct<XK, XF, TO, 1, 1, 8>(a, s);
+        return a.M <= 16 && !a.q ? launch_direct<XK, XF, TO, 1, 2, 16>(a, s) : launch_direct<XK, XF, TO, 2, 2, 8>(a, s);
     }
 }
 
@@ -710,33 +724,53 @@ extern "C" int mad_linear_fp8(const void* x, int x_type, const void* x_scale, co
         return launch_rows(row_args(x, w, w_scale, bias, residual, y, nullptr, nullptr, rows, K, N), (hipStream_t)stream);
     F8LinArgs a;
     a.x = x; a.xs = (const unsigned char*)x_scale; a.w = (const unsigned char*)w; a.ws = (const unsigned char*)w_scale;
+    a.q = a.scale = nullptr;
     a.bias = bias; a.residual = residual; a.y = y; a.M = rows; a.K = K; a.N = N; a.mtiles = a.ntiles = 0;
     hipStream_t s = (hipStream_t)stream;
     if (dtype == MAD_BF16) {
-        if (x_type == MAD_E4M3) return launch_linear<X_E4M3, bf16_t>(a, s);
-        if (x_type == MAD_E5M2) return launch_linear<X_E5M2, bf16_t>(a, s);
-        return launch_linear<X_BF16, bf16_t>(a, s);
+        if (x_type == MAD_E4M3) return launch_linear<X_E4M3, F8_E4M3, bf16_t>(a, s);
+        if (x_type == MAD_E5M2) return launch_linear<X_E5M2, F8_E5M2, bf16_t>(a, s);
+        return launch_linear<X_BF16, F8_E4M3, bf16_t>(a, s);
     }
-    if (x_type == MAD_E4M3) return launch_linear<X_E4M3, float>(a, s);
-    if (x_type == MAD_E5M2) return launch_linear<X_E5M2, float>(a, s);
-    return launch_linear<X_F32, float>(a, s);
+    if (x_type == MAD_E4M3) return launch_linear<X_E4M3, F8_E4M3, float>(a, s);
+    if (x_type == MAD_E5M2) return launch_linear<X_E5M2, F8_E5M2, float>(a, s);
+    return launch_linear<X_F32, F8_E4M3, float>(a, s);
 }
 
-// up to this many rows the direct form rounds x on its way in for less than a launch costs
-static constexpr long F8_FUSED_ROWS = 32;
+// Whether the direct form rounds x on its way in for less than a launch of its own costs: a few rows, or few workgroups of 32 x 32 results
+// and blocks for each (us of the GPU, rounding inside / packing first: bf16 777 x 1000 -> 328 6.6 / 8.9, 777 x 1000 -> 1024 11.3 / 11.5,
+// 2048 x 1000 -> 1024 25 / 16, 256 x 4096 -> 1024 14.5 / 15.3, 256 x 4096 -> 4096 48 / 26; fp32, twice the work to round: 777 x 1000 ->
+// 328 10.3 / 9.6, 777 x 1000 -> 1024 17 / 13).  The host's time for the second launch and its buffers, 6 us, comes on top.
+// Where the packed x is kept, only sizes whose packed form adds in the same order: y is then the product of what is kept, bit for bit.
+static bool direct_rounds(int dtype, long rows, int K, int N, bool keep) {
+    const long cus = f8_cus(), wgs = ((rows + 31) / 32) * ((N + 31) / 32);
+    if (keep && (((rows + 15) / 16) * ((N + 15) / 16) > 8 * cus || ((rows + 127) / 128) * ((N + 127) / 128) >= cus)) return false;
+    return rows <= 32 || (wgs <= 4 * cus && wgs * f8_blocks(K) * (dtype == MAD_F32 ? 2 : 1) <= 32 * cus);
+}
 
 extern "C" int mad_linear_fp8_needs_pack(const void* x, int dtype, long rows, int K, int N) {
-    return rows > F8_FUSED_ROWS && !rows_form_ok(x, dtype, rows, K, N);
+    return !direct_rounds(dtype, rows, K, N, false) && !rows_form_ok(x, dtype, rows, K, N);
 }
 
 extern "C" int mad_linear_fp8_save(const void* x, int dtype, int fmt, const void* w, const void* w_scale, const float* bias,
                                    const void* residual, void* y, void* q, void* scale, long rows, int K, int N, void* stream) {
     MAD_REQUIRE(rows >= 0 && N > 0 && N <= MAD_FP8_MAX_WIDTH, "mad_linear_fp8_save: bad shape rows=%ld N=%d", rows, N);
-    if (fmt == MAD_E4M3 && K > 0 && rows_form_ok(x, dtype, rows, K, N)) {
+    const bool rows_form = fmt == MAD_E4M3 && K > 0 && rows_form_ok(x, dtype, rows, K, N);
+    const bool typed = (dtype == MAD_BF16 || dtype == MAD_F32) && (fmt == MAD_E4M3 || fmt == MAD_E5M2);
+    if (rows_form || (typed && rows > 0 && K > 0 && K <= MAD_FP8_MAX_WIDTH && direct_rounds(dtype, rows, K, N, true))) {
         MAD_REQUIRE(x && w && w_scale && y && q && scale, "mad_linear_fp8_save: null pointer");
         MAD_REQUIRE(f8_aligned(w, w_scale) && f8_aligned(q, scale),
                     "mad_linear_fp8_save: packed bytes must be 16-byte, scales 4-byte aligned");
-        return launch_rows(row_args(x, w, w_scale, bias, residual, y, q, scale, rows, K, N), (hipStream_t)stream);
+        if (rows_form)
+            return launch_rows(row_args(x, w, w_scale, bias, residual, y, q, scale, rows, K, N), (hipStream_t)stream);
+        F8LinArgs a;
+        a.x = x; a.xs = nullptr; a.w = (const unsigned char*)w; a.ws = (const unsigned char*)w_scale;
+        a.q = (unsigned char*)q; a.scale = (unsigned char*)scale;
+        a.bias = bias; a.residual = residual; a.y = y; a.M = rows; a.K = K; a.N = N; a.mtiles = a.ntiles = 0;
+        hipStream_t s = (hipStream_t)stream;
+        if (dtype == MAD_BF16)
+            return fmt == MAD_E4M3 ? launch_linear<X_BF16, F8_E4M3, bf16_t>(a, s) : launch_linear<X_BF16, F8_E5M2, bf16_t>(a, s);
+        return fmt == MAD_E4M3 ? launch_linear<X_F32, F8_E4M3, float>(a, s) : launch_linear<X_F32, F8_E5M2, float>(a, s);
     }
     if (int rc = mad_pack_fp8(x, dtype, fmt, rows, K, q, scale, stream)) return rc;
     return mad_linear_fp8(q, fmt, scale, w, w_scale, bias, residual, y, dtype, rows, K, N, stream);

@@ -10,7 +10,8 @@
 // Shares of the rows write partial sums that a second kernel adds in share order: the result does not depend on timing.
 //
 // db is the gradient of an input column of ones: one more product per fragment of dy.  A workgroup makes it for every
-// ktiles-th step only (kt = step mod ktiles), so that no tile of dw has more work than another; the parts are joined.
+// ktiles-th step only (kt = step mod turns, turns = ktiles), so that no tile of dw has more work than another; the parts are
+// joined.  Where that would be all there is to join, and the launch costs more than the sixteenth it saves, turns is 1.
 #include "fp8.h"
 #include <math.h>
 
@@ -20,7 +21,7 @@ struct F8WgradArgs {
     const void* dy; const unsigned char* x; const unsigned char* xs;
     float* dw; float* db;                      // destinations, or partial slabs when splits > 1
     long M, per;                               // rows, rows per share (a multiple of 32)
-    int N, K, ntiles, ktiles, splits, acc_w, acc_b;
+    int N, K, ntiles, ktiles, splits, turns, acc_w, acc_b;
 };
 
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -164,7 +165,7 @@ __global__ __launch_bounds__(2 * BK) void wgrad_fp8_kernel(F8WgradArgs a) {
     for (int j = 0; j < FB; ++j) accb[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const __bf16 one = (__bf16)1.0f;
     const bf16x8 ones = {one, one, one, one, one, one, one, one};
-    int turn = a.db ? 0 : -1;                                 // step mod ktiles
+    int turn = a.db ? 0 : -1;                                 // step mod turns
 
     const int g = lane >> 4, q = (lane >> 2) & 3, pp = lane & 3;
     const int frow = (4 * g + q) * 256 + (pp & 1) * 8, fswz = swizzle(4 * g + q);
@@ -186,7 +187,7 @@ __global__ __launch_bounds__(2 * BK) void wgrad_fp8_kernel(F8WgradArgs a) {
                 for (int j = 0; j < FB; ++j)
                     accb[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, frag(st + p * TILE, wn * 64 + 16 * (wk * FB + j)), accb[j], 0, 0, 0);
         }
-        if (a.db) turn = turn + 1 == a.ktiles ? 0 : turn + 1;
+        if (a.db) turn = turn + 1 == a.turns ? 0 : turn + 1;
         bf16x8 xf[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) xf[i] = frag(st + (NP + wk / 2) * TILE, wk % 2 * 64 + 16 * i);
@@ -220,12 +221,12 @@ __global__ __launch_bounds__(2 * BK) void wgrad_fp8_kernel(F8WgradArgs a) {
             store4_tail<float>(p, k, a.K, v);
         }
     }
-    if (a.db && g == 0) {
+    if (a.db && g == 0 && kt < a.turns) {
 #pragma unroll
         for (int j = 0; j < FB; ++j) {
             const int n = n0 + wn * 64 + 16 * (wk * FB + j) + r;
             if (n >= a.N) continue;
-            float* p = a.db + ((size_t)split * a.ktiles + kt) * a.N + n;
+            float* p = a.db + ((size_t)split * a.turns + kt) * a.N + n;
             *p = (a.acc_b ? *p : 0.0f) + accb[j][0];
         }
     }
@@ -343,7 +344,7 @@ __global__ __launch_bounds__(64 * WN * WK) void wgrad_fp8_tile_kernel(F8WgradArg
     }
     const __bf16 one = (__bf16)1.0f;
     const bf16x8 ones = {one, one, one, one, one, one, one, one};
-    int turn = a.db ? 0 : -1;                                 // step mod ktiles
+    int turn = a.db ? 0 : -1;                                 // step mod turns
 
     // fragment of 16 columns: rows 4g + q and 16 rows on, 8 bytes at columns 4 pp
     const int frow = (4 * g + q) * 256 + (pp & 1) * 8, fswz = swizzle(4 * g + q);
@@ -375,7 +376,7 @@ __global__ __launch_bounds__(64 * WN * WK) void wgrad_fp8_tile_kernel(F8WgradArg
                 for (int j = 0; j < FB; ++j)
                     accb[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, frag(st, wn * (BN / WN) + 16 * (wk * FB + j), h), accb[j], 0, 0, 0);
         }
-        if (a.db) turn = turn + 1 == a.ktiles ? 0 : turn + 1;
+        if (a.db) turn = turn + 1 == a.turns ? 0 : turn + 1;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             bf16x8 xf[FK], d[FN];
@@ -413,12 +414,12 @@ __global__ __launch_bounds__(64 * WN * WK) void wgrad_fp8_tile_kernel(F8WgradArg
             store4_tail<float>(p, k, a.K, v);
         }
     }
-    if (a.db && g == 0) {
+    if (a.db && g == 0 && kt < a.turns) {
 #pragma unroll
         for (int j = 0; j < FB; ++j) {
             const int n = n0 + wn * (BN / WN) + 16 * (wk * FB + j) + r;
             if (n >= a.N) continue;
-            float* p = a.db + ((size_t)split * a.ktiles + kt) * a.N + n;
+            float* p = a.db + ((size_t)split * a.turns + kt) * a.N + n;
             *p = (a.acc_b ? *p : 0.0f) + accb[j][0];
         }
     }
@@ -463,25 +464,34 @@ __global__ __launch_bounds__(256) void wgrad_fp8_join_kernel(F8JoinArgs a) {
 // once, and of the tiles the ones that come out shortest (us, 128 x 128 / 128 x 384 / 256 x 256: 65536 x 384 -> 1152 99 / 86 / 105, 16384 x 768 -> 2304
 // 91 / 77 / 77, 8192 x 4096 -> 4096 319 / 388 / 234, 32768 x 256 -> 768 33 / 38 / 40).
 enum F8WgradForm { WG_TILED, WG_BF16, WG_F32 };
-struct F8WgradPlan { int bn, bk, ntiles, ktiles, splits; long per; double us; };
+struct F8WgradPlan { int bn, bk, ntiles, ktiles, splits, turns; long per; double us; };
 
 static F8WgradPlan wgrad_plan(long rows, int N, int K, F8WgradForm form) {
     const long cus = f8_cus();
     auto plan = [&](int bn, int bk, int resident, double step_us) {
-        F8WgradPlan p;
-        p.bn = bn; p.bk = bk;
-        p.ntiles = (N + bn - 1) / bn; p.ktiles = (K + bk - 1) / bk;
-        const long tiles = (long)p.ntiles * p.ktiles, steps = (rows + 63) / 64;
         const double share_us = (double)N * K * 2.0e-6;                     // 8 bytes an element at 4 TB/s: written, then joined
+        const double join_us = 5.0;                                         // another launch, for GPU and host
+        const long steps = (rows + 63) / 64;
+        auto with = [&](long s) {
+            F8WgradPlan p;
+            p.bn = bn; p.bk = bk;
+            p.ntiles = (N + bn - 1) / bn; p.ktiles = (K + bk - 1) / bk;
+            p.splits = (int)s;
+            p.per = ((rows + s - 1) / s + 63) / 64 * 64;
+            const double rounds = (double)(((long)p.ntiles * p.ktiles * s + resident * cus - 1) / (resident * cus));
+            p.us = rounds * (double)(p.per / 64) * step_us;
+            p.turns = s == 1 && p.us < 16 * join_us ? 1 : p.ktiles;
+            if (s > 1) p.us += join_us + s * share_us;
+            return p;
+        };
+        const F8WgradPlan one = with(1);
         long s = (long)sqrt((double)steps * step_us / share_us + 1.0);
-        const long most = resident * cus / tiles;
+        const long most = resident * cus / ((long)one.ntiles * one.ktiles);
         if (s > most) s = most;
         if (s > steps) s = steps;
-        p.splits = (int)(s < 1 ? 1 : s);
-        p.per = ((rows + p.splits - 1) / p.splits + 63) / 64 * 64;
-        const double rounds = (double)((tiles * p.splits + resident * cus - 1) / (resident * cus));
-        p.us = rounds * (double)(p.per / 64) * step_us + (p.splits > 1 ? 3.0 + p.splits * share_us : 0.0);
-        return p;
+        if (s < 2) return one;
+        const F8WgradPlan many = with(s);
+        return many.us < one.us ? many : one;
     };
     if (form == WG_BF16) return plan(128, 128, 2, 1.7);
     if (form == WG_F32) {
@@ -504,7 +514,7 @@ static bool wgrad_shape_ok(long rows, int N, int K) {
 
 static size_t wgrad_workspace(const F8WgradPlan& p, int N, int K) {
     const size_t w = p.splits > 1 ? (size_t)p.splits * N * K : 0;
-    const size_t b = (size_t)p.splits * p.ktiles > 1 ? (size_t)p.splits * p.ktiles * N : 0;
+    const size_t b = (size_t)p.splits * p.turns > 1 ? (size_t)p.splits * p.turns * N : 0;
     return (w + b) * sizeof(float);
 }
 
@@ -561,7 +571,7 @@ extern "C" int mad_linear_fp8_wgrad(const void* dy, int dtype, const void* x, in
     const long wgs = (long)p.ntiles * p.ktiles * p.splits;
     MAD_REQUIRE(wgs <= 0x7fffffffL, "mad_linear_fp8_wgrad: N=%d K=%d need more workgroups than a launch holds", N, K);
     const size_t nk = (size_t)N * K;
-    const bool join_w = p.splits > 1, join_b = db && (size_t)p.splits * p.ktiles > 1;
+    const bool join_w = p.splits > 1, join_b = db && (size_t)p.splits * p.turns > 1;
     float* part_w = (float*)workspace;
     float* part_b = part_w + (join_w ? (size_t)p.splits * nk : 0);
     F8WgradArgs a;
@@ -569,7 +579,7 @@ extern "C" int mad_linear_fp8_wgrad(const void* dy, int dtype, const void* x, in
     a.dw = join_w ? part_w : dw;
     a.db = join_b ? part_b : db;
     a.M = rows; a.per = p.per; a.N = N; a.K = K;
-    a.ntiles = p.ntiles; a.ktiles = p.ktiles; a.splits = p.splits;
+    a.ntiles = p.ntiles; a.ktiles = p.ktiles; a.splits = p.splits; a.turns = p.turns;
     a.acc_w = accumulate; a.acc_b = !join_b && bias_accumulate;
     hipStream_t s = (hipStream_t)stream;
     const int rc = x_type == MAD_E4M3 ? launch_wgrad<F8_E4M3>(form, p, a, s) : launch_wgrad<F8_E5M2>(form, p, a, s);
@@ -577,7 +587,7 @@ extern "C" int mad_linear_fp8_wgrad(const void* dy, int dtype, const void* x, in
     if (!join_w && !join_b) return 0;
     F8JoinArgs j;
     j.part = part_w; j.dst = dw; j.part_b = part_b; j.dst_b = db;
-    j.n = join_w ? nk : 0; j.nb = join_b ? N : 0; j.parts = p.splits; j.parts_b = p.splits * p.ktiles;
+    j.n = join_w ? nk : 0; j.nb = join_b ? N : 0; j.parts = p.splits; j.parts_b = p.splits * p.turns;
     j.acc = accumulate; j.acc_b = bias_accumulate;
     const size_t blocks = (j.n + 1023) / 1024;
     j.blocks = (int)(blocks < 4096 ? blocks : 4096);

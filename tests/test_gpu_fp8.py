@@ -312,6 +312,41 @@ def test_one_launch_is_packing_and_product(dev, rows, k, n):
     assert _same(buf[:rows], want) and bool((buf[rows:] == 7.0).all()) and bool((q[rows:] == 0x11).all()) and bool((s[rows:] == 0x11).all())
 
 
+# sizes around the limits of the form that rounds x inside a small product: rows, K, N
+SMALL_SAVE = [(1, 1, 1), (1, 1000, 70), (16, 272, 4200), (31, 130, 33), (32, 520, 40), (33, 128, 16), (64, 1001, 328), (777, 200, 137), (1000, 384, 500),
+              (512, 1024, 640), (20, 4097, 64), (2048, 96, 328), (777, 1000, 1024)]
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,k,n", SMALL_SAVE)
+def test_packed_inside_a_small_product(dev, rows, k, n, dt, fmt):
+    """The kept x is that of packing alone and y that of the kept x, bit for bit; nothing behind either is written, and y without
+    keeping x holds the product's bound."""
+    from mad_amd import _lib, ops
+    x, w, bias, res = (t.to(dev) for t in _linear_case(rows, k, n, dt, dev, 60))
+    if rows > 8:
+        x[3, k // 2], x[5, 0], x[6] = float("nan"), float("inf"), 0.0
+        x[7] *= 2.0 ** -120
+    pw = ops.pack_weight_fp8(w)
+    x8 = ops.pack_fp8(x, fmt)
+    stored = {"e4m3": _lib.MAD_E4M3, "e5m2": _lib.MAD_E5M2}[fmt]
+    for b, r in ((None, None), (bias, res)):
+        want = ops.linear_fp8(x8, pw, bias=b, residual=r)
+        y = torch.full((rows + 2, n), 7.0, dtype=dt, device=dev)
+        q, s = (torch.full((rows + 2, t.shape[1]), 0x11, dtype=torch.uint8, device=dev) for t in (x8.q, x8.scale))
+        ops.check(_lib.lib.mad_linear_fp8_save(x.data_ptr(), ops._dtype_code(x), stored, pw.q.data_ptr(), pw.scale.data_ptr(),
+                                               None if b is None else b.data_ptr(), None if r is None else r.data_ptr(), y.data_ptr(),
+                                               q.data_ptr(), s.data_ptr(), rows, k, n, torch.cuda.current_stream().cuda_stream), "mad_linear_fp8_save")
+        assert _same(q[:rows].view(x8.q.dtype).float(), x8.q.float()) and torch.equal(s[:rows], x8.scale) and not bool(q[:rows, k:].any())
+        assert _same(y[:rows], want)
+        assert bool((y[rows:] == 7.0).all()) and bool((q[rows:] == 0x11).all()) and bool((s[rows:] == 0x11).all())
+    if fmt == "e4m3":
+        ok = [i for i in range(rows) if i not in (3, 5)]
+        xv, wv = R.pack_rows(x.cpu()[ok])[0], R.pack_weight(w.cpu())[0]
+        _close(ops.linear_fp8(x, pw)[ok], xv @ wv.t(), xv.abs() @ wv.abs().t(), k, dt, _eights(xv, wv))
+
+
 @pytest.mark.parametrize("rows", [3, 300])
 def test_rows_do_not_touch_each_other(dev, rows):
     """NaN and infinities in one row reach that row of y alone, and zero rows give the bias."""
