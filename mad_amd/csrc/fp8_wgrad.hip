@@ -5,8 +5,8 @@
 // The scale of x changes along the reduction (one per row m), so the product cannot run on 8-bit operands; but bf16 holds
 // every restored value exactly (to 2^-133, its smallest step), so x is widened on its way into LDS and the product runs on
 // v_mfma_f32_16x16x32_bf16 without a further rounding.  dy is bf16, or fp32 cut into three bf16 terms whose sum is dy (x is
-// exact, so three products give fp32 accuracy).  Both operands are stored with the reduction index slow and read with the transposing LDS
-// read (ds_read_b64_tr_b16: a row of 16 lanes fetches 4 rows m x 16 columns, lane i receives column i).
+// exact, so three products give fp32 accuracy).  Both operands are stored with the reduction index slow and read with the
+// transposing LDS read (ds_read_b64_tr_b16: a row of 16 lanes fetches 4 rows m x 16 columns, lane i receives column i).
 // Shares of the rows write partial sums that a second kernel adds in share order: the result does not depend on timing.
 //
 // db is the gradient of an input column of ones: one more product per fragment of dy.  A workgroup makes it for every
@@ -185,7 +185,8 @@ __global__ __launch_bounds__(2 * BK) void wgrad_fp8_kernel(F8WgradArgs a) {
             for (int p = 0; p < NP; ++p)
 #pragma unroll
                 for (int j = 0; j < FB; ++j)
-                    accb[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, frag(st + p * TILE, wn * 64 + 16 * (wk * FB + j)), accb[j], 0, 0, 0);
+                    accb[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, frag(st + p * TILE, wn * 64 + 16 * (wk * FB + j)), accb[j],
+                                                                      0, 0, 0);
         }
         if (a.db) turn = turn + 1 == a.turns ? 0 : turn + 1;
         bf16x8 xf[4];
@@ -237,6 +238,8 @@ __global__ __launch_bounds__(2 * BK) void wgrad_fp8_kernel(F8WgradArgs a) {
 // slots that only the lane that copied them reads (registers filled by ordinary loads had the compiler wait for them early), and are
 // widened into the next stage between the products of this one, so that one barrier per step remains.  Columns past the end read
 // what lies there, which only reaches results that are not stored; rows past the share are zeros (reads outside their buffer).
+// 8192 x 4096 -> 4096 234 us, 1170 TFLOP/s (a library's bf16 product of 8192^3: 1383).  Bound by LDS: a step of 64 rows reads and writes
+// about 270 KB of it for 1500 cycles of products.
 template <int BN, int BK> struct F8Wg {
     static constexpr int ROWS = 64, DY = ROWS * BN * 2, STAGE = DY + ROWS * BK * 2;
     static constexpr int RAW = ROWS * BK, SCALES = 2 * ROWS * 8;          // x as it comes; scales of two steps, two dwords per row
@@ -276,7 +279,8 @@ __global__ __launch_bounds__(64 * WN * WK) void wgrad_fp8_tile_kernel(F8WgradArg
 #pragma unroll
     for (int j = 0; j < DPW; ++j) {
         const int c = j * NW + wave;                                      // half c / 16, rows 4 (c % 16) ..
-        doff[j] = (unsigned)((4 * (c & 15) + lr) * a.N * 2 + (n0 + (c >> 4) * 128) * 2 + (((lane & 15) ^ swizzle(4 * wave + lr)) << 4));   // NW is even
+        doff[j] = (unsigned)((4 * (c & 15) + lr) * a.N * 2 + (n0 + (c >> 4) * 128) * 2 +
+                             (((lane & 15) ^ swizzle(4 * wave + lr)) << 4));                  // (NW is even)
     }
     unsigned xoff[XPT];
     int xdst[XPT], sbyte[XPT], odd = 0;
@@ -374,7 +378,8 @@ __global__ __launch_bounds__(64 * WN * WK) void wgrad_fp8_tile_kernel(F8WgradArg
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int j = 0; j < FB; ++j)
-                    accb[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, frag(st, wn * (BN / WN) + 16 * (wk * FB + j), h), accb[j], 0, 0, 0);
+                    accb[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, frag(st, wn * (BN / WN) + 16 * (wk * FB + j), h), accb[j],
+                                                                      0, 0, 0);
         }
         if (a.db) turn = turn + 1 == a.turns ? 0 : turn + 1;
 #pragma unroll
