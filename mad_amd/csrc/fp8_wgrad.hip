@@ -238,7 +238,7 @@ __global__ __launch_bounds__(2 * BK) void wgrad_fp8_kernel(F8WgradArgs a) {
 // slots that only the lane that copied them reads (registers filled by ordinary loads had the compiler wait for them early), and are
 // widened into the next stage between the products of this one, so that one barrier per step remains.  Columns past the end read
 // what lies there, which only reaches results that are not stored; rows past the share are zeros (reads outside their buffer).
-// 8192 x 4096 -> 4096 234 us, 1170 TFLOP/s (a library's bf16 product of 8192^3: 1383).  Bound by LDS: a step of 64 rows reads and writes
+// 8192 x 4096 -> 4096 247 us, 1110 TFLOP/s (a library's bf16 product of 8192^3: 1383).  Bound by LDS: a step of 64 rows reads and writes
 // about 270 KB of it for 1500 cycles of products.
 template <int BN, int BK> struct F8Wg {
     static constexpr int ROWS = 64, DY = ROWS * BN * 2, STAGE = DY + ROWS * BK * 2;
