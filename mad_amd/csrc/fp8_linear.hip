@@ -67,24 +67,22 @@ __host__ __device__ __forceinline__ bool whole_pieces(const void* x, int dtype, 
     return K % (dtype == MAD_BF16 ? 8 : 4) == 0 && ((uintptr_t)x & 15) == 0;
 }
 
-// Lanes g = 0 .. 3 (16 apart) hold the 8-byte pieces g, 4 + g, 8 + g, 12 + g of a block: afterwards pieces 4g .. 4g + 3.
-__device__ __forceinline__ void gather_pieces(i32x8& v) {
-#pragma unroll
-    for (int d = 0; d < 2; ++d) {
-        const auto a = __builtin_amdgcn_permlane16_swap((unsigned)v[d], (unsigned)v[2 + d], false, false);
-        const auto b = __builtin_amdgcn_permlane16_swap((unsigned)v[4 + d], (unsigned)v[6 + d], false, false);
-        const auto e = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
-        const auto o = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
-        v[d] = (int)e[0]; v[2 + d] = (int)o[0]; v[4 + d] = (int)e[1]; v[6 + d] = (int)o[1];
-    }
+// Lanes come in pairs with rows r and r + 1.  Each has loaded a piece of both, so that a load of the wave touches eight rows, a whole
+// line of each: even lanes keep that of r and pass on the other, odd lanes the other way round.  (With 16 rows and half a line of
+// each to a load, us: packed 256 x 2048 -> 2048 11.3 / 8.2 in pairs, fp32 16 x 4096 -> 8192 15.5 / 11.6.)
+__device__ __forceinline__ void swap_pair(bool odd, unsigned& a, unsigned& b) {
+    const unsigned t = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(odd ? a : b), 0xB1, 0xF, 0xF, true);     // lane ^ 1
+    a = odd ? t : a;
+    b = odd ? b : t;
 }
 
 // Direct form: operands from global memory straight into registers, (16 MF) x (16 NF) outputs per workgroup, its NW
 // waves taking every NW-th block of the reduction.  Few rows are bound by the latency of reading the weights once, so the reduction
 // is spread over many waves; their sums are joined through LDS pairwise, wave w and w + NW/2 first: a fixed order.  x may come
 // unpacked: it is rounded to XF on its way in, by every workgroup that needs it, and kept in memory by the first of them if asked.
-// Measured: 1 x 768 -> 768 2.6 us packed, 3.1 from bf16 (a launch); 32 x 4096 -> 8192 13.8 / 18.2 (the weights at 2.4 TB/s; loading a
-// block ahead of the products gains nothing, and costs the forms that round x their registers: 1024 x 384 -> 384 5.4 / 8.5).
+// Measured: 1 x 768 -> 768 2.6 us packed, 3.3 from bf16 (a launch); 32 x 4096 -> 8192 from bf16 12.1 with the weights in the
+// last-level cache (2.8 TB/s), 16.6 with none there.  Loading a block ahead of the products gained nothing and cost the forms that
+// round x their registers; so did starting the workgroups at different blocks.
 template <int XK, int XF, typename TO, int MF, int NF, int NW>
 __global__ __launch_bounds__(64 * NW) void linear_fp8_direct_kernel(F8LinArgs a) {
     __shared__ __attribute__((aligned(16))) f32x4 red[NW / 2][MF * NF][64];
@@ -113,15 +111,22 @@ __global__ __launch_bounds__(64 * NW) void linear_fp8_direct_kernel(F8LinArgs a)
 #pragma unroll
         for (int i = 0; i < MF; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
+    // a lane's 32 bytes of a block are chunks g and g + 4 of its row
+    const bool odd = r & 1;
+    auto fragment = [&](const auto& rsrc, int row0, int kt) {
+        const int c = kt * F8_BLOCK + 64 * (r & 1) + 16 * g, off = (row0 + (r & ~1)) * wp + c;
+        uint4 v = load16(rsrc, c < wp ? off : (int)F8_OUTSIDE), w = load16(rsrc, c < wp ? off + wp : (int)F8_OUTSIDE);
+        swap_pair(odd, v.x, w.x); swap_pair(odd, v.y, w.y); swap_pair(odd, v.z, w.z); swap_pair(odd, v.w, w.w);
+        return pair16(v, w);
+    };
 #pragma unroll 1
     for (int kt = wave; kt < kb; kt += NW) {
-        const int c = kt * F8_BLOCK + 32 * g;
+        const int c = kt * F8_BLOCK + 16 * g;
         i32x8 wf[NF];
         int wsc[NF];
 #pragma unroll
         for (int j = 0; j < NF; ++j) {
-            const int off = (16 * j + r) * wp + c;
-            wf[j] = pair16(load16(wbuf, c < wp ? off : (int)F8_OUTSIDE), load16(wbuf, c + 16 < wp ? off + 16 : (int)F8_OUTSIDE));
+            wf[j] = fragment(wbuf, 16 * j, kt);
             wsc[j] = (unsigned char)__builtin_amdgcn_raw_buffer_load_b8(wsbuf, ((n0 % F8_BLOCK + 16 * j + r) / F8_BLOCK) * sp + kt, 0, 0);
         }
 #pragma unroll
@@ -129,74 +134,98 @@ __global__ __launch_bounds__(64 * NW) void linear_fp8_direct_kernel(F8LinArgs a)
             i32x8 xf;
             int xsc;
             if constexpr (XK < X_BF16) {
-                const int off = (16 * i + r) * wp + c;
-                xf = pair16(load16(xbuf, c < wp ? off : (int)F8_OUTSIDE), load16(xbuf, c + 16 < wp ? off + 16 : (int)F8_OUTSIDE));
+                xf = fragment(xbuf, 16 * i, kt);
                 xsc = (unsigned char)__builtin_amdgcn_raw_buffer_load_b8(xsbuf, (16 * i + r) * sp + kt, 0, 0);
             } else {
                 using T = typename std::conditional<XK == X_BF16, bf16_t, float>::type;
-                // unpacked, the lanes of a row load pieces of eight columns in turn, so that a load touches one or two lines of each
-                // row, and exchange them once rounded (fp32 16 x 4096 -> 8192 18.3 us with 32 columns in a run, 15.7 so)
-                const int c8 = kt * F8_BLOCK + 8 * g;
-                unsigned u = 0;
-                // the row's block: this lane's quarter and those of the lanes 16, 32 and 48 on
-                auto over_block = [](unsigned v) {
-                    unsigned t = __shfl_xor(v, 16); v = t > v ? t : v;
-                    t = __shfl_xor(v, 32); return t > v ? t : v;
+                // unpacked: pieces q of eight columns, 0 and 1 of the pair's even row, 2 and 3 of its odd one
+                const int c8 = kt * F8_BLOCK + 16 * g + 8 * (r & 1), row0 = 16 * i + (r & ~1);
+                auto reduce = [](unsigned v, auto top) {                   // over the eight lanes that hold a row
+                    v = top(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
+                    v = top(v, __shfl_xor(v, 16));
+                    return top(v, __shfl_xor(v, 32));
                 };
+                int sc[2];
                 if (XK == X_BF16 && whole) {
                     // on pairs of bf16 as they are: their magnitudes' maximum as 16-bit integers, and one conversion for two
+                    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+                    auto top16 = [](unsigned a, unsigned b) {
+                        return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+                    };
                     uint4 v[4];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) v[q] = load16(xbuf, c8 + 32 * q < a.K ? (16 * i + r) * xpitch + 2 * c8 + 64 * q : (int)F8_OUTSIDE);
+                    for (int q = 0; q < 4; ++q) {
+                        const int col = c8 + 64 * (q & 1);
+                        v[q] = load16(xbuf, col < a.K ? (row0 + (q >> 1)) * xpitch + 2 * col : (int)F8_OUTSIDE);
+                    }
                     const unsigned* w = &v[0].x;
-                    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-                    u16x2 m = {0, 0};
+                    unsigned m[2] = {0, 0};
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[e] & 0x7fff7fffu));
-                    u = m[0] > m[1] ? m[0] : m[1];
-                    if (__any(u >= 0x7f80u)) {                             // something is not finite: it does not count
-                        u = 0;
+                    for (int e = 0; e < 16; ++e) m[e >> 3] = top16(m[e >> 3], w[e] & 0x7fff7fffu);
+                    // of the even row in the low half, of the odd one in the high half
+                    unsigned u = top16(m[0] & 0xffffu, m[0] >> 16) | top16(m[1] & 0xffffu, m[1] >> 16) << 16;
+                    if (__any((u & 0xffffu) >= 0x7f80u || u >= 0x7f800000u)) {     // something is not finite: it does not count
+                        unsigned f[2] = {0, 0};
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             const unsigned lo = w[e] & 0x7fffu, hi = w[e] >> 16 & 0x7fffu;
-                            u = lo < 0x7f80u && lo > u ? lo : u;
-                            u = hi < 0x7f80u && hi > u ? hi : u;
+                            unsigned& t = f[e >> 3];
+                            t = lo < 0x7f80u && lo > t ? lo : t;
+                            t = hi < 0x7f80u && hi > t ? hi : t;
                         }
+                        u = f[0] | f[1] << 16;
                     }
-                    xsc = (int)f8_scale_byte<XF>(over_block(u) << 16);
-                    const float scale = f8_scale((unsigned)xsc);
+                    u = reduce(u, top16);
+                    sc[0] = (int)f8_scale_byte<XF>(u << 16);
+                    sc[1] = (int)f8_scale_byte<XF>(u & 0xffff0000u);
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) xf[q] = (int)f8_cvt4_bf16<XF>(w[2 * q], w[2 * q + 1], scale);
+                    for (int q = 0; q < 8; ++q) xf[q] = (int)f8_cvt4_bf16<XF>(w[2 * q], w[2 * q + 1], f8_scale((unsigned)sc[q >> 2]));
                 } else {
+                    auto top32 = [](unsigned a, unsigned b) { return a > b ? a : b; };
                     float f[32];
                     if (whole) {
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) {                      // 32 floats; the last block's lanes behind K read zeros
-                            const int col = c8 + 32 * (q >> 1) + 4 * (q & 1);
-                            const uint4 v = load16(xbuf, col < a.K ? (16 * i + r) * xpitch + 4 * col : (int)F8_OUTSIDE);
+                        for (int q = 0; q < 8; ++q) {                      // 32 floats; lanes behind K read zeros
+                            const int col = c8 + 64 * (q >> 1 & 1) + 4 * (q & 1);
+                            const uint4 v = load16(xbuf, col < a.K ? (row0 + (q >> 2)) * xpitch + 4 * col : (int)F8_OUTSIDE);
                             f[4 * q] = __uint_as_float(v.x); f[4 * q + 1] = __uint_as_float(v.y);
                             f[4 * q + 2] = __uint_as_float(v.z); f[4 * q + 3] = __uint_as_float(v.w);
                         }
                     } else {                                               // rows that start, or end, anywhere
-                        const long m = m0 + 16 * i + r < a.M ? m0 + 16 * i + r : a.M - 1;
-                        const T* p = (const T*)a.x + (size_t)m * a.K + c8;
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) load8_tail<T>(p + 32 * q, c8 + 32 * q, a.K, f + 8 * q);
+                        for (int q = 0; q < 4; ++q) {
+                            const long m = m0 + row0 + (q >> 1) < a.M ? m0 + row0 + (q >> 1) : a.M - 1;
+                            const int col = c8 + 64 * (q & 1);
+                            load8_tail<T>((const T*)a.x + (size_t)m * a.K + col, col, a.K, f + 8 * q);
+                        }
                     }
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) { const unsigned t = f8_mag(f[e]); u = t > u ? t : u; }
-                    xsc = (int)f8_scale_byte<XF>(over_block(u));
-                    const float inv = f8_inv_scale((unsigned)xsc);
+                    for (int h = 0; h < 2; ++h) {
+                        unsigned u = 0;
 #pragma unroll
-                    for (int q = 0; q < 8; ++q)
-                        xf[q] = (int)f8_cvt4<XF>(f[4 * q] * inv, f[4 * q + 1] * inv, f[4 * q + 2] * inv, f[4 * q + 3] * inv);
+                        for (int e = 0; e < 16; ++e) u = top32(u, f8_mag(f[16 * h + e]));
+                        sc[h] = (int)f8_scale_byte<XF>(reduce(u, top32));
+                        const float inv = f8_inv_scale((unsigned)sc[h]);
+#pragma unroll
+                        for (int q = 4 * h; q < 4 * h + 4; ++q)
+                            xf[q] = (int)f8_cvt4<XF>(f[4 * q] * inv, f[4 * q + 1] * inv, f[4 * q + 2] * inv, f[4 * q + 3] * inv);
+                    }
                 }
-                gather_pieces(xf);
+                xsc = odd ? sc[1] : sc[0];
+                // after the swap xf[0 .. 3] are the even lane's pieces of this lane's row, xf[4 .. 7] the odd lane's
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    unsigned u = (unsigned)xf[q], w = (unsigned)xf[4 + q];
+                    swap_pair(odd, u, w);
+                    xf[q] = (int)u; xf[4 + q] = (int)w;
+                }
+                // xf[0,1], xf[4,5] are the halves of chunk g, xf[2,3], xf[6,7] those of chunk g + 4
+                { const int t0 = xf[2], t1 = xf[3]; xf[2] = xf[4]; xf[3] = xf[5]; xf[4] = t0; xf[5] = t1; }
                 if (a.q && n0 == 0 && 16 * i + r < mrem) {
                     const size_t row = (size_t)m0 + 16 * i + r;
                     uint4* to = reinterpret_cast<uint4*>(a.q + row * wp + c);
                     if (c < wp) to[0] = uint4{(unsigned)xf[0], (unsigned)xf[1], (unsigned)xf[2], (unsigned)xf[3]};
-                    if (c + 16 < wp) to[1] = uint4{(unsigned)xf[4], (unsigned)xf[5], (unsigned)xf[6], (unsigned)xf[7]};
+                    if (c + 64 < wp) to[4] = uint4{(unsigned)xf[4], (unsigned)xf[5], (unsigned)xf[6], (unsigned)xf[7]};
                     if (g == 0) {
                         a.scale[row * sp + kt] = (unsigned char)xsc;
                         for (int k = kt + 1; kt == kb - 1 && k < sp; ++k) a.scale[row * sp + k] = 127;
@@ -684,12 +713,12 @@ template <int XK, int XF, typename TO> static int launch_linear(F8LinArgs a, hip
         }
     }
     // Of the direct form, the smaller its workgroups the more of them share the latency, until re-reading costs more.  Sixteen by
-    // sixteen results each up to two workgroups for each unit, then 32 x 32, then 64 x 64 (packed x, us: 64 x 1024 -> 1024 3.6 / 4.9
-    // / 7.5, 64 x 4096 -> 4096 20.9 / 12.4 / 25, 1024 x 4096 -> 1024 73 / 39 / 23).  Where x is rounded on its way in, every
-    // workgroup rounds it again, so they get wider in n first (16 x 4096 -> 8192 19.7 / 14.9 for 16 / 32 columns); in m too if it is
-    // bf16, not if it is fp32, whose registers leave room for one such workgroup to a unit (777 x 1000 -> 328 9.6 / 12.3 for 16 / 32
-    // rows, 501 x 200 -> 137 4.0 / 5.5).  Eight waves in the first two, so that a result is the same sum whether x came packed or is
-    // kept packed on the way (four / eight in 32 x 32: 1024 x 384 -> 384 4.4 / 4.7, fp32 64 x 4096 -> 4096 13.8 / 12.5).
+    // sixteen results each up to two workgroups for each unit, then 32 x 32, then 64 x 64 (packed x, us, 16 / 32: 64 x 4096 -> 4096
+    // 14.5 / 12.8, 256 x 4096 -> 1024 13.3 / 9.7; 32 / 64: 1024 x 4096 -> 1024 39 / 23).  Where x is rounded on its way in, every
+    // workgroup rounds it again, so they get wider in n first (16 x 4096 -> 8192 10.6 / 8.2 for 16 / 32 columns), not in m, which
+    // costs registers (32 x 4096 -> 8192 11.9 / 14.7 for 16 / 32 rows, fp32 777 x 1000 -> 328 9.6 / 12.3).  Eight waves, so that a
+    // result is the same sum whether x came packed or is kept packed on the way (packed, four / eight waves in 32 x 32:
+    // 1024 x 384 -> 384 4.4 / 4.7, fp32 64 x 4096 -> 4096 13.8 / 12.5).
     const long f = ((a.M + 15) / 16) * ((a.N + 15) / 16), cus = f8_cus();
     if constexpr (XK < X_BF16) {
         if (f <= 2 * cus) return launch_direct<XK, XF, TO, 1, 1, 8>(a, s);
@@ -697,7 +726,7 @@ template <int XK, int XF, typename TO> static int launch_linear(F8LinArgs a, hip
     } else {
         if (f <= cus) return launch_direct<XK, XF, TO, 1, 1, 8>(a, s);
         if (a.M <= 16 && !a.q) return launch_direct<XK, XF, TO, 1, 2, 16>(a, s);
-        return launch_direct<XK, XF, TO, XK == X_BF16 ? 2 : 1, 2, 8>(a, s);
+        return launch_direct<XK, XF, TO, 1, 2, 8>(a, s);
     }
 }
 
@@ -768,9 +797,9 @@ extern "C" int mad_linear_fp8(const void* x, int x_type, const void* x_scale, co
 }
 
 // Whether the direct form rounds x on its way in for less than a launch of its own costs: a few rows, or few 32 x 32 pieces of y and
-// blocks for each (us of the GPU, rounding inside / packing first: bf16 777 x 1000 -> 328 6.8 / 9.1, 777 x 1000 -> 1024 11.4 / 11.4,
-// 2048 x 1000 -> 1024 25 / 16, 256 x 4096 -> 1024 14.5 / 15.3, 256 x 4096 -> 4096 48 / 26; fp32, or rows that start anywhere, twice
-// the work: fp32 777 x 1000 -> 328 9.6 / 9.6, 777 x 1000 -> 1024 18 / 13, 32 x 4096 -> 8192 26 / 15).  The host's time for the
+// blocks for each (us of the GPU, rounding inside / packing first: bf16 777 x 1000 -> 328 7.0 / 8.8, 777 x 1000 -> 1024 13.1 / 12.4,
+// 2048 x 1000 -> 1024 30 / 16, 256 x 4096 -> 1024 12.1 / 13.4, 256 x 4096 -> 4096 38 / 25; fp32, or rows that start anywhere, twice
+// the work: fp32 777 x 1000 -> 328 8.8 / 8.8, 777 x 1000 -> 1024 17 / 13, 32 x 4096 -> 8192 18 / 12).  The host's time for the
 // second launch and its buffers, 6 us, comes on top.
 // Where the packed x is kept, only sizes whose packed form adds in the same order: y is then the product of what is kept, bit for bit.
 static bool direct_rounds(const void* x, int dtype, long rows, int K, int N, bool keep) {
