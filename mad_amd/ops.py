@@ -849,6 +849,8 @@ def _fp8_empty(rows: int, c: int, fmt: str, device) -> Tuple[Tensor, Tensor]:
 
 def _fp8_check(p: Fp8Tensor, what: str) -> Tuple[int, int, int]:
     """(rows, columns, type code) of a packed tensor whose parts fit its shape."""
+    if not isinstance(p, Fp8Tensor):
+        raise TypeError(f"{what}: needs an Fp8Tensor, got {type(p).__name__}")
     rows, c = _fp8_rows(p.shape, what)
     _dev(p.q, p.scale)
     if p.q.dtype not in _FP8_CODES or p.scale.dtype != torch.uint8:
@@ -977,6 +979,8 @@ def linear_fp8(x: Union[Tensor, Fp8Tensor], w: Fp8Weight, bias: Optional[Tensor]
     """y (..., N) = x . w^T + bias (+ residual) with both operands in 8 bits and fp32 sums, in the type of ``x``.  ``x``
     (..., K) is bf16 / fp32, rounded to e4m3 as ``pack_fp8`` does, or already packed.  ``save`` also returns the packed x, which
     ``linear_fp8_backward`` takes."""
+    if not isinstance(w, Fp8Weight):
+        raise TypeError(f"linear_fp8: needs a weight packed by pack_weight_fp8, got {type(w).__name__}")
     N, K = w.shape
     _fp8_weight_check(w.q, w.scale, N, K, "linear_fp8")
     if isinstance(x, Fp8Tensor):
@@ -1019,7 +1023,7 @@ def linear_fp8_backward(dy: Tensor, x: Fp8Tensor, w: Optional[Fp8Weight] = None,
             raise ValueError(f"linear_fp8_backward: {what} must be fp32 with {n} elements")
     dx = None
     if need_dx:
-        if w is None or tuple(w.shape) != (N, K):
+        if not isinstance(w, Fp8Weight) or tuple(w.shape) != (N, K):
             raise ValueError(f"linear_fp8_backward: dx needs the packed weight ({N}, {K})")
         _fp8_weight_check(w.qt, w.scale_t, K, N, "linear_fp8_backward")
         dx, _ = _linear_fp8(dy, rows, N, grad_fmt, False, w.qt, w.scale_t, K, None, None, "linear_fp8_backward")

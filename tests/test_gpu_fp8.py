@@ -483,6 +483,20 @@ def test_refusals_on_the_gpu(dev):
         ops.gn_apply_save(x.view(1, 2, 4, 96), torch.zeros((1, 95, 2), device=dev), True)
 
 
+def test_refusals_of_what_is_not_packed(dev):
+    from mad_amd import ops
+    x, w, _, _ = _linear_case(8, 96, 40, torch.bfloat16, dev, 3)
+    x, w = x.to(dev), w.to(dev)
+    pw = ops.pack_weight_fp8(w, transposed=True)
+    y, x8 = ops.linear_fp8(x, pw, save=True)
+    for call in (lambda: ops.linear_fp8(x, w), lambda: ops.unpack_fp8(x), lambda: ops.linear_fp8_backward(y, x, pw),
+                 lambda: ops.gn_apply_restore(x.view(1, 2, 4, 96), torch.zeros((1, 96, 2), device=dev), True)):
+        with pytest.raises(TypeError, match="pack_weight_fp8|Fp8Tensor"):
+            call()
+    with pytest.raises(ValueError, match="packed weight"):
+        ops.linear_fp8_backward(y, x8, w)
+
+
 # ------------------------------------------------------------------ gradients
 BACKWARD = [(1, 16, 8), (5, 200, 137), (64, 128, 128), (300, 96, 260), (700, 384, 130), (1500, 130, 70), (2100, 256, 384)]
 
@@ -514,6 +528,10 @@ def test_linear_backward(dev, rows, k, n, fmt, dt):
 # rows, K, N: many shares of the rows, tiles of 128 and of 256, ragged in every direction, rows of dy that are no whole 16 bytes
 WGRAD_LARGE = [(66000, 272, 136), (333, 4000, 4104), (20001, 384, 1152), (5000, 16, 8), (3000, 1040, 131), (64, 4096, 4096), (129, 130, 264),
                (30000, 768, 2304), (9000, 640, 520), (2000, 1152, 1536), (40000, 200, 1152)]
+
+
+# as many tiles as units and rows enough that the bias gradient is shared over them: one share, and its parts joined alone
+WGRAD_LARGE += [(5000, 4096, 4112), (4001, 4100, 4095)]
 
 
 @pytest.mark.parametrize("dt", DTYPES)
