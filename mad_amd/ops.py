@@ -822,9 +822,19 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
 
-def _fp8_call(name: str, t: Tensor, *args) -> None:
-    """One entry point on the device of ``t``, on the stream that is current there."""
+def _fp8_dev(t: Tensor, *others: Optional[Tensor]) -> int:
+    """The index of the device that all of them are on; ``_dev`` says what is wrong with them otherwise."""
     i = t.get_device()
+    if i < 0 or not t.is_contiguous():
+        _dev(t)
+    for o in others:
+        if o is not None and (o.get_device() != i or not o.is_contiguous()):
+            _dev(t, o)
+    return i
+
+
+def _fp8_call(name: str, i: int, *args) -> None:
+    """One entry point on device ``i``, on the stream that is current there."""
     if i == _current_device():
         status = getattr(lib, name)(*args, _raw_stream(i))
     else:
@@ -851,13 +861,15 @@ def _fp8_check(p: Fp8Tensor, what: str) -> Tuple[int, int, int]:
     """(rows, columns, type code) of a packed tensor whose parts fit its shape."""
     if not isinstance(p, Fp8Tensor):
         raise TypeError(f"{what}: needs an Fp8Tensor, got {type(p).__name__}")
-    rows, c = _fp8_rows(p.shape, what)
-    _dev(p.q, p.scale)
-    if p.q.dtype not in _FP8_CODES or p.scale.dtype != torch.uint8:
-        raise TypeError(f"{what}: a packed tensor is float8_e4m3fn or float8_e5m2 with uint8 scales, got {p.q.dtype} / {p.scale.dtype}")
-    if p.q.shape != (rows, _pitch(c)) or p.scale.shape != (rows, _scale_pitch(c)):
-        raise ValueError(f"{what}: packed parts {tuple(p.q.shape)} / {tuple(p.scale.shape)} do not belong to shape {tuple(p.shape)}")
-    return rows, c, _FP8_CODES[p.q.dtype]
+    q, scale, shape, _ = p
+    rows, c = _fp8_rows(shape, what)
+    _fp8_dev(q, scale)
+    code = _FP8_CODES.get(q.dtype)
+    if code is None or scale.dtype != torch.uint8:
+        raise TypeError(f"{what}: a packed tensor is float8_e4m3fn or float8_e5m2 with uint8 scales, got {q.dtype} / {scale.dtype}")
+    if q.shape != (rows, _pitch(c)) or scale.shape != (rows, _scale_pitch(c)):
+        raise ValueError(f"{what}: packed parts {tuple(q.shape)} / {tuple(scale.shape)} do not belong to shape {tuple(shape)}")
+    return rows, c, code
 
 
 def _fp8_weight_check(q: Optional[Tensor], scale: Optional[Tensor], n: int, k: int, what: str) -> None:
@@ -872,19 +884,19 @@ def _fp8_weight_check(q: Optional[Tensor], scale: Optional[Tensor], n: int, k: i
 def pack_fp8(x: Tensor, fmt: str = "e4m3") -> Fp8Tensor:
     """``x`` (..., C) bf16 / fp32 in 8 bits, one power-of-two scale per row and 128 columns (the format: ``Fp8Tensor``).
     NaN stays NaN and does not count towards its block's scale; an infinity becomes NaN (e4m3) or stays one (e5m2)."""
-    _dev(x)
-    code = _dtype_code(x)
-    rows, c = _fp8_rows(x.shape, "pack_fp8")
+    i = _fp8_dev(x)
+    code, shape = _dtype_code(x), x.shape
+    rows, c = _fp8_rows(shape, "pack_fp8")
     q, scale = _fp8_empty(rows, c, fmt, x.device)
-    _fp8_call("mad_pack_fp8", x, _ptr(x), code, _FP8_TYPES[fmt][1], rows, c, _ptr(q), _ptr(scale))
-    return Fp8Tensor(q, scale, x.shape, x.dtype)
+    _fp8_call("mad_pack_fp8", i, x.data_ptr(), code, _FP8_TYPES[fmt][1], rows, c, q.data_ptr(), scale.data_ptr())
+    return Fp8Tensor(q, scale, shape, x.dtype)
 
 
 def unpack_fp8(p: Fp8Tensor) -> Tensor:
     """The values ``p`` stands for, in the type and shape of the tensor that was packed."""
     rows, c, fmt = _fp8_check(p, "unpack_fp8")
     x = torch.empty(p.shape, dtype=p.dtype, device=p.q.device)
-    _fp8_call("mad_unpack_fp8", x, _ptr(p.q), _ptr(p.scale), fmt, rows, c, _ptr(x), _dtype_code(x))
+    _fp8_call("mad_unpack_fp8", x.get_device(), p.q.data_ptr(), p.scale.data_ptr(), fmt, rows, c, x.data_ptr(), _dtype_code(x))
     return x
 
 
@@ -898,16 +910,16 @@ def _coef_check(coef: Tensor, shape: Sequence[int], what: str) -> None:
 def gn_apply_save(x: Tensor, coef: Tensor, act: bool, drop_seed: int = 0, drop_p: float = 0.0) -> Tuple[Tensor, Fp8Tensor]:
     """``gn_apply(x, coef, act, drop_seed=, drop_p=)`` and, from the same pass, ``x`` packed in e4m3: what
     ``gn_apply_restore`` gives the backward ``x`` and the activation back from."""
-    _dev(x, coef)
-    code = _dtype_code(x)
-    _coef_check(coef, x.shape, "gn_apply_save")
-    B, H, W_, C = x.shape
-    rows, _ = _fp8_rows(x.shape, "gn_apply_save")
+    i = _fp8_dev(x, coef)
+    code, shape = _dtype_code(x), x.shape
+    _coef_check(coef, shape, "gn_apply_save")
+    rows, C = _fp8_rows(shape, "gn_apply_save")
+    B = shape[0]
     y = torch.empty_like(x)
     q, scale = _fp8_empty(rows, C, "e4m3", x.device)
-    _fp8_call("mad_gn_apply_save_fp8", x, _ptr(x), _ptr(coef), _ptr(y), _ptr(q), _ptr(scale), code, B, H * W_, C, int(act),
-              drop_seed, float(drop_p))
-    return y, Fp8Tensor(q, scale, x.shape, x.dtype)
+    _fp8_call("mad_gn_apply_save_fp8", i, x.data_ptr(), coef.data_ptr(), y.data_ptr(), q.data_ptr(), scale.data_ptr(), code, B,
+              shape[1] * shape[2], C, int(act), drop_seed, float(drop_p))
+    return y, Fp8Tensor(q, scale, shape, x.dtype)
 
 
 def gn_apply_restore(p: Fp8Tensor, coef: Tensor, act: bool, drop_seed: int = 0, drop_p: float = 0.0) -> Tuple[Tensor, Tensor]:
@@ -917,19 +929,19 @@ def gn_apply_restore(p: Fp8Tensor, coef: Tensor, act: bool, drop_seed: int = 0, 
     if fmt != _lib.MAD_E4M3:
         raise TypeError("gn_apply_restore: checkpoints are e4m3")
     _coef_check(coef, p.shape, "gn_apply_restore")
-    _dev(p.q, coef)
+    i = _fp8_dev(p.q, coef)
     B, H, W_, _ = p.shape
     x = torch.empty(p.shape, dtype=p.dtype, device=p.q.device)
     y = torch.empty_like(x)
-    _fp8_call("mad_gn_apply_restore_fp8", x, _ptr(p.q), _ptr(p.scale), _ptr(coef), _ptr(x), _ptr(y), _dtype_code(x), B, H * W_, C,
-              int(act), drop_seed, float(drop_p))
+    _fp8_call("mad_gn_apply_restore_fp8", i, p.q.data_ptr(), p.scale.data_ptr(), coef.data_ptr(), x.data_ptr(), y.data_ptr(),
+              _dtype_code(x), B, H * W_, C, int(act), drop_seed, float(drop_p))
     return x, y
 
 
 def pack_weight_fp8(w: Tensor, transposed: bool = False) -> Fp8Weight:
     """A weight (N, K) bf16 / fp32 in e4m3 with one power-of-two scale per 128 x 128 block; ``transposed`` also writes the
     copy ``linear_fp8_backward`` needs for the data gradient."""
-    _dev(w)
+    i = _fp8_dev(w)
     code = _dtype_code(w)
     if w.dim() != 2:
         raise ValueError(f"pack_weight_fp8: needs a matrix (N, K), got shape {tuple(w.shape)}")
@@ -941,7 +953,7 @@ def pack_weight_fp8(w: Tensor, transposed: bool = False) -> Fp8Weight:
     scales = lambda r, c: torch.empty(-(-r // FP8_BLOCK), _scale_pitch(c), dtype=torch.uint8, device=device)
     q, scale = new(N, _pitch(K)), scales(N, K)
     qt, scale_t = (new(K, _pitch(N)), scales(K, N)) if transposed else (None, None)
-    _fp8_call("mad_pack_weight_fp8", w, _ptr(w), code, N, K, _ptr(q), _ptr(scale), _ptr(qt), _ptr(scale_t))
+    _fp8_call("mad_pack_weight_fp8", i, _ptr(w), code, N, K, _ptr(q), _ptr(scale), _ptr(qt), _ptr(scale_t))
     return Fp8Weight(q, scale, (N, K), qt, scale_t)
 
 
@@ -950,7 +962,7 @@ def _linear_fp8(x: Union[Tensor, Fp8Tensor], rows: int, k: int, fmt: str, keep: 
     """(y (rows, n), x packed if ``keep``) of an x whose parts are checked."""
     packed = isinstance(x, Fp8Tensor)
     xq = x.q if packed else x
-    _dev(xq, q, scale, bias, residual)
+    i = _fp8_dev(xq, q, scale, bias, residual)
     if bias is not None and (bias.dtype != torch.float32 or bias.numel() != n):
         raise ValueError(f"{what}: bias must be fp32 with {n} elements")
     y = torch.empty(rows, n, dtype=x.dtype, device=xq.device)
@@ -959,15 +971,15 @@ def _linear_fp8(x: Union[Tensor, Fp8Tensor], rows: int, k: int, fmt: str, keep: 
     code = _dtype_code(y)
     end = TIMER.bracket("linear_fp8", 2.0 * rows * k * n)
     if packed:
-        _fp8_call("mad_linear_fp8", y, xq.data_ptr(), _FP8_CODES[xq.dtype], x.scale.data_ptr(), q.data_ptr(), scale.data_ptr(), _ptr(bias),
+        _fp8_call("mad_linear_fp8", i, xq.data_ptr(), _FP8_CODES[xq.dtype], x.scale.data_ptr(), q.data_ptr(), scale.data_ptr(), _ptr(bias),
                   _ptr(residual), y.data_ptr(), code, rows, k, n)
     elif keep or fmt != "e4m3" or lib.mad_linear_fp8_needs_pack(x.data_ptr(), code, rows, k, n):
         pq, ps = _fp8_empty(rows, k, fmt, xq.device)
-        _fp8_call("mad_linear_fp8_save", y, x.data_ptr(), code, _FP8_TYPES[fmt][1], q.data_ptr(), scale.data_ptr(), _ptr(bias),
+        _fp8_call("mad_linear_fp8_save", i, x.data_ptr(), code, _FP8_TYPES[fmt][1], q.data_ptr(), scale.data_ptr(), _ptr(bias),
                   _ptr(residual), y.data_ptr(), pq.data_ptr(), ps.data_ptr(), rows, k, n)
         x = Fp8Tensor(pq, ps, x.shape, x.dtype)
     else:
-        _fp8_call("mad_linear_fp8", y, x.data_ptr(), code, None, q.data_ptr(), scale.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(),
+        _fp8_call("mad_linear_fp8", i, x.data_ptr(), code, None, q.data_ptr(), scale.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(),
                   code, rows, k, n)
     if end is not None:
         end.record()
@@ -986,7 +998,7 @@ def linear_fp8(x: Union[Tensor, Fp8Tensor], w: Fp8Weight, bias: Optional[Tensor]
     if isinstance(x, Fp8Tensor):
         rows, c, _ = _fp8_check(x, "linear_fp8")
     else:
-        _dev(x)
+        _fp8_dev(x)
         _dtype_code(x)
         rows, c = _fp8_rows(x.shape, "linear_fp8")
     if c != K:
@@ -1009,7 +1021,7 @@ def linear_fp8_backward(dy: Tensor, x: Fp8Tensor, w: Optional[Fp8Weight] = None,
     dw = dy^T . x and dbias = column sums of dy in fp32 from the unrounded dy.  ``dw`` / ``dbias`` may be given (fp32, N*K and N
     elements) and are then overwritten or, with ``accumulate``, added to."""
     rows, K, fmt = _fp8_check(x, "linear_fp8_backward")
-    _dev(dy, x.q, dw, dbias)
+    i = _fp8_dev(dy, x.q, dw, dbias)
     code = _dtype_code(dy)
     if dy.dtype != x.dtype or dy.dim() != len(x.shape) or tuple(dy.shape[:-1]) != tuple(x.shape[:-1]):
         raise ValueError(f"linear_fp8_backward: dy {dy.dtype} {tuple(dy.shape)} does not belong to x {x.dtype} {tuple(x.shape)}")
@@ -1035,7 +1047,7 @@ def linear_fp8_backward(dy: Tensor, x: Fp8Tensor, w: Optional[Fp8Weight] = None,
     nbytes = lib.mad_linear_fp8_wgrad_workspace(rows, N, K)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device) if nbytes else None
     end = TIMER.bracket("linear_fp8_wgrad", 2.0 * rows * K * N)
-    _fp8_call("mad_linear_fp8_wgrad", dy, _ptr(dy), code, _ptr(x.q), fmt, _ptr(x.scale), _ptr(dw), _ptr(dbias), _ptr(ws), nbytes,
+    _fp8_call("mad_linear_fp8_wgrad", i, _ptr(dy), code, _ptr(x.q), fmt, _ptr(x.scale), _ptr(dw), _ptr(dbias), _ptr(ws), nbytes,
               rows, N, K, int(accumulate), int(accumulate))
     if end is not None:
         end.record()
