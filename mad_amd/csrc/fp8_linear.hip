@@ -474,8 +474,8 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
     }
 }
 
-// Row form: x in bf16 with rows of whole 16-byte pieces and at most four blocks, many rows.  A workgroup of four waves rounds its 128
-// rows once, through LDS into the fragments' registers (and to memory, if the packed x is wanted), and then walks the columns in
+// Row form: x in bf16 with rows of whole 16-byte pieces and at most nine blocks, many rows.  A workgroup of four waves (eight from
+// five blocks on) rounds its 128 rows once, through LDS into the fragments' registers (and to memory, if the packed x is wanted), and then walks the columns in
 // strips of 64, whose weights all waves read from LDS; LDS-DMA brings the next strip while one is multiplied and stored.  Bound
 // by HBM: x is read once, where packing first writes and reads a byte more per element, in another launch.  65536 x 384 -> 384
 // 25 us (100 MB, 4.0 TB/s), 32768 x 256 -> 768 21 us.
@@ -486,12 +486,13 @@ struct F8RowArgs {
     int K, N, shares;                              // shares of the columns: workgroups that round the same rows
 };
 
-template <int KB>
-__global__ __launch_bounds__(256, 2) void linear_fp8_rows_kernel(F8RowArgs a) {
-    constexpr int MF = 2, ROWS = 64 * MF, STRIP = 64 * KB * F8_BLOCK;      // rows of a workgroup, bytes of a strip
+template <int KB, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void linear_fp8_rows_kernel(F8RowArgs a) {
+    constexpr int ROWS = 128, MF = ROWS / 16 / NW, STRIP = 64 * KB * F8_BLOCK;      // rows of a workgroup, bytes of a strip
+    constexpr int SD = (KB + 3) / 4;               // dwords of a row's scales
     static_assert(2 * STRIP == ROWS * KB * F8_BLOCK, "the strips take the place of the rounded rows");
     __shared__ __attribute__((aligned(16))) unsigned char xs[2 * STRIP];
-    __shared__ unsigned sc[ROWS];                  // the row's scales, a byte per block
+    __shared__ unsigned sc[ROWS][SD];              // the rows' scales, a byte per block
     __shared__ __attribute__((aligned(16))) float extra[2][2][64];         // of a strip: its bias, and the scales of its weights
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
@@ -501,14 +502,14 @@ __global__ __launch_bounds__(256, 2) void linear_fp8_rows_kernel(F8RowArgs a) {
     const int mrem = a.M - m0 < ROWS ? (int)(a.M - m0) : ROWS;
     const int pitch = f8_pitch(a.K), sp = f8_scale_pitch(a.K);
 
-    // ---- rounding: 16 lanes to a block, a pass of the workgroup is 16 rows
+    // ---- rounding: 16 lanes to a block, a pass of the workgroup is PASS rows
     {
         const int l = tid & 15, row0 = tid >> 4;
         const auto xbuf = f8_resource(a.x + (size_t)m0 * a.K, mrem * a.K * 2);
         const bool keep = a.q && share == 0;
-        constexpr int H = KB > 2 ? 4 : 8;                                  // passes whose loads are in flight together
+        constexpr int PASS = 4 * NW, H = KB > 4 ? 2 : KB > 2 ? 4 : 8;      // H passes' loads are in flight together
 #pragma unroll
-        for (int h0 = 0; h0 < ROWS / 16; h0 += H) {
+        for (int h0 = 0; h0 < ROWS / PASS; h0 += H) {
             uint4 v[KB][H];
 #pragma unroll
             for (int h = 0; h < H; ++h)
@@ -516,12 +517,14 @@ __global__ __launch_bounds__(256, 2) void linear_fp8_rows_kernel(F8RowArgs a) {
                 for (int b = 0; b < KB; ++b) {
                     const int c = b * F8_BLOCK + 8 * l;
                     v[b][h] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
-                        xbuf, c < a.K ? ((row0 + 16 * (h0 + h)) * a.K + c) * 2 : (int)F8_OUTSIDE, 0, 0));
+                        xbuf, c < a.K ? ((row0 + PASS * (h0 + h)) * a.K + c) * 2 : (int)F8_OUTSIDE, 0, 0));
                 }
 #pragma unroll
             for (int h = 0; h < H; ++h) {
-                const int row = row0 + 16 * (h0 + h);
-                unsigned scales = 0;
+                const int row = row0 + PASS * (h0 + h);
+                unsigned scales[SD];
+#pragma unroll
+                for (int d = 0; d < SD; ++d) scales[d] = 0;
 #pragma unroll
                 for (int b = 0; b < KB; ++b) {
                     const unsigned* w = &v[b][h].x;
@@ -538,14 +541,17 @@ __global__ __launch_bounds__(256, 2) void linear_fp8_rows_kernel(F8RowArgs a) {
                     o.x = f8_cvt4_bf16<F8_E4M3>(w[0], w[1], scale);
                     o.y = f8_cvt4_bf16<F8_E4M3>(w[2], w[3], scale);
                     *reinterpret_cast<uint2*>(xs + (b * ROWS + row) * F8_BLOCK + (((l >> 1) ^ (row >> 1 & 7)) << 4) + (l & 1) * 8) = o;
-                    scales |= s << (8 * b);
+                    scales[b / 4] |= s << (8 * (b & 3));
                     if (keep && row < mrem && b * F8_BLOCK + 8 * l < pitch)
                         *reinterpret_cast<uint2*>(a.q + (size_t)(m0 + row) * pitch + b * F8_BLOCK + 8 * l) = o;
                 }
 #pragma unroll
-                for (int b = KB; b < 4; ++b) scales |= 127u << (8 * b);
-                if (l == 0) sc[row] = scales;
-                if (keep && l == 0 && row < mrem) *reinterpret_cast<unsigned*>(a.scale + (size_t)(m0 + row) * sp) = scales;
+                for (int b = KB; b < 4 * SD; ++b) scales[b / 4] |= 127u << (8 * (b & 3));
+#pragma unroll
+                for (int d = 0; d < SD; ++d) {
+                    if (l == 0) sc[row][d] = scales[d];
+                    if (keep && l == 0 && row < mrem) *reinterpret_cast<unsigned*>(a.scale + (size_t)(m0 + row) * sp + 4 * d) = scales[d];
+                }
             }
         }
     }
@@ -553,11 +559,12 @@ __global__ __launch_bounds__(256, 2) void linear_fp8_rows_kernel(F8RowArgs a) {
 
     // ---- this wave's rows as fragments: chunks g and g + 4 of row r, as in the tiled form
     i32x8 xf[KB][MF];
-    unsigned xsc[MF];
+    unsigned xsc[MF][SD];
     const int c_lo = (g ^ (r >> 1)) << 4, c_hi = c_lo ^ 64;
 #pragma unroll
     for (int i = 0; i < MF; ++i) {
-        xsc[i] = sc[16 * (MF * wave + i) + r];
+#pragma unroll
+        for (int d = 0; d < SD; ++d) xsc[i][d] = sc[16 * (MF * wave + i) + r][d];
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
             const unsigned char* p = xs + (b * ROWS + 16 * (MF * wave + i) + r) * F8_BLOCK;
@@ -570,20 +577,20 @@ __global__ __launch_bounds__(256, 2) void linear_fp8_rows_kernel(F8RowArgs a) {
     const int first = share * per, end = first + per < strips ? first + per : strips;
     const int lr = lane >> 3, chunk = (lane & 7) ^ ((4 * wave + (lr >> 1)) & 7);
     const unsigned lds0 = lds_addr(xs), ex0 = lds_addr(extra);
-    auto load_strip = [&](int t, int buf) {        // a strip's 8 KB groups of 8 rows: each wave two of every block
+    auto load_strip = [&](int t, int buf) {        // a strip's groups of 8 rows, shared out to the waves block by block
         const int nrem = a.N - 64 * t < 64 ? a.N - 64 * t : 64;
         const u32x4 wb = f8_buffer(a.w + (size_t)(64 * t) * pitch, t < end ? (unsigned)(nrem * pitch) : 0u);
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
             const unsigned off = b * F8_BLOCK + 16 * chunk < pitch ? (unsigned)((8 * wave + lr) * pitch + 16 * chunk) : F8_OUTSIDE;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < 8 / NW; ++j)
                 buf_lds16(wb, off + j * 32 * pitch, b * F8_BLOCK, lds0 + buf * STRIP + b * 64 * F8_BLOCK + (4 * j + wave) * 1024);
         }
         // by LDS-DMA as well: the wait for an ordinary load would wait for the strip in front of it
         const u32x4 bb = f8_buffer((const unsigned char*)(a.bias + 64 * t), a.bias && t < end ? (unsigned)(nrem * 4) : 0u);
         if (wave == 2) buf_lds4(bb, lane * 4, 0, ex0 + buf * 512);
-        if (wave == 3) buf_lds4(f8_buffer(a.ws + (size_t)(64 * t / F8_BLOCK) * sp, t < end ? 4u : 0u), 0, 0, ex0 + buf * 512 + 256);
+        if (wave == 3) buf_lds4(f8_buffer(a.ws + (size_t)(64 * t / F8_BLOCK) * sp, t < end ? 4u * SD : 0u), lane * 4, 0, ex0 + buf * 512 + 256);
     };
     constexpr int STORES = MF * 2;
     __syncthreads();                               // every wave has its rows: the strips may take their place
@@ -594,7 +601,9 @@ __global__ __launch_bounds__(256, 2) void linear_fp8_rows_kernel(F8RowArgs a) {
         if (counted) dma_wait_upto<STORES>(); else dma_wait_all();         // the strip is older than the stores of the one before
         __syncthreads();
         load_strip(t + 1, buf ^ 1);
-        const unsigned wsc = __float_as_uint(extra[buf][1][0]);
+        unsigned wsc[SD];
+#pragma unroll
+        for (int d = 0; d < SD; ++d) wsc[d] = __float_as_uint(extra[buf][1][d]);
         const int n = 64 * t + (g & 1) * 16 + (g >> 1) * 8;                 // this lane's first column when it stores, pair 0
         float bias[2][8];
 #pragma unroll
@@ -626,10 +635,11 @@ __global__ __launch_bounds__(256, 2) void linear_fp8_rows_kernel(F8RowArgs a) {
         _Pragma("unroll") for (int j = 0; j < 4; ++j) {                                                                              \
             const i32x8 wf = wfrag(b, j);                                                                                            \
             _Pragma("unroll") for (int i = 0; i < MF; ++i) acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(             \
-                wf, xf[b < KB ? b : 0][i], acc[j][i], F8_E4M3, F8_E4M3, b, (int)wsc, b, (int)xsc[i]);                                \
+                wf, xf[b < KB ? b : 0][i], acc[j][i], F8_E4M3, F8_E4M3, b & 3, (int)wsc[b < KB ? b / 4 : 0], b & 3,                  \
+                (int)xsc[i][b < KB ? b / 4 : 0]);                                                                                    \
         }                                                                                                                            \
     }
-        BLOCK(0) BLOCK(1) BLOCK(2) BLOCK(3)
+        BLOCK(0) BLOCK(1) BLOCK(2) BLOCK(3) BLOCK(4) BLOCK(5) BLOCK(6) BLOCK(7) BLOCK(8)
 #undef BLOCK
         auto piece = [&](int i, int p, float* v) {
 #pragma unroll
@@ -730,11 +740,15 @@ template <int XK, int XF, typename TO> static int launch_linear(F8LinArgs a, hip
     }
 }
 
-// Where the row form serves: bf16 rows of whole pieces, four blocks at most (their fragments live in registers), rows enough for one
-// workgroup to a unit, and no more columns than pay (us, packing first / rows: 32768 x 256 -> 768 27 / 21, 65536 x 384 -> 384
-// 36 / 25, 32768 x 512 -> 2048 67 / 49, 40000 x 512 -> 4096 147 / 153).
+// Where the row form serves: bf16 rows of whole pieces, nine blocks at most (their fragments live in registers, two strips of the weights
+// in LDS), rows enough for one workgroup to a unit, and no more columns than pay (us, packing first / rows: 32768 x 256 -> 768
+// 27 / 21, 65536 x 384 -> 384 36 / 25, 32768 x 512 -> 2048 67 / 49, 40000 x 512 -> 4096 147 / 153, 65536 x 1152 -> 384 80 / 68,
+// 32768 x 1024 -> 2048 94 / 84).  Beyond four blocks a unit holds one workgroup, and the last round has to be three quarters full
+// (40000 x 640 -> 640 43 / 44, 40000 x 1152 -> 384 54 / 54).
 static bool rows_form_ok(const void* x, int dtype, long rows, int K, int N) {
-    return dtype == MAD_BF16 && K % 8 == 0 && K <= 4 * F8_BLOCK && ((uintptr_t)x & 15) == 0 && (rows + 127) / 128 >= f8_cus() && N <= 2048;
+    const long tiles = (rows + 127) / 128, cus = f8_cus();
+    return dtype == MAD_BF16 && whole_pieces(x, dtype, K) && K <= 9 * F8_BLOCK && N <= 2048 && tiles >= cus &&
+           (K <= 4 * F8_BLOCK || 4 * tiles >= 3 * ((tiles + cus - 1) / cus) * cus);
 }
 
 static F8RowArgs row_args(const void* x, const void* w, const void* ws, const float* bias, const void* residual, void* y, void* q,
@@ -750,15 +764,14 @@ static int launch_rows(F8RowArgs a, hipStream_t s) {
     const long mtiles = (a.M + 127) / 128;
     // with one workgroup to a unit its rounding, products and stores follow one another: two, of half the columns each, overlap
     // (32768 x 256 -> 768 25 us with one share, 22 with two); with more, rounding twice costs more (65536 x 384 -> 384 25 / 36)
-    a.shares = mtiles < 2 * f8_cus() && a.N >= 256 ? 2 : 1;
+    a.shares = a.K <= 4 * F8_BLOCK && mtiles < 2 * f8_cus() && a.N >= 256 ? 2 : 1;
     MAD_REQUIRE(mtiles <= 0x7fffffffL, "mad_linear_fp8: %ld rows need more workgroups than a launch holds", a.M);
     const dim3 grid((unsigned)(mtiles * a.shares));
+#define ROWS(KB, NW) case KB: hipLaunchKernelGGL((linear_fp8_rows_kernel<KB, NW>), grid, dim3(64 * NW), 0, s, a); break
     switch (f8_blocks(a.K)) {
-        case 1: hipLaunchKernelGGL(linear_fp8_rows_kernel<1>, grid, dim3(256), 0, s, a); break;
-        case 2: hipLaunchKernelGGL(linear_fp8_rows_kernel<2>, grid, dim3(256), 0, s, a); break;
-        case 3: hipLaunchKernelGGL(linear_fp8_rows_kernel<3>, grid, dim3(256), 0, s, a); break;
-        default: hipLaunchKernelGGL(linear_fp8_rows_kernel<4>, grid, dim3(256), 0, s, a); break;
+        ROWS(1, 4); ROWS(2, 4); ROWS(3, 4); ROWS(4, 4); ROWS(5, 8); ROWS(6, 8); ROWS(7, 8); ROWS(8, 8); ROWS(9, 8);
     }
+#undef ROWS
     return check_launch("mad_linear_fp8");
 }
 

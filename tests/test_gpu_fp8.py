@@ -284,6 +284,10 @@ ROWS_FORM = [(33000, 64, 200), (32768, 128, 128), (32769, 136, 513), (40001, 256
              (33000, 512, 2056), (33000, 520, 64), (33000, 60, 64)]
 
 
+# ... of five to nine blocks, where a unit holds one workgroup
+ROWS_FORM += [(32768, 640, 72), (32700, 1152, 200), (65500, 776, 130), (32768, 1024, 2048), (65536, 904, 66), (32768, 1160, 64), (45000, 1152, 96)]
+
+
 @pytest.mark.parametrize("rows,k,n", ROWS_FORM)
 def test_one_launch_is_packing_and_product(dev, rows, k, n):
     """The rounded x, if wanted, and y are those of the two calls, bit for bit; rows that are not finite included."""
