@@ -464,10 +464,10 @@ __global__ __launch_bounds__(256) void wgrad_fp8_join_kernel(F8JoinArgs a) {
 
 // How a gradient is cut: the form, its tiles and the shares of the rows.  A step of 64 rows takes a workgroup about 1.5 us with tiles of
 // 128 x 128 (two workgroups to a unit), 1.9 with 128 x 384 and 1.85 with 256 x 256; a share more shortens the rows of each and
-// adds a partial sum to write and join.  The general form takes 1.7 us (bf16; 128 x 256 is no faster there) and 3.5 (fp32; 3.15 with 128 x
-// 256, one workgroup: 16384 x 2048 -> 2048 483 / 428 us, 65536 x 128 -> 384 48 / 53).  The shares that balance the two, or fill the units
-// once, and of the tiles the ones that come out shortest (us, 128 x 128 / 128 x 384 / 256 x 256: 65536 x 384 -> 1152 99 / 86 / 105, 16384 x 768 -> 2304
-// 91 / 77 / 77, 8192 x 4096 -> 4096 319 / 388 / 234, 32768 x 256 -> 768 33 / 38 / 40).
+// adds a partial sum to write and join.  The general form takes 1.7 us (bf16; 128 x 256 is no faster there) and 3.5 (fp32; 3.15 with
+// 128 x 256, one workgroup: 16384 x 2048 -> 2048 483 / 428 us, 65536 x 128 -> 384 48 / 53).  The shares that balance the two, or fill
+// the units once, and of the tiles the ones that come out shortest (us, 128 x 128 / 128 x 384 / 256 x 256: 65536 x 384 -> 1152
+// 99 / 86 / 105, 16384 x 768 -> 2304 91 / 77 / 77, 8192 x 4096 -> 4096 319 / 388 / 245, 32768 x 256 -> 768 33 / 38 / 40).
 enum F8WgradForm { WG_TILED, WG_BF16, WG_F32 };
 struct F8WgradPlan { int bn, bk, ntiles, ktiles, splits, turns; long per; double us; };
 
