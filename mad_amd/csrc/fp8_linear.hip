@@ -577,9 +577,11 @@ __global__ __launch_bounds__(64 * NW, 2) void linear_fp8_rows_kernel(F8RowArgs a
     const int first = share * per, end = first + per < strips ? first + per : strips;
     const int lr = lane >> 3, chunk = (lane & 7) ^ ((4 * wave + (lr >> 1)) & 7);
     const unsigned lds0 = lds_addr(xs), ex0 = lds_addr(extra);
-    auto load_strip = [&](int t, int buf) {        // a strip's groups of 8 rows, shared out to the waves block by block
+    // A strip's groups of 8 rows, shared out to the waves block by block.  Only strips that exist: the scalar offset b * 128 is kept
+    // below the buffer's size (a strip has a row at least), because the range check compares against size - scalar offset.
+    auto load_strip = [&](int t, int buf) {
         const int nrem = a.N - 64 * t < 64 ? a.N - 64 * t : 64;
-        const u32x4 wb = f8_buffer(a.w + (size_t)(64 * t) * pitch, t < end ? (unsigned)(nrem * pitch) : 0u);
+        const u32x4 wb = f8_buffer(a.w + (size_t)(64 * t) * pitch, (unsigned)(nrem * pitch));
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
             const unsigned off = b * F8_BLOCK + 16 * chunk < pitch ? (unsigned)((8 * wave + lr) * pitch + 16 * chunk) : F8_OUTSIDE;
@@ -588,9 +590,9 @@ __global__ __launch_bounds__(64 * NW, 2) void linear_fp8_rows_kernel(F8RowArgs a
                 buf_lds16(wb, off + j * 32 * pitch, b * F8_BLOCK, lds0 + buf * STRIP + b * 64 * F8_BLOCK + (4 * j + wave) * 1024);
         }
         // by LDS-DMA as well: the wait for an ordinary load would wait for the strip in front of it
-        const u32x4 bb = f8_buffer((const unsigned char*)(a.bias + 64 * t), a.bias && t < end ? (unsigned)(nrem * 4) : 0u);
+        const u32x4 bb = f8_buffer((const unsigned char*)(a.bias + 64 * t), a.bias ? (unsigned)(nrem * 4) : 0u);
         if (wave == 2) buf_lds4(bb, lane * 4, 0, ex0 + buf * 512);
-        if (wave == 3) buf_lds4(f8_buffer(a.ws + (size_t)(64 * t / F8_BLOCK) * sp, t < end ? 4u * SD : 0u), lane * 4, 0, ex0 + buf * 512 + 256);
+        if (wave == 3) buf_lds4(f8_buffer(a.ws + (size_t)(64 * t / F8_BLOCK) * sp, 4u * SD), lane * 4, 0, ex0 + buf * 512 + 256);
     };
     constexpr int STORES = MF * 2;
     __syncthreads();                               // every wave has its rows: the strips may take their place
@@ -600,7 +602,7 @@ __global__ __launch_bounds__(64 * NW, 2) void linear_fp8_rows_kernel(F8RowArgs a
         const int buf = (t - first) & 1;
         if (counted) dma_wait_upto<STORES>(); else dma_wait_all();         // the strip is older than the stores of the one before
         __syncthreads();
-        load_strip(t + 1, buf ^ 1);
+        if (t + 1 < end) load_strip(t + 1, buf ^ 1);
         unsigned wsc[SD];
 #pragma unroll
         for (int d = 0; d < SD; ++d) wsc[d] = __float_as_uint(extra[buf][1][d]);
@@ -681,7 +683,6 @@ __global__ __launch_bounds__(64 * NW, 2) void linear_fp8_rows_kernel(F8RowArgs a
                 }
         }
     }
-    dma_wait_all();                                // the copies of the strip behind the last
 }
 
 template <int XK, int XF, typename TO, int MF, int NF, int NW> static int launch_direct(F8LinArgs a, hipStream_t s) {

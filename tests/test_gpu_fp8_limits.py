@@ -1,0 +1,42 @@
+"""The 8-bit operators at the limits of their operands: ends of allocations, share and step borders, the largest and smallest sizes
+and values (GPU only).  Where operands are small whole numbers every product and sum is exact, so results are compared for equality;
+other tolerances are derived beside the tests."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+torch.set_grad_enabled(False)
+
+
+@pytest.fixture(scope="module")
+def dev():
+    return torch.device("cuda:0")
+
+
+def _at_the_end(t):
+    """A copy of t whose last byte is the last one of an allocation of its own (whole 2 MiB pages, far above what a pool shares)."""
+    n = t.numel() * t.element_size()
+    page = 2 << 20
+    buf = torch.empty(max(16 << 20, -(-n // page) * page), dtype=torch.uint8, device=t.device)
+    view = buf[buf.numel() - n:].view(t.dtype).view(t.shape)
+    view.copy_(t)
+    return view
+
+
+# rows, K, N: one to nine blocks, one share of the columns and two, last strips that are whole and that are not
+@pytest.mark.parametrize("rows,k,n", [(32768, 64, 64), (33000, 136, 200), (40001, 256, 768), (33000, 512, 2048), (32768, 1152, 200)])
+def test_rounding_product_with_weights_at_the_end_of_memory(dev, rows, k, n):
+    """A long bf16 input is rounded inside the product, which copies the weights ahead in strips of 64 rows: nothing is asked for
+    behind the last one, and y is that of weights that lie elsewhere."""
+    from mad_amd import ops
+    g = torch.Generator(device=dev).manual_seed(k)
+    rand = lambda *s: torch.randn(s, generator=g, device=dev)
+    x = rand(rows, k).to(torch.bfloat16)
+    w, bias = ops.pack_weight_fp8(rand(n, k) / math.sqrt(k)), rand(n)
+    q = _at_the_end(w.q.view(torch.uint8)).view(w.q.dtype)
+    edge = w._replace(q=q, scale=_at_the_end(w.scale))
+    want = ops.linear_fp8(ops.pack_fp8(x), w, bias=bias)
+    assert torch.equal(ops.linear_fp8(x, edge, bias=_at_the_end(bias)), want)
+    assert torch.equal(ops.linear_fp8(x, edge, bias=bias, save=True)[0], want)
