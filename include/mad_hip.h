@@ -458,7 +458,7 @@ int mad_unpack_fp8(const void* q, const void* scale, int fmt, long rows, int C, 
 
 /* mad_gn_apply / mad_gn_apply_dropout of one source without pooling, y = drop(act(x*a + d)) over x (B, HW, C), that also
  * packs x (MAD_E4M3) in the same pass: the checkpoint the backward restores x and y from.  Same y, bit for bit.  C a multiple
- * of 8 (bf16) / 4 (fp32); x, y and coef 16-byte aligned.
+ * of 8 (bf16) / 4 (fp32); x, y and coef 16-byte aligned; B at most 65535.
  * Restore: x = what q and scale stand for, in `dtype`, and y computed from that x. */
 int mad_gn_apply_save_fp8(const void* x, const float* coef, void* y, void* q, void* scale, int dtype, int B, int HW,
                           int C, int act, unsigned long long seed, float p, void* stream);

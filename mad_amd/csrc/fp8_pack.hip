@@ -105,8 +105,9 @@ __global__ __launch_bounds__(256) void gn_fp8_kernel(T* __restrict__ x, const fl
     const int kb = f8_blocks(C), pitch = f8_pitch(C), sp = f8_scale_pitch(C);
     const int l = threadIdx.x & 15, grp = threadIdx.x >> 4;
     const int b = blockIdx.y;
-    const int per = (HW + gridDim.x - 1) / gridDim.x;
-    const int p0 = blockIdx.x * per, p1 = p0 + per < HW ? p0 + per : HW;
+    // unsigned: a share that starts or ends behind the last pixel of the largest image (2^31 - 1 of them) does not fit an int
+    const unsigned n = HW, per = (n + gridDim.x - 1) / gridDim.x;
+    const unsigned p0 = blockIdx.x * per, p1 = p0 + per < n ? p0 + per : n;
     const int step = kb >= 16 ? 1 : 16 / kb;                  // pixels a workgroup covers per sweep
     for (int kbase = 0; kbase < kb; kbase += 16) {
         const int k = kbase + (kb >= 16 ? grp : grp % kb);
@@ -126,7 +127,7 @@ __global__ __launch_bounds__(256) void gn_fp8_kernel(T* __restrict__ x, const fl
                     a[i] = v.x; d[i] = v.y; a[i + 1] = v.z; d[i + 1] = v.w;
                 }
         }
-        for (int p = p0 + row0; p < p1; p += step) {
+        for (unsigned p = p0 + row0; p < p1; p += step) {
             const size_t row = (size_t)b * HW + p;
             float f[8];
 #pragma unroll
@@ -329,9 +330,11 @@ static int gn_fp8(const char* what, void* x, const float* coef, void* y, void* q
     // pixel shares: eight sweeps of pixels to a workgroup, or as few as keep 4096 workgroups (32 x 128 x 128 x 256, save / restore, us:
     // 134 / 108 with 2048 workgroups, 120 / 101 with 8192; 32 x 64 x 64 x 256 29 / 28 with 4096, 34 / 29 with 8192)
     const int kb = f8_blocks(C), step = kb >= 16 ? 1 : 16 / kb;
-    const long sweeps = (long)B * ((HW + step - 1) / step);
+    const long sweeps = (long)B * (((long)HW + step - 1) / step);
     int shares = (int)(((sweeps / 8 > 4096 ? sweeps / 8 : 4096) + B - 1) / B);
-    if (shares > (HW + step - 1) / step) shares = (HW + step - 1) / step;
+    const int most = HW / step + (HW % step != 0);
+    if (shares > most) shares = most;
+    if (shares > 1 << 22) shares = 1 << 22;                                 // a launch counts fewer than 2^32 threads
     const DropMask dm = make_drop_mask(seed, p);
     if (dtype == MAD_BF16)
         hipLaunchKernelGGL((gn_fp8_kernel<bf16_t, SAVE>), dim3(shares, B), dim3(256), 0, (hipStream_t)stream, (bf16_t*)x, coef,

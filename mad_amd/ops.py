@@ -903,6 +903,8 @@ def unpack_fp8(p: Fp8Tensor) -> Tensor:
 def _coef_check(coef: Tensor, shape: Sequence[int], what: str) -> None:
     if len(shape) != 4:
         raise ValueError(f"{what}: needs an NHWC tensor, got shape {tuple(shape)}")
+    if shape[0] > 65535 or shape[1] * shape[2] > 0x7fffffff:              # HW is an int of the entry point
+        raise ValueError(f"{what}: at most 65535 images of 2^31 - 1 pixels, got shape {tuple(shape)}")
     if coef.dtype != torch.float32 or coef.shape != (shape[0], shape[3], 2):
         raise ValueError(f"{what}: coef must be fp32 ({shape[0]}, {shape[3]}, 2), got {coef.dtype} {tuple(coef.shape)}")
 

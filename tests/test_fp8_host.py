@@ -216,3 +216,19 @@ def test_types_agree_with_the_header():
     a, b = re.search(r"#define MAD_FP8_MAX_WIDTH \((\d+) << (\d+)\)", h).groups()
     assert int(a) << int(b) == _lib.FP8_MAX_WIDTH
     assert ctypes.sizeof(ctypes.c_long) == 8
+
+
+# ------------------------------------------------------------------ sizes that an int does not hold
+@pytest.mark.parametrize("shape", [(1, 1 << 16, 1 << 16, 8), (1, 1 << 16, 1 << 15, 8), (1, (1 << 16) + 1, 1 << 16, 8), (65536, 1, 1, 8)])
+def test_norm_refuses_sizes_beyond_the_entry_point(shape, monkeypatch):
+    """H * W of 2^32 arrived at the C entry point as 0: it reported success and wrote nothing."""
+    from mad_amd import _lib, ops
+    monkeypatch.setattr(ops, "_fp8_dev", lambda *t: 0)
+    monkeypatch.setattr(ops, "_fp8_call", lambda *a: pytest.fail("called"))
+    empty = lambda s, dt: torch.empty(s, dtype=dt, device="meta")
+    coef, rows = empty((shape[0], 8, 2), torch.float32), shape[0] * shape[1] * shape[2]
+    with pytest.raises(ValueError, match="at most 65535 images"):
+        ops.gn_apply_save(empty(shape, torch.bfloat16), coef, act=True)
+    p = ops.Fp8Tensor(empty((rows, 16), torch.float8_e4m3fn), empty((rows, 4), torch.uint8), shape, torch.bfloat16)
+    with pytest.raises(ValueError, match="at most 65535 images"):
+        ops.gn_apply_restore(p, coef, act=True)

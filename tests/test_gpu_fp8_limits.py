@@ -40,3 +40,29 @@ def test_rounding_product_with_weights_at_the_end_of_memory(dev, rows, k, n):
     want = ops.linear_fp8(ops.pack_fp8(x), w, bias=bias)
     assert torch.equal(ops.linear_fp8(x, edge, bias=_at_the_end(bias)), want)
     assert torch.equal(ops.linear_fp8(x, edge, bias=bias, save=True)[0], want)
+
+
+def test_norm_of_the_largest_image(dev):
+    """2^31 - 1 pixels, the most that the entry point counts: the shares of the last workgroups end behind them."""
+    from mad_amd import ops
+    c, n, m = 8, (1 << 31) - 1, 1000
+    torch.cuda.empty_cache()
+    g = torch.Generator(device=dev).manual_seed(1)
+    ends = [torch.randn((m, c), generator=g, device=dev).to(torch.bfloat16) for _ in range(2)]
+    coef = torch.randn((1, c, 2), generator=g, device=dev)
+    x = torch.zeros((1, n, 1, c), dtype=torch.bfloat16, device=dev)
+    x[0, :m, 0], x[0, -m:, 0] = ends
+    at = lambda t, i: (t[:m], t[-m:])[i]
+    y, p = ops.gn_apply_save(x, coef, act=True)
+    for i, e in enumerate(ends):
+        want, small = ops.gn_apply_save(e.view(1, m, 1, c), coef, act=True)
+        assert torch.equal(at(y[0], i), want[0])
+        assert torch.equal(at(p.q, i).view(torch.uint8), small.q.view(torch.uint8)) and torch.equal(at(p.scale, i), small.scale)
+    del x, y
+    torch.cuda.empty_cache()
+    xr, yr = ops.gn_apply_restore(p, coef, act=True)
+    for i, e in enumerate(ends):
+        x2, y2 = ops.gn_apply_restore(ops.pack_fp8(e.view(1, m, 1, c)), coef, act=True)
+        assert torch.equal(at(xr[0], i), x2[0]) and torch.equal(at(yr[0], i), y2[0])
+    del xr, yr, p
+    torch.cuda.empty_cache()
