@@ -312,11 +312,18 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
     const int first = xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8;
     const int last = first + q8 + (xcd < r8 ? 1 : 0);
 
-    // lane of a copy: row lane/8 of its 8 rows, and the chunk that belongs at position lane%8 of that row
-    const int lr = lane >> 3, chunk = (lane & 7) ^ ((4 * wave + (lr >> 1)) & 7);
-    const unsigned off0 = (unsigned)((8 * wave + lr) * pitch + 16 * chunk), rowstep = (unsigned)(8 * CW * pitch);
-    const int tail = pitch - 16 * chunk;             // step offsets below it have this lane's chunk inside the row
     const unsigned lds0 = lds_addr(smem);
+    // In large tiles the products of widened operands (fp32 results) leave no registers for what copies and stores derive from the
+    // lane: kept over the products it was spilled, and a reload waits for every copy before it.  There it is made anew, from a lane
+    // number that the compiler knows nothing of, and a residual is loaded one row fragment at a time (us, before / after: 65536 x 128
+    // -> 1024 76 / 56, with a residual 16384 x 4096 -> 8192 1171 / 1089, 32768 x 1024 -> 1024 142 / 110; small tiles, which have the
+    // registers, lose 2 % by it).
+    constexpr bool CROWDED = sizeof(TO) == 4 && BM > 128;
+    auto fresh_lane = [&]() {
+        int l = lane;
+        if constexpr (CROWDED) asm volatile("" : "+v"(l));
+        return l;
+    };
 
     struct Tile { long m0; int n0; u32x4 x, w, xs, ws; };
     auto open = [&](int t) {
@@ -335,7 +342,10 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
     };
     // step kt of a tile into a stage, panel p of its scales into a slot
     auto stage = [&](const Tile& t, int kt, int buf) {
-        const unsigned off = kt * F8_BLOCK < tail ? off0 : F8_OUTSIDE, dst = lds0 + buf * L::STAGE + wave * 1024;
+        // lane of a copy: row l/8 of its 8 rows, and the chunk that belongs at position l%8 of that row, if the row reaches that far
+        const int l = fresh_lane(), lr = l >> 3, chunk = (l & 7) ^ ((4 * wave + (lr >> 1)) & 7);
+        const unsigned off = kt * F8_BLOCK + 16 * chunk < pitch ? (unsigned)((8 * wave + lr) * pitch + 16 * chunk) : F8_OUTSIDE;
+        const unsigned rowstep = (unsigned)(8 * CW * pitch), dst = lds0 + buf * L::STAGE + wave * 1024;
 #pragma unroll
         for (int j = 0; j < XPW; ++j) buf_lds16(t.x, off + j * rowstep, kt * F8_BLOCK, dst + j * CW * 1024);
 #pragma unroll
@@ -343,8 +353,9 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
     };
     auto panel = [&](const Tile& t, int p, int slot) {
         const unsigned dst = lds0 + 2 * L::STAGE + slot * L::PANEL;
-        if (64 * wave < BM) buf_lds4(t.xs, (unsigned)((64 * wave + lane) * sp), 4 * p, dst + wave * 256);
-        if (wave == NW - 1) buf_lds4(t.ws, (unsigned)(lane * sp), 4 * p, dst + BM * 4);
+        const int l = fresh_lane();
+        if (64 * wave < BM) buf_lds4(t.xs, (unsigned)((64 * wave + l) * sp), 4 * p, dst + wave * 256);
+        if (wave == NW - 1) buf_lds4(t.ws, (unsigned)(l * sp), 4 * p, dst + BM * 4);
     };
 
     int t = first + (blockIdx.x >> 3);
@@ -406,7 +417,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
             buf ^= 1;
         }
 
-        const int nb = cur.n0 + wn * (BN / WN) + (g & 1) * 16 + (g >> 1) * 8;     // this lane's first column, pair 0
+        const int el = fresh_lane(), nb = cur.n0 + wn * (BN / WN) + (el >> 4 & 1) * 16 + (el >> 5) * 8;     // this lane's first column, pair 0
         float bias[NF / 2][8];
 #pragma unroll
         for (int p = 0; p < NF / 2; ++p) {
@@ -428,7 +439,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
         // G row fragments at a time before their stores (a load behind a store waits for it: they complete in order).
         counted = cur.m0 + BM <= a.M && cur.n0 + BN <= a.N;
         if (counted) {
-            constexpr int G = sizeof(TO) == 2 ? 4 : 2;                        // row fragments at a time: what registers hold
+            constexpr int G = sizeof(TO) == 2 ? 4 : CROWDED ? 1 : 2;          // row fragments at a time: what registers hold
 #pragma unroll
             for (int i0 = 0; i0 < MF; i0 += G) {
                 Piece8<TO> res[G][NF / 2];
@@ -713,7 +724,8 @@ template <int XF, typename TO, int BM, int BN, int WM, int WN> static int launch
 // Which form.  The units work in rounds of one tile of 256 x 256, or two of 128 x 128, each: the form whose rounds cover less area
 // takes less time, where a round of small tiles counts 1.18 of its area from K = 1024 on (16384 x 4096 -> 4096 240 us with
 // large tiles, 274 with small; 4096 x 4096 -> 1024 52 / 26) and nothing extra below (65536 x 384 -> 1152 51 / 47,
-// 16384 x 256 -> 4096 37 / 37).  With fewer than one small tile for each unit the direct form is as fast or faster
+// 16384 x 256 -> 4096 37 / 37).  fp32 results, large / small: 8192 x 4096 -> 4096 239 / 271, 12288 x 2048 -> 6144 315 / 326,
+// 65536 x 1152 -> 384 79 / 70, 65536 x 384 -> 1152 101 / 98, 16384 x 256 -> 4096 77 / 70.  With fewer than one small tile for each unit the direct form is as fast or faster
 // (1024 x 4096 -> 1024 23 / 24, 64 x 256 -> 4096 3.5 / 5.7; fp32 777 x 1000 -> 328 7 / 15).
 template <int XK, int XF, typename TO> static int launch_linear(F8LinArgs a, hipStream_t s) {
     if constexpr (XK < X_BF16) {

@@ -232,3 +232,39 @@ def test_norm_refuses_sizes_beyond_the_entry_point(shape, monkeypatch):
     p = ops.Fp8Tensor(empty((rows, 16), torch.float8_e4m3fn), empty((rows, 4), torch.uint8), shape, torch.bfloat16)
     with pytest.raises(ValueError, match="at most 65535 images"):
         ops.gn_apply_restore(p, coef, act=True)
+
+
+# ------------------------------------------------------------------ the built kernels
+def _kernels():
+    """Name -> metadata of every kernel in the built library (the notes of its gfx950 code objects)."""
+    import struct
+    from mad_amd import _lib
+    msgpack = pytest.importorskip("msgpack")
+    blob, magic, out = open(_lib.LIB_PATH, "rb").read(), b"__CLANG_OFFLOAD_BUNDLE__", {}
+    at = blob.find(magic)
+    while at >= 0:
+        entry = at + 32
+        for _ in range(struct.unpack_from("<Q", blob, at + 24)[0]):
+            offset, size, n = struct.unpack_from("<QQQ", blob, entry)
+            target, entry = blob[entry + 24:entry + 24 + n], entry + 24 + n
+            if b"gfx" not in target:
+                continue
+            elf = blob[at + offset:at + offset + size]
+            table, (step, count) = struct.unpack_from("<Q", elf, 0x28)[0], struct.unpack_from("<HH", elf, 0x3a)
+            for h in range(table, table + step * count, step):
+                if struct.unpack_from("<I", elf, h + 4)[0] != 7:                 # SHT_NOTE
+                    continue
+                note = struct.unpack_from("<Q", elf, h + 0x18)[0]
+                name, desc, _ = struct.unpack_from("<III", elf, note)
+                start = note + 12 + ((name + 3) & ~3)
+                for k in msgpack.unpackb(elf[start:start + desc])["amdhsa.kernels"]:
+                    out[k[".name"]] = k
+        at = blob.find(magic, at + 24)
+    return out
+
+
+def test_kernels_keep_their_registers():
+    """None of them spills: a reload from scratch memory waits for every copy in flight."""
+    found = {n: k[".private_segment_fixed_size"] for n, k in _kernels().items() if "fp8" in n}
+    assert len(found) > 50
+    assert not {n: v for n, v in found.items() if v}
