@@ -696,10 +696,12 @@ __global__ __launch_bounds__(64 * NW, 2) void linear_fp8_rows_kernel(F8RowArgs a
     }
 }
 
+constexpr long LAUNCH_THREADS = 0xffffffffL;       // a launch counts fewer than 2^32 threads
+
 template <int XK, int XF, typename TO, int MF, int NF, int NW> static int launch_direct(F8LinArgs a, hipStream_t s) {
     const long mtiles = (a.M + 16 * MF - 1) / (16 * MF);
     a.ntiles = (a.N + 16 * NF - 1) / (16 * NF);
-    MAD_REQUIRE(mtiles * a.ntiles <= 0x7fffffffL, "mad_linear_fp8: %ld rows x %d columns need more workgroups than a launch holds",
+    MAD_REQUIRE(mtiles * a.ntiles <= LAUNCH_THREADS / (64 * NW), "mad_linear_fp8: %ld rows x %d columns need more workgroups than a launch holds",
                 a.M, a.N);
     hipLaunchKernelGGL((linear_fp8_direct_kernel<XK, XF, TO, MF, NF, NW>), dim3((unsigned)(mtiles * a.ntiles)), dim3(64 * NW), 0, s, a);
     return check_launch("mad_linear_fp8");
@@ -760,7 +762,7 @@ template <int XK, int XF, typename TO> static int launch_linear(F8LinArgs a, hip
 // (40000 x 640 -> 640 43 / 44, 40000 x 1152 -> 384 54 / 54).
 static bool rows_form_ok(const void* x, int dtype, long rows, int K, int N) {
     const long tiles = (rows + 127) / 128, cus = f8_cus();
-    return dtype == MAD_BF16 && whole_pieces(x, dtype, K) && K <= 9 * F8_BLOCK && N <= 2048 && tiles >= cus &&
+    return dtype == MAD_BF16 && whole_pieces(x, dtype, K) && K <= 9 * F8_BLOCK && N <= 2048 && tiles >= cus && tiles <= LAUNCH_THREADS / 512 &&
            (K <= 4 * F8_BLOCK || 4 * tiles >= 3 * ((tiles + cus - 1) / cus) * cus);
 }
 
@@ -778,7 +780,6 @@ static int launch_rows(F8RowArgs a, hipStream_t s) {
     // with one workgroup to a unit its rounding, products and stores follow one another: two, of half the columns each, overlap
     // (32768 x 256 -> 768 25 us with one share, 22 with two); with more, rounding twice costs more (65536 x 384 -> 384 25 / 36)
     a.shares = a.K <= 4 * F8_BLOCK && mtiles < 2 * f8_cus() && a.N >= 256 ? 2 : 1;
-    MAD_REQUIRE(mtiles <= 0x7fffffffL, "mad_linear_fp8: %ld rows need more workgroups than a launch holds", a.M);
     const dim3 grid((unsigned)(mtiles * a.shares));
 #define ROWS(KB, NW) case KB: hipLaunchKernelGGL((linear_fp8_rows_kernel<KB, NW>), grid, dim3(64 * NW), 0, s, a); break
     switch (f8_blocks(a.K)) {

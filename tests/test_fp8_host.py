@@ -268,3 +268,12 @@ def test_kernels_keep_their_registers():
     found = {n: k[".private_segment_fixed_size"] for n, k in _kernels().items() if "fp8" in n}
     assert len(found) > 50
     assert not {n: v for n, v in found.items() if v}
+
+
+def test_launches_stay_below_the_threads_they_count():
+    """A launch counts fewer than 2^32 threads: longer inputs are packed first, or refused."""
+    lib, L = _lib()
+    assert lib.mad_linear_fp8_needs_pack(P, L.MAD_BF16, (1 << 30) - 128, 8, 8) == 0
+    assert lib.mad_linear_fp8_needs_pack(P, L.MAD_BF16, 1 << 30, 8, 8) == 1
+    _refused(lib.mad_linear_fp8(P, L.MAD_BF16, None, P, P, None, None, P, L.MAD_BF16, 1 << 28, 5, 16, None), "need more")
+    _refused(lib.mad_linear_fp8(P, L.MAD_F32, None, P, P, None, None, P, L.MAD_F32, 1 << 20, 8, 1 << 15, None), "need more")

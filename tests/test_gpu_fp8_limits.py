@@ -66,3 +66,22 @@ def test_norm_of_the_largest_image(dev):
         assert torch.equal(at(xr[0], i), x2[0]) and torch.equal(at(yr[0], i), y2[0])
     del xr, yr, p
     torch.cuda.empty_cache()
+
+
+def test_product_of_more_rows_than_one_launch_rounds(dev):
+    """2^31 rows and some: the form that rounds 128 rows to a workgroup would count more threads than a launch holds."""
+    from mad_amd import ops
+    k, n, m = 8, 8, 1000
+    torch.cuda.empty_cache()
+    g = torch.Generator(device=dev).manual_seed(2)
+    tail = torch.randn((m, k), generator=g, device=dev).to(torch.bfloat16)
+    w = ops.pack_weight_fp8(torch.randn((n, k), generator=g, device=dev))
+    x = torch.zeros(((1 << 31) + m, k), dtype=torch.bfloat16, device=dev)
+    x[-m:] = tail
+    y, x8 = ops.linear_fp8(x, w, save=True)
+    del x
+    small, t8 = ops.linear_fp8(tail, w, save=True)
+    assert torch.equal(x8.q[-m:].view(torch.uint8), t8.q.view(torch.uint8)) and torch.equal(x8.scale[-m:], t8.scale)
+    assert torch.equal(y[-m:], small) and not bool(y[:m].any())
+    del y, x8
+    torch.cuda.empty_cache()
