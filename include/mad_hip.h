@@ -487,8 +487,9 @@ int mad_linear_fp8_save(const void* x, int dtype, int fmt, const void* w, const 
                         const void* residual, void* y, void* q, void* scale, long rows, int K, int N, void* stream);
 
 /* dw (N, K) (+)= dy^T . x and db (N) (+)= column sums of dy (db may be NULL), fp32; x packed (rows, K), dy (rows, N) in
- * `dtype`, unrounded; x to bf16's smallest step, 2^-133.  Partial sums are added in a fixed order (deterministic).  The data
- * gradient is mad_linear_fp8 of the packed dy and the transposed weight. */
+ * `dtype`.  Both operands enter as they are down to bf16's smallest step, 2^-133: x is rounded to a multiple of it, an fp32 dy cut
+ * toward zero to one (what lies below is lost to elements under 2^-109).  Partial sums are added in a fixed order (deterministic).
+ * The data gradient is mad_linear_fp8 of the packed dy and the transposed weight. */
 size_t mad_linear_fp8_wgrad_workspace(long rows, int N, int K);
 int mad_linear_fp8_wgrad(const void* dy, int dtype, const void* x, int x_type, const void* x_scale, float* dw, float* db,
                          void* workspace, size_t workspace_bytes, long rows, int N, int K, int accumulate,

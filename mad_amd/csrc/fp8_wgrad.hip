@@ -4,8 +4,8 @@
 //
 // The scale of x changes along the reduction (one per row m), so the product cannot run on 8-bit operands; but bf16 holds
 // every restored value exactly (to 2^-133, its smallest step), so x is widened on its way into LDS and the product runs on
-// v_mfma_f32_16x16x32_bf16 without a further rounding.  dy is bf16, or fp32 cut into three bf16 terms whose sum is dy (x is
-// exact, so three products give fp32 accuracy).  Both operands are stored with the reduction index slow and read with the
+// v_mfma_f32_16x16x32_bf16 without a further rounding.  dy is bf16, or fp32 cut into three bf16 terms whose sum is dy down
+// to 2^-133 too, i.e. all 24 bits from 2^-109 on (x is exact, so three products give fp32 accuracy).  Both operands are stored with the reduction index slow and read with the
 // transposing LDS read (ds_read_b64_tr_b16: a row of 16 lanes fetches 4 rows m x 16 columns, lane i receives column i).
 // Shares of the rows write partial sums that a second kernel adds in share order: the result does not depend on timing.
 //

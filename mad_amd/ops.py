@@ -1020,7 +1020,7 @@ def linear_fp8_backward(dy: Tensor, x: Fp8Tensor, w: Optional[Fp8Weight] = None,
     """Gradients of ``linear_fp8`` from dy (..., N) and the saved packed input: (dx, dw, dbias).
 
     dx = Q(dy) . w with dy rounded to ``grad_fmt`` by rows as ``pack_fp8`` does (``w`` packed with its transposed copy);
-    dw = dy^T . x and dbias = column sums of dy in fp32 from the unrounded dy.  ``dw`` / ``dbias`` may be given (fp32, N*K and N
+    dw = dy^T . x and dbias = column sums of dy in fp32 from dy as it is (fp32: cut to multiples of 2^-133).  ``dw`` / ``dbias`` may be given (fp32, N*K and N
     elements) and are then overwritten or, with ``accumulate``, added to."""
     rows, K, fmt = _fp8_check(x, "linear_fp8_backward")
     i = _fp8_dev(dy, x.q, dw, dbias)

@@ -85,3 +85,22 @@ def test_product_of_more_rows_than_one_launch_rounds(dev):
     assert torch.equal(y[-m:], small) and not bool(y[:m].any())
     del y, x8
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("n", [64, 61])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_gradients_near_the_smallest_numbers(dev, dt, n):
+    """dy of 2^-136 to 2^-117.  bf16 enters the products as it is, fp32 in three bf16 terms cut toward zero to multiples of 2^-133.  The
+    sums are whole numbers of the last place below 2^24 (300 * 2^12 * 8), so they are exact: dw and db are those of the cut dy."""
+    from mad_amd import ops
+    rows, k = 300, 96
+    g = torch.Generator().manual_seed(n)
+    x = torch.randint(-8, 9, (rows, k), generator=g).float() * 2.0 ** 60
+    x8 = ops.pack_fp8(x.to(dt).to(dev))
+    whole = torch.randint(1, 1 << 12, (rows, n), generator=g) * (2 * torch.randint(0, 2, (rows, n), generator=g) - 1)
+    for e in (-136, -129):                                    # -129: nothing lies below 2^-133
+        dy = (whole.double() * 2.0 ** e).float().to(dt)
+        _, dw, db = ops.linear_fp8_backward(dy.to(dev), x8, need_dx=False)
+        d = torch.trunc(dy.double() * 2.0 ** 133) * 2.0 ** -133
+        assert torch.equal(d, dy.double()) == (e == -129 or dt == torch.bfloat16)
+        assert torch.equal(dw.double().cpu(), d.t() @ x.double()) and torch.equal(db.double().cpu(), d.sum(0))
