@@ -104,3 +104,73 @@ def test_gradients_near_the_smallest_numbers(dev, dt, n):
         d = torch.trunc(dy.double() * 2.0 ** 133) * 2.0 ** -133
         assert torch.equal(d, dy.double()) == (e == -129 or dt == torch.bfloat16)
         assert torch.equal(dw.double().cpu(), d.t() @ x.double()) and torch.equal(db.double().cpu(), d.sum(0))
+
+
+# rows, K, N of many shares, tiles of every size and ragged ends; one row, one step, one share and a row more
+WGRAD = [(66000, 272, 136), (333, 4000, 4104), (20001, 384, 1152), (5000, 16, 8), (3000, 1040, 131), (64, 4096, 4096), (129, 130, 264),
+         (30000, 768, 2304), (9000, 640, 520), (2000, 1152, 1536), (40000, 200, 1152), (5000, 4096, 4112), (4001, 4100, 4095),
+         (1, 40, 24), (63, 384, 384), (65, 200, 520), (16384, 2048, 2048), (65536, 128, 384)]
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,k,n", WGRAD)
+def test_weight_gradient_of_whole_numbers(dev, rows, k, n, dt):
+    """Every sum is a whole number below 2^24 whatever the order of its additions, so dw and db are equal bit for bit in every form:
+    a row, a step or a share that is lost, counted twice or scaled by its neighbour's scale shows.
+    First in every row: |dy| <= 3, |x| <= 3 * 2^s with s = 0..3 by rows, at most 72 * 66000.  Then, in three rows of each column of dy,
+    numbers of 22 bits (in fp32 all three terms of the split) against |x| <= 1: at most 3 * 2^22."""
+    from mad_amd import ops
+    g = torch.Generator(device=dev).manual_seed(rows + k + n)
+    ints = lambda lo, hi, *s: torch.randint(lo, hi + 1, s, generator=g, device=dev)
+    fmt = "e5m2" if rows % 2 else "e4m3"
+    sparse = torch.zeros((rows, n), dtype=torch.int64, device=dev)
+    for _ in range(min(3, rows)):
+        sparse.scatter_(0, ints(0, rows - 1, 1, n), (2 * ints(0, (1 << 21) - 1, 1, n) + 1) * (2 * ints(0, 1, 1, n) - 1))
+    size = 2.0 ** ints(0, 3, rows, 1).double()
+    if dt == torch.bfloat16:
+        sparse = sparse.clamp(-255, 255)                      # what eight bits hold
+    for x, dy in ((ints(-3, 3, rows, k).double() * size, ints(-3, 3, rows, n)), (ints(-1, 1, rows, k).double(), sparse)):
+        x8, dy = ops.pack_fp8(x.to(dt), fmt), dy.to(dt)
+        want, want_b = dy.double().t() @ x, dy.double().sum(0)
+        off = torch.cat([dy.flatten()[:1], dy.flatten()])[1:].view(rows, n)             # rows that start anywhere
+        for d in (dy, off):
+            _, dw, db = ops.linear_fp8_backward(d, x8, need_dx=False)
+            assert torch.equal(dw.double(), want) and torch.equal(db.double(), want_b)
+            dw, db = torch.full((n + 1, k), 5.0, device=dev), torch.full((n + 1,), -3.0, device=dev)
+            ops.linear_fp8_backward(d, x8, need_dx=False, dw=dw[:n], dbias=db[:n], accumulate=True)
+            assert torch.equal(dw[:n].double(), want + 5) and torch.equal(db[:n].double(), want_b - 3)
+            assert bool((dw[n] == 5).all()) and float(db[n]) == -3
+
+
+# rows, K, N of every form of the product: direct with 16, 32 and 64 rows, tiles of 128 and 256, rounding inside by 16 and by 128 rows
+PRODUCT = [(1, 768, 768), (3, 4100, 40), (31, 1000, 130), (200, 640, 384), (1000, 384, 500), (2100, 130, 4100), (5000, 17, 2303), (4100, 272, 1000),
+           (16384, 2048, 2048), (20000, 1000, 3001), (65536, 128, 1024), (33000, 60, 64), (33000, 512, 2048), (33333, 384, 66), (32768, 1152, 200),
+           (45000, 776, 130)]
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,k,n", PRODUCT)
+def test_product_of_whole_numbers(dev, rows, k, n, dt):
+    """Products of at most 9, scaled by 2^0..3 by row and block and by 2^0..2 by block of the weight, sum to whole numbers below 2^24
+    (9 * 32 * 4100, with bias and residual), and no eight of them spans 2^13: y is the exact result rounded once, in every form, and so
+    is dx, for which y's operands change places."""
+    from mad_amd import ops
+    g = torch.Generator(device=dev).manual_seed(rows + k + n)
+    ints = lambda lo, hi, *s: torch.randint(lo, hi + 1, s, generator=g, device=dev)
+    each = lambda t, size, by: size.repeat_interleave(by, 1)[:, :t.shape[1]] * t
+    x = each(ints(-3, 3, rows, k).double(), 2.0 ** ints(0, 3, rows, -(-k // 128)).double(), 128)
+    w = ints(-3, 3, n, k).double()
+    w = each(w, (2.0 ** ints(0, 2, -(-n // 128), -(-k // 128)).double()).repeat_interleave(128, 0)[:n], 128)
+    bias, res, dy = ints(-9, 9, n), ints(-9, 9, rows, n), ints(-3, 3, rows, n)
+    pw = ops.pack_weight_fp8(w.float(), transposed=True)
+    want = x @ w.t()
+    full = (want + bias + res).float().to(dt)                 # fp32 holds the sums: one rounding
+    want = want.float().to(dt)
+    x8 = ops.pack_fp8(x.to(dt))
+    for a in (x.to(dt), x8, ops.pack_fp8(x.to(dt), "e5m2")):
+        assert torch.equal(ops.linear_fp8(a, pw), want)
+        y, _ = ops.linear_fp8(a, pw, bias=bias.float(), residual=res.to(dt), save=True)
+        assert torch.equal(y, full)
+    for fmt in ("e4m3", "e5m2"):
+        dx, _, _ = ops.linear_fp8_backward(dy.to(dt), x8, pw, grad_fmt=fmt)
+        assert torch.equal(dx, (dy.double() @ w).float().to(dt))
