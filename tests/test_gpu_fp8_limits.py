@@ -174,3 +174,23 @@ def test_product_of_whole_numbers(dev, rows, k, n, dt):
     for fmt in ("e4m3", "e5m2"):
         dx, _, _ = ops.linear_fp8_backward(dy.to(dt), x8, pw, grad_fmt=fmt)
         assert torch.equal(dx, (dy.double() @ w).float().to(dt))
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,c", [(1, 1), (9, 128), (7, 250), (33, 1001), (2, 2500), (16, 384)])
+def test_packed_bytes(dev, rows, c, dt, fmt):
+    """Every byte is the oracle's, padding included; only a NaN may be any of the type's NaNs, and a zero either zero."""
+    from mad_amd import ops
+    from oracle import fp8_ref as R
+    g = torch.Generator().manual_seed(rows + c)
+    x = (torch.randn((rows, c), generator=g) * torch.exp(4 * torch.randn((rows, c), generator=g))).to(dt)
+    x[0, c // 3], x[rows - 1, c - 1] = float("nan"), -float("inf")
+    q, s = R.stored(*R.pack_rows(x, fmt), fmt)
+    p = ops.pack_fp8(x.to(dev), fmt)
+    got = p.q.cpu().view(torch.uint8)
+    nan = torch.isnan(q.view(R.TYPE[fmt]).float())
+    assert torch.equal(torch.isnan(p.q.cpu().float()), nan)
+    plain = lambda t: torch.where(t == 0x80, 0, t)[~nan]
+    assert torch.equal(plain(got), plain(q)) and torch.equal(p.scale.cpu(), s)
+    assert got.shape == (rows, (c + 15) // 16 * 16) and not bool(got[:, c:].any())
