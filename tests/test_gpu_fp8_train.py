@@ -137,3 +137,64 @@ def test_products_and_checkpoints_together_are_deterministic(dev):
         loss = tr.forward_backward(x.to(dev), t.to(dev), lab.to(dev), target.to(dev))
         got.append((loss, tr.gflat.clone()))
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]) and bool(torch.isfinite(got[0][1]).all())
+
+
+def _disturb_tape(tr, tape):
+    """Every activation that 8-bit checkpoints round, times 1 + an independent uniform disturbance of at most 2^-4."""
+    from mad_amd import ops
+    g = torch.Generator(device=tape["h_last"].device).manual_seed(5)
+    seen = {}                                                 # a block's input may be the skip of another: disturbed once, as it is rounded once
+
+    def rt(t):
+        if t is not None and id(t) not in seen:
+            seen[id(t)] = (t, (t * (1 + 2.0 ** -4 * (2 * torch.rand(t.shape, generator=g, device=t.device) - 1))).to(t.dtype))
+        return None if t is None else seen[id(t)][1]
+    for e, sv in zip(tape["P"]["blocks"], tape["saved"]):
+        sv.x, sv.skip, sv.h = rt(sv.x), rt(sv.skip), rt(sv.h)
+        sv.h0 = ops.gn_apply(sv.x, sv.c0, act=True, x2=sv.skip, pool=e["spec"].down)
+        sv.h1 = ops.gn_apply(sv.h, sv.c1, act=True, drop_seed=sv.seed or 0, drop_p=tr.dropout if sv.seed is not None else 0.0)
+        if e["spec"].attention:
+            sv.y = rt(sv.y)
+            sv.hn = ops.gn_apply(sv.y, sv.c2, act=False)
+    tape["h_last"] = rt(tape["h_last"])
+    tape["hact"] = ops.gn_apply(tape["h_last"], tape["c_out"], act=True)
+
+
+@pytest.mark.parametrize("precision", ["bf16", "fp32"])
+@pytest.mark.parametrize("cfg_file", ["model_tiny.yaml", "model_tiny64.yaml"])
+@pytest.mark.parametrize("checkpoints,products", [("fp8", None), (None, "fp8"), ("fp8", "fp8")])
+def test_gradients_stay_close_to_the_ordinary_ones(dev, cfg_file, checkpoints, products, precision):
+    """The gradients of a step with 8-bit checkpoints, products or both against those of the same step without, block by block.
+
+    Checkpoints: rounding to three fraction bits is off by at most 2^-4 of the element, evenly spread below that.  A uniform disturbance
+    of at most 2^-4 of every such element is at least as large in the mean square, and to first order both reach the gradients the
+    same way: so the gradients are off by no more than with that disturbance, times 1.5 for the spread of two random draws.
+    Products: a rounded operand is off by r = 2^-4 / sqrt(3) of its size in the mean square, and so is its product.  An attention
+    block has four operands forward (two of them weights) and four backward; q, k, v and the softmax pass a disturbance on by at most
+    its size (scores of about one), and the blocks' residual carries what does not go through them: r * sqrt(8 * blocks) in all."""
+    from mad_amd import ops
+    from mad_amd.train import UNetTrainer
+    runs = []
+    for disturb, options in ((False, {}), (True, {}), (False, {"checkpoints": checkpoints, "products": products})):
+        _, m, _, x, t, lab, target = _setup(cfg_file, precision, dev, B=3)
+        tr = UNetTrainer(m.unet, dropout=0.1, **options)
+        tr._drop_calls = 0
+        pred, tape = tr.forward(x.to(dev), t.to(dev), lab.to(dev))
+        loss, dpred = ops.mse_loss_grad(pred, target.to(dev))
+        if disturb:
+            _disturb_tape(tr, tape)
+        tr.backward(tape, dpred)
+        runs.append((pred.double(), {k: v.double().flatten() for k, v in tr.grads.items()}))
+    blocks = [e["spec"] for e in tape["P"]["blocks"]]
+    attentions = sum(b.attention for b in blocks)
+    r = 2.0 ** -4 / 3 ** 0.5
+    off = lambda a, b: float((a - b).norm() / b.norm())
+    (pred0, want), (_, disturbed), (pred, got) = runs
+    if products:
+        assert 0 < off(pred, pred0) <= r * (4 * attentions) ** 0.5
+    else:
+        assert torch.equal(pred, pred0)
+    for name in [b.name + "." for b in blocks] + [""]:
+        join = lambda d: torch.cat([v for k, v in d.items() if k.startswith(name)])
+        bound = (1.5 * off(join(disturbed), join(want)) if checkpoints else 0.0) + (r * (8 * attentions) ** 0.5 if products else 0.0)
+        assert 0 < off(join(got), join(want)) <= bound, name
