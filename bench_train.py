@@ -133,6 +133,7 @@ def main():
         dist.init_process_group("nccl", device_id=dev)
 
     from mad_amd import ops
+    from mad_amd.buildid import library_build_id
     from mad_amd.config import load_cfg
     from mad_amd.model import build_model
     from mad_amd.synthetic import synthetic_faces
@@ -199,7 +200,7 @@ def main():
             "metric": f"training images/sec @{R}x{R}, DDP step (forward + backward + gradient all-reduce + AdamW + EMA)",
             "value": value, "unit": "images/s", "n_gpus": world, "steps": args.steps, "warmup": args.warmup,
             "ms_per_step": elapsed / args.steps * 1e3, "higher_is_better": True, "scaling": "weak",
-            "vs_baseline": None, "dtype": args.precision, "data": "synthetic",
+            "vs_baseline": None, "dtype": args.precision, "data": "synthetic", "build_id": library_build_id(),
             "config": {"workload": f"{os.path.basename(args.config)} training step (main.py loop body): {B * accum} images "
                                    f"per GPU per optimizer step (the config's {accum} micro-batches of {B}), run as "
                                    + (f"{accum} forward/backward passes of {B}" if passes > 1 else

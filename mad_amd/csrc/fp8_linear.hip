@@ -486,10 +486,10 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_fp8_tile_kernel(F8LinArgs
 }
 
 // Row form: x in bf16 with rows of whole 16-byte pieces and at most nine blocks, many rows.  A workgroup of four waves (eight from
-// five blocks on) rounds its 128 rows once, through LDS into the fragments' registers (and to memory, if the packed x is wanted), and then walks the columns in
-// strips of 64, whose weights all waves read from LDS; LDS-DMA brings the next strip while one is multiplied and stored.  Bound
-// by HBM: x is read once, where packing first writes and reads a byte more per element, in another launch.  65536 x 384 -> 384
-// 25 us (100 MB, 4.0 TB/s), 32768 x 256 -> 768 21 us.
+// five blocks on) rounds its 128 rows once, through LDS into the fragments' registers (and to memory, if the packed x is wanted),
+// and then walks the columns in strips of 64, whose weights all waves read from LDS; LDS-DMA brings the next strip while one is
+// multiplied and stored.  Bound by HBM: x is read once, where packing first writes and reads a byte more per element, in another
+// launch.  65536 x 384 -> 384 25 us (100 MB, 4.0 TB/s), 32768 x 256 -> 768 21 us.
 struct F8RowArgs {
     const bf16_t* x; const unsigned char* w; const unsigned char* ws; const float* bias; const bf16_t* residual; bf16_t* y;
     unsigned char* q; unsigned char* scale;        // the packed x, or null
@@ -762,8 +762,8 @@ template <int XK, int XF, typename TO> static int launch_linear(F8LinArgs a, hip
 // (40000 x 640 -> 640 43 / 44, 40000 x 1152 -> 384 54 / 54).
 static bool rows_form_ok(const void* x, int dtype, long rows, int K, int N) {
     const long tiles = (rows + 127) / 128, cus = f8_cus();
-    return dtype == MAD_BF16 && whole_pieces(x, dtype, K) && K <= 9 * F8_BLOCK && N <= 2048 && tiles >= cus && tiles <= LAUNCH_THREADS / 512 &&
-           (K <= 4 * F8_BLOCK || 4 * tiles >= 3 * ((tiles + cus - 1) / cus) * cus);
+    return dtype == MAD_BF16 && whole_pieces(x, dtype, K) && K <= 9 * F8_BLOCK && N <= 2048 && tiles >= cus &&
+           tiles <= LAUNCH_THREADS / 512 && (K <= 4 * F8_BLOCK || 4 * tiles >= 3 * ((tiles + cus - 1) / cus) * cus);
 }
 
 static F8RowArgs row_args(const void* x, const void* w, const void* ws, const float* bias, const void* residual, void* y, void* q,

@@ -238,8 +238,9 @@ __global__ __launch_bounds__(2 * BK) void wgrad_fp8_kernel(F8WgradArgs a) {
 // slots that only the lane that copied them reads (registers filled by ordinary loads had the compiler wait for them early), and are
 // widened into the next stage between the products of this one, so that one barrier per step remains.  Columns past the end read
 // what lies there, which only reaches results that are not stored; rows past the share are zeros (reads outside their buffer).
-// 8192 x 4096 -> 4096 247 us, 1110 TFLOP/s (a library's bf16 product of 8192^3: 1383).  Bound by LDS: a step of 64 rows reads and writes
-// about 270 KB of it for 1500 cycles of products.
+// 8192 x 4096 -> 4096 247 us, 1110 TFLOP/s (a library's bf16 product of 8192^3: 1383).  A step of 64 rows and 256 x 256 is 2048 cycles of
+// products and 295 KB through LDS (197 of them fragments, the rest copies in and x read and written to widen it), 2300 cycles at 128
+// bytes each.  It takes 4600 cycles, about their sum: neither pipe is the bound by itself, the two hardly overlap.
 template <int BN, int BK> struct F8Wg {
     static constexpr int ROWS = 64, DY = ROWS * BN * 2, STAGE = DY + ROWS * BK * 2;
     static constexpr int RAW = ROWS * BK, SCALES = 2 * ROWS * 8;          // x as it comes; scales of two steps, two dwords per row

@@ -76,8 +76,8 @@ class UNetTrainer:
     """Owns flat fp32 parameter / gradient / AdamW / EMA buffers of a ``DhariwalUNet`` and runs training steps.
 
     ``checkpoints="fp8"`` keeps the activations between forward and backward in 8 bits (one power-of-two scale per pixel and
-    128 channels) and restores them block by block: the forward's results do not change, the gradients are those of the
-    rounded activations.  The attention's q, k, v and output stay in the compute type: its scores are exponentiated, and its
+    128 channels) and restores them block by block: the forward's results do not change, the gradients are taken at the
+    rounded activations (the norms' mean and deviation stay those of the unrounded).  The attention's q, k, v and output stay in the compute type: its scores are exponentiated, and its
     tensors are few (32x32 pixels at most).  ``products="fp8"`` runs the qkv and output projections of the attention blocks, and
     their data gradients, on 8-bit operands (``ops.linear_fp8``); master weights, weight gradients and sums stay fp32."""
 
