@@ -107,7 +107,9 @@ __global__ __launch_bounds__(256) void gn_fp8_kernel(T* __restrict__ x, const fl
     const int b = blockIdx.y;
     // unsigned: a share that starts or ends behind the last pixel of the largest image (2^31 - 1 of them) does not fit an int
     const unsigned n = HW, per = (n + gridDim.x - 1) / gridDim.x;
-    const unsigned p0 = blockIdx.x * per, p1 = p0 + per < n ? p0 + per : n;
+    const unsigned p0 = blockIdx.x * per;
+    const int pixels = p0 >= n ? 0 : n - p0 < per ? n - p0 : per;
+    const size_t first = (size_t)b * n + p0;
     const int step = kb >= 16 ? 1 : 16 / kb;                  // pixels a workgroup covers per sweep
     for (int kbase = 0; kbase < kb; kbase += 16) {
         const int k = kbase + (kb >= 16 ? grp : grp % kb);
@@ -127,8 +129,8 @@ __global__ __launch_bounds__(256) void gn_fp8_kernel(T* __restrict__ x, const fl
                     a[i] = v.x; d[i] = v.y; a[i + 1] = v.z; d[i + 1] = v.w;
                 }
         }
-        for (unsigned p = p0 + row0; p < p1; p += step) {
-            const size_t row = (size_t)b * HW + p;
+        for (int p = row0; p < pixels; p += step) {
+            const size_t row = first + p;
             float f[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] = 0.0f;
