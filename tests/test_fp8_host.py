@@ -277,3 +277,16 @@ def test_launches_stay_below_the_threads_they_count():
     assert lib.mad_linear_fp8_needs_pack(P, L.MAD_BF16, 1 << 30, 8, 8) == 1
     _refused(lib.mad_linear_fp8(P, L.MAD_BF16, None, P, P, None, None, P, L.MAD_BF16, 1 << 28, 5, 16, None), "need more")
     _refused(lib.mad_linear_fp8(P, L.MAD_F32, None, P, P, None, None, P, L.MAD_F32, 1 << 20, 8, 1 << 15, None), "need more")
+
+
+def test_rounding_is_as_small_as_documented():
+    """e4m3: at most 2^-4 of an element down to 2^-13 of its block's largest, at most 2^-17 of the largest below, zero from 2^-19 on."""
+    from oracle import fp8_ref as R
+    g = torch.Generator().manual_seed(2)
+    for top in (1.0, 1.75, 1.7500002, 3.4e5, 2.0 ** -40):
+        ratio = torch.cat([2.0 ** (-21 * torch.rand(126, generator=g)), torch.tensor([2.0 ** -19])])
+        x = torch.cat([torch.tensor([top]), top * ratio]).float()
+        v = R.pack_rows(x[None])[0][0]
+        err, x = (v - x.double()).abs(), x.double()
+        near, far = x >= x[0] * 2.0 ** -13, x <= x[0] * 2.0 ** -19
+        assert bool((err <= torch.where(near, x * 2.0 ** -4, x[0] * 2.0 ** -17)).all()) and bool((v[far] == 0).all())
