@@ -194,3 +194,67 @@ def test_packed_bytes(dev, rows, c, dt, fmt):
     plain = lambda t: torch.where(t == 0x80, 0, t)[~nan]
     assert torch.equal(plain(got), plain(q)) and torch.equal(p.scale.cpu(), s)
     assert got.shape == (rows, (c + 15) // 16 * 16) and not bool(got[:, c:].any())
+
+
+# the widest tensors there are on either side: rows, K, N
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,k,n", [(3, 1 << 20, 17), (70, (1 << 20) - 5, 24), (2, 40, 1 << 20), (70, 24, (1 << 20) - 3), (2048, 1 << 20, 2048)])
+def test_widest_tensors(dev, rows, k, n, dt):
+    """Whole numbers again: sums of 2^20 products of at most 9 stay below 2^24, so they are exact in any order (in the reference too)."""
+    from mad_amd import ops
+    g = torch.Generator(device=dev).manual_seed(k % 1000 + n % 1000)
+    ints = lambda *s: torch.randint(-3, 4, s, generator=g, device=dev, dtype=torch.int8).to(torch.float32)
+    x, w, dy = ints(rows, k), ints(n, k), ints(rows, n)
+    pw = ops.pack_weight_fp8(w, transposed=True)
+    want = (x @ w.t()).to(dt)
+    y, x8 = ops.linear_fp8(x.to(dt), pw, save=True)
+    assert torch.equal(y, want) and torch.equal(ops.linear_fp8(x.to(dt), pw), want)
+    assert torch.equal(ops.unpack_fp8(x8).float(), x)
+    dx, dw, db = ops.linear_fp8_backward(dy.to(dt), x8, pw)
+    assert torch.equal(dx, (dy @ w).to(dt)) and torch.equal(dw, dy.t() @ x) and torch.equal(db, dy.sum(0))
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_norm_of_the_widest_tensor(dev, dt):
+    from mad_amd import ops
+    c = 1 << 20
+    g = torch.Generator(device=dev).manual_seed(3)
+    x = torch.randn((2, 1, 3, c), generator=g, device=dev).to(dt)
+    coef = torch.randn((2, c, 2), generator=g, device=dev)
+    y, p = ops.gn_apply_save(x, coef, act=True, drop_seed=9, drop_p=0.1)
+    ref = ops.pack_fp8(x)
+    assert torch.equal(y, ops.gn_apply(x, coef, act=True, drop_seed=9, drop_p=0.1))
+    assert torch.equal(p.q.view(torch.uint8), ref.q.view(torch.uint8)) and torch.equal(p.scale, ref.scale)
+    xr, yr = ops.gn_apply_restore(p, coef, act=True, drop_seed=9, drop_p=0.1)
+    assert torch.equal(xr, ops.unpack_fp8(ref)) and torch.equal(yr, ops.gn_apply(xr, coef, act=True, drop_seed=9, drop_p=0.1))
+
+
+@pytest.mark.parametrize("rows,k,n,dt", [(32768, 1152, 384, torch.bfloat16), (4100, 272, 1000, torch.bfloat16), (9000, 640, 521, torch.bfloat16),
+                                         (5000, 777, 900, torch.float32), (31, 4096, 512, torch.float32)])
+def test_large_forms_in_a_graph(dev, rows, k, n, dt):
+    """Captured once and replayed on new inputs, with eager work between the replays: the eager results, bit for bit."""
+    from mad_amd import ops
+
+    def step(x, w, bias, dy):
+        pw = ops.pack_weight_fp8(w, transposed=True)
+        y, x8 = ops.linear_fp8(x, pw, bias=bias, save=True)
+        return (y, ops.linear_fp8(x, pw, residual=y), *ops.linear_fp8_backward(dy, x8, pw))
+
+    def inputs(seed):
+        g = torch.Generator(device=dev).manual_seed(seed)
+        rand = lambda *s: torch.randn(s, generator=g, device=dev)
+        return rand(rows, k).to(dt), rand(n, k) / math.sqrt(k), rand(n), rand(rows, n).to(dt)
+    args = inputs(0)
+    step(*args)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*args)
+    for seed in (1, 2, 3):
+        fresh = inputs(seed)
+        for t, v in zip(args, fresh):
+            t.copy_(v)
+        graph.replay()
+        want = step(*fresh)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
